@@ -509,6 +509,104 @@ int ufpn_conv3x3_act(int dtype, const void* x, const void* w, const float* bias,
   return e == cudaSuccess ? UFPN_OK : cuda_fail(e, "conv3x3 launch");
 }
 
+namespace {
+// The checks that both directions of the group norm share; fills `lv`.
+int group_norm_levels(int dtype, int levels, const void* const* x, const void* const* grad,
+                      void* const* y, const float* const* weight, const float* const* bias,
+                      float* const* mean, float* const* rstd, int N, int C,
+                      const long long* pixels, int groups, int activation, const void* workspace,
+                      size_t workspace_bytes, bool backward, DType* dt, ufpn::GroupNormLevel* lv) {
+  if (!parse_dtype(dtype, dt)) return fail(UFPN_ERR_UNSUPPORTED, "unsupported dtype");
+  if (levels < 1 || levels > 8) return fail(UFPN_ERR_INVALID_ARG, "group norm takes 1 to 8 levels");
+  if (!x || !pixels || (!backward && !y) || (backward && (!grad || !mean || !rstd)) || (!mean != !rstd))
+    return fail(UFPN_ERR_INVALID_ARG, "NULL array");
+  if (N <= 0 || C <= 0 || groups <= 0) return fail(UFPN_ERR_INVALID_ARG, "sizes must be positive");
+  if (C % 8 != 0 || C > 2048)
+    return fail(UFPN_ERR_UNSUPPORTED, "C must be a multiple of 8, at most 2048");
+  if (C % groups != 0) return fail(UFPN_ERR_INVALID_ARG, "groups must divide C");
+  if (activation < 0 || activation > 3)
+    return fail(UFPN_ERR_INVALID_ARG, "activation must be 0 (none), 1 (ReLU), 2 (LeakyReLU) or 3 (Swish)");
+  std::memset(lv, 0, sizeof(*lv) * levels);
+  for (int l = 0; l < levels; ++l) {
+    if (pixels[l] <= 0) return fail(UFPN_ERR_INVALID_ARG, "sizes must be positive");
+    lv[l].x = x[l];
+    lv[l].grad = grad ? grad[l] : nullptr;
+    lv[l].y = y ? y[l] : nullptr;
+    lv[l].weight = weight ? weight[l] : nullptr;
+    lv[l].bias = bias ? bias[l] : nullptr;
+    lv[l].mean = mean ? mean[l] : nullptr;
+    lv[l].rstd = rstd ? rstd[l] : nullptr;
+    if (!lv[l].x || (!backward && !lv[l].y) || (backward && !lv[l].grad) || (mean && !lv[l].mean) ||
+        (rstd && !lv[l].rstd))
+      return fail(UFPN_ERR_INVALID_ARG, "NULL tensor pointer");
+    if (!ufpn::aligned16(lv[l].x) || !ufpn::aligned16(lv[l].y) || !ufpn::aligned16(lv[l].grad))
+      return fail(UFPN_ERR_ALIGNMENT, "tensors must be 16-byte aligned");
+  }
+  const size_t need = ufpn::group_norm_workspace_bytes(*dt, levels, N, C, pixels, groups, backward);
+  if (need == 0) return fail(UFPN_ERR_INVALID_ARG, "sizes out of range");
+  if (!workspace || workspace_bytes < need)
+    return fail(UFPN_ERR_INVALID_ARG, "workspace smaller than ufpn_group_norm_workspace");
+  if (!ufpn::aligned16(workspace)) return fail(UFPN_ERR_ALIGNMENT, "workspace must be 16-byte aligned");
+  return UFPN_OK;
+}
+}  // namespace
+
+size_t ufpn_group_norm_workspace(int dtype, int levels, int N, int C, const long long* pixels,
+                                 int groups, int backward) {
+  DType dt;
+  if (!parse_dtype(dtype, &dt) || !pixels) return 0;
+  try {
+    return ufpn::group_norm_workspace_bytes(dt, levels, N, C, pixels, groups, backward != 0);
+  } catch (...) {
+    return 0;
+  }
+}
+
+int ufpn_group_norm(int dtype, int levels, const void* const* x, void* const* y,
+                    const float* const* weight, const float* const* bias, float* const* mean,
+                    float* const* rstd, int N, int C, const long long* pixels, int groups, float eps,
+                    int activation, float alpha, void* workspace, size_t workspace_bytes,
+                    void* stream) {
+  return guarded([&] {
+    DType dt;
+    ufpn::GroupNormLevel lv[8];
+    if (!(eps >= 0.f)) return fail(UFPN_ERR_INVALID_ARG, "eps must not be negative");
+    const int rc = group_norm_levels(dtype, levels, x, nullptr, y, weight, bias, mean, rstd, N, C, pixels,
+                                     groups, activation, workspace, workspace_bytes, false, &dt, lv);
+    if (rc != UFPN_OK) return rc;
+    const cudaError_t e =
+        ufpn::launch_group_norm(dt, lv, levels, N, C, pixels, groups, eps, activation, alpha, false,
+                                workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? UFPN_OK : cuda_fail(e, "group norm");
+  });
+}
+
+int ufpn_group_norm_backward(int dtype, int levels, const void* const* x, const void* const* grad_y,
+                             void* const* grad_x, const float* const* weight,
+                             const float* const* bias, const float* const* mean,
+                             const float* const* rstd, float* const* grad_weight,
+                             float* const* grad_bias, int N, int C, const long long* pixels,
+                             int groups, int activation, float alpha, void* workspace,
+                             size_t workspace_bytes, void* stream) {
+  return guarded([&] {
+    DType dt;
+    ufpn::GroupNormLevel lv[8];
+    const int rc = group_norm_levels(dtype, levels, x, grad_y, grad_x, weight, bias,
+                                     const_cast<float* const*>(mean), const_cast<float* const*>(rstd),
+                                     N, C, pixels, groups, activation, workspace, workspace_bytes, true,
+                                     &dt, lv);
+    if (rc != UFPN_OK) return rc;
+    for (int l = 0; l < levels; ++l) {
+      lv[l].dweight = grad_weight ? grad_weight[l] : nullptr;
+      lv[l].dbias = grad_bias ? grad_bias[l] : nullptr;
+    }
+    const cudaError_t e =
+        ufpn::launch_group_norm(dt, lv, levels, N, C, pixels, groups, 0.f, activation, alpha, true,
+                                workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? UFPN_OK : cuda_fail(e, "group norm backward");
+  });
+}
+
 int ufpn_upsample_add(int dtype, int layout, const void* coarse, const void* lateral, void* out,
                       int N, int C, int Hc, int Wc, int H, int W, int align_corners,
                       void* stream) {

@@ -94,6 +94,14 @@ SIGNATURES = {
     "ufpn_fold_batch_norm": (
         c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_float, c_int, c_longlong,
                 c_void_p, c_void_p]),
+    # (the pointer-array arguments of the group norm are ctypes arrays, passed by address)
+    "ufpn_group_norm": (
+        c_int, [c_int, c_int] + [c_void_p] * 6 + [c_int, c_int, c_void_p, c_int, c_float, c_int, c_float,
+                                                  c_void_p, c_size_t, c_void_p]),
+    "ufpn_group_norm_backward": (
+        c_int, [c_int, c_int] + [c_void_p] * 9 + [c_int, c_int, c_void_p, c_int, c_int, c_float,
+                                                  c_void_p, c_size_t, c_void_p]),
+    "ufpn_group_norm_workspace": (c_size_t, [c_int, c_int, c_int, c_int, c_void_p, c_int, c_int]),
     "ufpn_upsample_add": (
         c_int, [c_int, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
                 c_void_p]),

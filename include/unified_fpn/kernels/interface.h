@@ -105,6 +105,25 @@ cudaError_t launch_fp32_conv3x3(const float* x, const float* w, const float* bia
                                 int N, int Cin, int Cout, int H, int W, cudaStream_t s,
                                 int act = 0, float act_alpha = 0.01f);
 
+// ---- group norm with an activation (groupnorm.cu), NHWC maps of one batch and channel count
+struct GroupNormLevel {
+  const void* x;
+  const void* grad;     // backward: gradient of the output
+  void* y;              // forward: the output (may be x); backward: grad_input (null: none)
+  const float* weight;  // [C], null = 1
+  const float* bias;    // [C], null = 0
+  float* mean;          // [N][groups]: written forward (null: not wanted), read backward
+  float* rstd;
+  float* dweight;  // backward, [C], null: not wanted; a level after the first with neither adds
+  float* dbias;    // its sums to the level before it (weights shared by several levels)
+};
+// Scratch of one call (0: sizes out of range).  pixels[l] = H * W of level l.
+size_t group_norm_workspace_bytes(DType dt, int levels, int N, int C, const long long* pixels,
+                                  int groups, bool backward);
+cudaError_t launch_group_norm(DType dt, const GroupNormLevel* lv, int levels, int N, int C,
+                              const long long* pixels, int groups, float eps, int act, float alpha,
+                              bool backward, void* ws, size_t ws_bytes, cudaStream_t s);
+
 // ---- tensor-core kernels (tc_kernels.cu)
 // Spatial tiling of the 3x3 implicit GEMM: tile_w * tile_h = 128 output pixels.
 struct Conv3x3Tiling {

@@ -276,6 +276,38 @@ int ufpn_conv3x3_act(int dtype, const void* x, const void* w, const float* bias,
                      void* p6, int N, int H, int W, int tile_w, int activation, float alpha,
                      void* stream);
 
+/* Group norm with an activation on channels-last maps, for `levels` (1..8) maps of one batch
+ * and channel count in one call: per image and group of C / groups adjacent channels, xhat =
+ * (x - mean) * rstd with rstd = 1 / sqrt(var + eps) and the biased variance, y = act(xhat *
+ * weight[c] + bias[c]) (activation as ufpn_conv3x3_act).  dtype F32, F16 or BF16, NHWC; C a
+ * multiple of 8 and of groups, at most 2048; statistics in fp32.  No reference counterpart
+ * (its engine had BatchNorm with frozen statistics only, fpn_compute_kernels.cu:342-371).
+ *   x, y: [levels] maps, 16-byte aligned; y[l] may be x[l].
+ *   weight, bias: [levels] fp32 [C] device vectors; the array or an entry may be NULL (1, 0).
+ *   mean, rstd: [levels] fp32 [N][groups] outputs for the backward; the arrays may be NULL.
+ *   pixels: [levels] H * W.
+ *   workspace: ufpn_group_norm_workspace(...) bytes of device memory, 16-byte aligned, used by
+ *   this call alone until it has run. */
+int ufpn_group_norm(int dtype, int levels, const void* const* x, void* const* y,
+                    const float* const* weight, const float* const* bias, float* const* mean,
+                    float* const* rstd, int N, int C, const long long* pixels, int groups, float eps,
+                    int activation, float alpha, void* workspace, size_t workspace_bytes,
+                    void* stream);
+/* Its gradients, with mean and rstd of the forward: grad_x[l] (entry or array NULL: none), and
+ * fp32 [C] sums grad_weight[l], grad_bias[l] over images and pixels.  A level after the first
+ * whose grad_weight and grad_bias entries are both NULL adds its sums to the level before it (weights
+ * shared by the levels); arrays NULL: no weight gradients.  Deterministic. */
+int ufpn_group_norm_backward(int dtype, int levels, const void* const* x, const void* const* grad_y,
+                             void* const* grad_x, const float* const* weight,
+                             const float* const* bias, const float* const* mean,
+                             const float* const* rstd, float* const* grad_weight,
+                             float* const* grad_bias, int N, int C, const long long* pixels,
+                             int groups, int activation, float alpha, void* workspace,
+                             size_t workspace_bytes, void* stream);
+/* Workspace bytes of either (0 for sizes that they refuse). */
+size_t ufpn_group_norm_workspace(int dtype, int levels, int N, int C, const long long* pixels,
+                                 int groups, int backward);
+
 /* out = lateral + bilinear_upsample(coarse -> H x W); lateral may be NULL (pure upsample).
  * Replaces launch_upsample_and_add (fpn_engine.cu:274-313) = bilinear_upsample_kernel +
  * element_wise_add_kernel (fpn_compute_kernels.cu:232-275, 397-409). */
