@@ -931,6 +931,92 @@ int conv3x3_backward(int dtype, const void* x, const void* w, const void* w_f,
   return UFPN_OK;
 }
 
+namespace {
+// The checks of the adapter calls on sizes; fills `p`.
+int adapter_problem(int dtype, int N, int Cin, int H, int W, int rank, int adapters, const int* index,
+                    const float* scales, float scale, ufpn::AdapterProblem* p) {
+  if (!parse_16bit(dtype, &p->dtype)) return fail(UFPN_ERR_UNSUPPORTED, "adapters take bf16 or fp16");
+  if (N <= 0 || Cin <= 0 || H <= 0 || W <= 0 || adapters <= 0)
+    return fail(UFPN_ERR_INVALID_ARG, "sizes must be positive");
+  if (Cin % 8 != 0 || Cin > 2048)
+    return fail(UFPN_ERR_UNSUPPORTED, "Cin must be a multiple of 8, at most 2048");
+  if (rank < 1 || rank > 64) return fail(UFPN_ERR_UNSUPPORTED, "adapters have rank 1 to 64");
+  if (adapters > 65535) return fail(UFPN_ERR_UNSUPPORTED, "at most 65535 adapters");
+  if (static_cast<long long>(H) * W >= (1LL << 31) - 256)
+    return fail(UFPN_ERR_UNSUPPORTED, "map too large");
+  p->N = N;
+  p->Cin = Cin;
+  p->H = H;
+  p->W = W;
+  p->rank = rank;
+  p->adapters = adapters;
+  p->index = index;
+  p->scales = scales;
+  p->scale = scale;
+  return UFPN_OK;
+}
+}  // namespace
+
+int ufpn_lateral_adapters(int dtype, const void* x, const void* w, const float* bias,
+                          const void* down, const void* up, const int* index, const float* scales,
+                          float scale, const void* coarse, void* out, void* hidden, int N, int Cin,
+                          int H, int W, int rank, int adapters, int Hc, int Wc, void* stream) {
+  return guarded([&] {
+    ufpn::AdapterProblem p;
+    const int rc = adapter_problem(dtype, N, Cin, H, W, rank, adapters, index, scales, scale, &p);
+    if (rc != UFPN_OK) return rc;
+    if (!x || !w || !bias || !down || !up || !index || !out)
+      return fail(UFPN_ERR_INVALID_ARG, "NULL tensor pointer");
+    if (coarse && (Hc <= 0 || Wc <= 0 || Hc > H || Wc > W))
+      return fail(UFPN_ERR_INVALID_ARG, "coarse map must be non-empty and not larger than output");
+    for (const void* q : {x, w, static_cast<const void*>(bias), down, up, coarse,
+                          static_cast<const void*>(out), static_cast<const void*>(hidden)})
+      if (!ufpn::aligned16(q)) return fail(UFPN_ERR_ALIGNMENT, "tensors must be 16-byte aligned");
+    int* status = device_status_word();
+    if (!status) return fail(UFPN_ERR_CUDA, "could not allocate the device status word");
+    const cudaError_t e = ufpn::launch_lateral_adapters(p, x, w, bias, down, up, coarse, Hc, Wc, out,
+                                                        hidden, status, static_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? UFPN_OK : cuda_fail(e, "lateral adapters");
+  });
+}
+
+size_t ufpn_lateral_adapters_workspace(int dtype, int N, int Cin, int H, int W, int rank,
+                                       int adapters, int has_w_t, int need_grad_x) {
+  ufpn::AdapterProblem p;
+  if (adapter_problem(dtype, N, Cin, H, W, rank, adapters, nullptr, nullptr, 1.f, &p) != UFPN_OK) return 0;
+  return ufpn::lateral_adapters_workspace_bytes(p, has_w_t != 0, need_grad_x != 0);
+}
+
+int ufpn_lateral_adapters_backward(int dtype, const void* x, const void* w, const void* w_t,
+                                   const void* grad_out, const void* down, const void* up,
+                                   const int* index, const float* scales, float scale,
+                                   const void* hidden, void* grad_x, float* grad_down,
+                                   float* grad_up, int N, int Cin, int H, int W, int rank,
+                                   int adapters, void* workspace, size_t workspace_bytes,
+                                   void* stream) {
+  return guarded([&] {
+    ufpn::AdapterProblem p;
+    const int rc = adapter_problem(dtype, N, Cin, H, W, rank, adapters, index, scales, scale, &p);
+    if (rc != UFPN_OK) return rc;
+    if (!x || !grad_out || !down || !up || !index || !hidden || !grad_down || !grad_up ||
+        (grad_x && !w && !w_t))
+      return fail(UFPN_ERR_INVALID_ARG, "NULL tensor pointer");
+    for (const void* q : {x, w, w_t, grad_out, down, up, hidden, static_cast<const void*>(grad_x)})
+      if (!ufpn::aligned16(q)) return fail(UFPN_ERR_ALIGNMENT, "tensors must be 16-byte aligned");
+    if (!workspace ||
+        workspace_bytes < ufpn::lateral_adapters_workspace_bytes(p, w_t != nullptr, grad_x != nullptr))
+      return fail(UFPN_ERR_INVALID_ARG, "workspace smaller than ufpn_lateral_adapters_workspace");
+    if ((reinterpret_cast<uintptr_t>(workspace) & 255u) != 0)
+      return fail(UFPN_ERR_ALIGNMENT, "workspace must be 256-byte aligned");
+    int* status = device_status_word();
+    if (!status) return fail(UFPN_ERR_CUDA, "could not allocate the device status word");
+    const cudaError_t e = ufpn::launch_lateral_adapters_backward(
+        p, x, w, w_t, grad_out, down, up, hidden, grad_x, grad_down, grad_up, workspace,
+        workspace_bytes, status, static_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? UFPN_OK : cuda_fail(e, "lateral adapters backward");
+  });
+}
+
 int ufpn_lateral_conv_backward(int dtype, const void* x, const void* w, const void* grad_out,
                                void* grad_x, float* grad_w, float* grad_b, int N, int Cin, int H,
                                int W, void* stream) {

@@ -422,4 +422,30 @@ int sm_count();
 // L2 size of the current device in bytes (cached per device).
 long long l2_bytes();
 
+// ---- lateral 1x1 convs with a low-rank adapter per image (adapters.cu); bf16 / fp16, NHWC,
+// Cin a multiple of 8 and at most 2048, 256 outputs, rank 1..64.
+struct AdapterProblem {
+  DType dtype;
+  int N, Cin, H, W;
+  int rank, adapters;
+  const int* index;     // [N] device: the image's adapter, outside 0 .. adapters - 1: none
+  const float* scales;  // [adapters] device, or null (1)
+  float scale;          // times scales[a]
+};
+// out = x w^T + bias + h up[a]^T [+ bilinear(coarse)], h = scale x down[a]^T; hidden (optional):
+// [pixels][2][rank padded to 8] 16-bit, h as hi + lo.
+cudaError_t launch_lateral_adapters(const AdapterProblem& p, const void* x, const void* w,
+                                    const float* bias, const void* down, const void* up,
+                                    const void* coarse, int Hc, int Wc, void* out, void* hidden,
+                                    int* status, cudaStream_t s);
+// Scratch of the backward (0: sizes out of range); need_dx: dx is asked for, has_w_t: with w_t.
+size_t lateral_adapters_workspace_bytes(const AdapterProblem& p, bool has_w_t, bool need_dx);
+// dx (null: none), ddown [adapters][rank][Cin], dup [adapters][256][rank] (fp32).  w [256][Cin], or
+// w_t [ceil(Cin / 256) * 256][256]; neither without dx.
+cudaError_t launch_lateral_adapters_backward(const AdapterProblem& p, const void* x, const void* w,
+                                             const void* w_t, const void* dy, const void* down,
+                                             const void* up, const void* hidden, void* dx, float* ddown,
+                                             float* dup, void* ws, size_t ws_bytes, int* status,
+                                             cudaStream_t s);
+
 }  // namespace ufpn

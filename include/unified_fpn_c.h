@@ -276,6 +276,37 @@ int ufpn_conv3x3_act(int dtype, const void* x, const void* w, const float* bias,
                      void* p6, int N, int H, int W, int tile_w, int activation, float alpha,
                      void* stream);
 
+/* The 16-bit lateral (NHWC, Cout = 256) with a low-rank adapter per image, many adapters in one
+ * batch: image n carries adapter a = index[n] (any value outside 0 .. adapters - 1: none), and
+ *   h = scale * scales[a] * conv1x1(x, down[a]);  out = conv1x1(x, w) + bias + conv1x1(h, up[a])
+ *   [+ bilinear(coarse)].
+ * dtype F16/BF16 (x, w, down, up, coarse, out); Cin a multiple of 8, at most 2048; rank 1..64;
+ * every tensor 16-byte aligned.  No reference counterpart.
+ *   down [adapters][rank][Cin], up [adapters][256][rank], index int32 [N] on the device, scales fp32
+ *   [adapters] on the device or NULL (1); coarse as ufpn_lateral_conv, or NULL.
+ *   hidden: NULL, or [N * H * W][2][rank rounded up to 8] elements that receive h for the backward
+ *   (the 16-bit value nearest to h, then the nearest to what is left; zeros without an adapter). */
+int ufpn_lateral_adapters(int dtype, const void* x, const void* w, const float* bias,
+                          const void* down, const void* up, const int* index, const float* scales,
+                          float scale, const void* coarse, void* out, void* hidden, int N, int Cin,
+                          int H, int W, int rank, int adapters, int Hc, int Wc, void* stream);
+/* Its gradients but for w, bias (ufpn_lateral_conv_backward) and coarse (ufpn_upsample_add_backward):
+ * grad_x (NULL: none), grad_down [adapters][rank][Cin] and grad_up [adapters][256][rank] in fp32 (zeros
+ * for an adapter without images).  hidden: from the forward.  For grad_x the weights as w
+ * [256][Cin] or, transposed, w_t [ceil(Cin / 256) * 256][256] (ufpn_prepare_neck_weights).
+ * workspace: ufpn_lateral_adapters_workspace(..., w_t != NULL, grad_x != NULL) bytes of device
+ * memory, 256-byte aligned, used by this call alone until it has run.  Deterministic. */
+int ufpn_lateral_adapters_backward(int dtype, const void* x, const void* w, const void* w_t,
+                                   const void* grad_out, const void* down, const void* up,
+                                   const int* index, const float* scales, float scale,
+                                   const void* hidden, void* grad_x, float* grad_down,
+                                   float* grad_up, int N, int Cin, int H, int W, int rank,
+                                   int adapters, void* workspace, size_t workspace_bytes,
+                                   void* stream);
+/* (0 for sizes that the call refuses) */
+size_t ufpn_lateral_adapters_workspace(int dtype, int N, int Cin, int H, int W, int rank,
+                                       int adapters, int has_w_t, int need_grad_x);
+
 /* Group norm with an activation on channels-last maps, for `levels` (1..8) maps of one batch
  * and channel count in one call: per image and group of C / groups adjacent channels, xhat =
  * (x - mean) * rstd with rstd = 1 / sqrt(var + eps) and the biased variance, y = act(xhat *
