@@ -574,9 +574,11 @@ int ufpn_group_norm(int dtype, int levels, const void* const* x, void* const* y,
     const int rc = group_norm_levels(dtype, levels, x, nullptr, y, weight, bias, mean, rstd, N, C, pixels,
                                      groups, activation, workspace, workspace_bytes, false, &dt, lv);
     if (rc != UFPN_OK) return rc;
+    int* status = device_status_word();
+    if (!status) return fail(UFPN_ERR_CUDA, "could not allocate the device status word");
     const cudaError_t e =
         ufpn::launch_group_norm(dt, lv, levels, N, C, pixels, groups, eps, activation, alpha, false,
-                                workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
+                                workspace, workspace_bytes, status, static_cast<cudaStream_t>(stream));
     return e == cudaSuccess ? UFPN_OK : cuda_fail(e, "group norm");
   });
 }
@@ -600,9 +602,11 @@ int ufpn_group_norm_backward(int dtype, int levels, const void* const* x, const 
       lv[l].dweight = grad_weight ? grad_weight[l] : nullptr;
       lv[l].dbias = grad_bias ? grad_bias[l] : nullptr;
     }
+    int* status = device_status_word();
+    if (!status) return fail(UFPN_ERR_CUDA, "could not allocate the device status word");
     const cudaError_t e =
         ufpn::launch_group_norm(dt, lv, levels, N, C, pixels, groups, 0.f, activation, alpha, true,
-                                workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
+                                workspace, workspace_bytes, status, static_cast<cudaStream_t>(stream));
     return e == cudaSuccess ? UFPN_OK : cuda_fail(e, "group norm backward");
   });
 }

@@ -8,38 +8,122 @@
 //   dbias[c] = sum dz;  dweight[c] = sum dz * xhat   (over images and pixels)
 //   dx = rstd * (w dz - mean_g(w dz) - xhat * mean_g(w dz xhat))
 //
-// All statistics and sums are fp32.  The variance never comes from a difference of raw moments:
-// every thread takes the mean of a few pixels in registers, the squares about that mean, and
-// merges such (count, mean, M2) triples,
+// All statistics and sums are fp32.  The variance never comes from a difference of raw moments: a
+// thread sums its pixels relative to its first one, so that what it subtracts is of the size of the
+// spread, and such (count, mean, M2) triples merge as
 //   M2_ab = M2_a + M2_b + (mean_b - mean_a)^2 n_a n_b / (n_a + n_b),
-// and fp32 values are taken relative to the group's first value of the image (the pivot), so that
-// the means in between are not rounded at the height of a mean far above the spread.  (16-bit
-// values have at most 11 bits: their spread is never that far below their mean.)  Every sum has a
-// fixed order (no atomics): the same inputs give the same bits.
+// their means taken relative to the group's first value in the image (the pivot): a mean far above
+// the spread costs no digits in between.  Every sum has a fixed order (no atomics): the same inputs
+// give the same bits.
 //
-// The kernels move bytes: two passes over the maps (statistics, then apply), each a stream of
-// 16-byte loads, the batch cut into runs of images whose maps stay in the 126 MB L2 cache, so
-// that the second pass reads there instead of HBM.
+// The kernel moves bytes.  The batch is cut into segments whose maps stay in the 126 MB L2 cache;
+// in one cooperative launch of a block per SM, eight warps of a block take the statistics of the
+// segments one after the other from HBM while eight others apply the norm to the segment before,
+// which they read again from L2: HBM reads and writes overlap, and the second reading costs no
+// HBM traffic.  A segment's blocks count themselves into a device counter when their sums are
+// written; four more warps wait for the count and merge the sums for the apply warps, while these
+// still work on the segment before.  Every warp keeps bulk copies in flight into a ring of its own
+// in shared memory and waits for no other warp (a ring shared by eight warps cost about 800 cycles
+// a 16 KB piece), and the arithmetic runs on pairs of channels (add / mul / fma on f32x2).
 #include "kernels.h"
 #include "ptx.cuh"
 #include "vec16.cuh"
 
 #include <algorithm>
+#include <atomic>
 #include <cstring>
-#include <vector>
 
 namespace ufpn {
 
 namespace {
 
-constexpr int kGnThreads = 512;
-constexpr int kGnBatch = 8;      // pixels per thread and step: 16-byte loads in flight
-constexpr int kGnMaxRuns = 8;    // runs (images of one level) per launch
-constexpr int kGnMaxChannels = 2048;  // a thread keeps one vector of a pixel: C / V <= 512
+constexpr int kGnWarps = 8;            // statistics warps, and as many apply warps
+constexpr int kGnThreads = 32 * kGnWarps;
+constexpr int kGnMergeThreads = 128;
+constexpr int kGnMaxRuns = 8;         // runs (images of one level) per segment
+constexpr int kGnMaxChannels = 2048;  // 8 per thread of a half
+constexpr int kGnStage = 4096;         // one copy of a warp; backward: half of it x, half dy
+constexpr int kGnK = 8;                // pixels read before their arithmetic
+constexpr int kGnStatsStages = 3, kGnApplyStages = 2;  // per warp
+constexpr int kDevTimeoutNorm = 0x108;
 
 enum : int { kGnNone = 0, kGnRelu = 1, kGnLeaky = 2, kGnSwish = 3 };
 
-// One run: consecutive images of one level, each cut into `chunks` runs of `per` pixels.
+// Pairs of fp32 values, one instruction for both.
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+      "add.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+      "mul.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y, z, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+      "mov.b64 z, {%6, %7};\n\tfma.rn.f32x2 w, x, y, z;\n\tmov.b64 {%0, %1}, w;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {  // (fmaxf drops a NaN)
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+
+// Eight adjacent channels of a pixel: one 16-byte vector of a 16-bit type, two of fp32.
+template <typename T>
+struct Gn8 {
+  static constexpr int kVecs = static_cast<int>(sizeof(T)) / 2;
+  uint4 u[kVecs];
+  __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+    for (int i = 0; i < kVecs; ++i) u[i] = *(reinterpret_cast<const uint4*>(p) + i);
+  }
+  __device__ __forceinline__ void load_shared(uint32_t p) {
+#pragma unroll
+    for (int i = 0; i < kVecs; ++i)
+      asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                   : "=r"(u[i].x), "=r"(u[i].y), "=r"(u[i].z), "=r"(u[i].w)
+                   : "r"(p + 16 * i));
+  }
+  __device__ __forceinline__ void get(float2 (&f)[4]) const {  // as pairs
+#pragma unroll
+    for (int i = 0; i < kVecs; ++i) {
+      constexpr int V = Vec16<T>::V;
+      float h[V];
+      Vec16<T>::unpack(u[i], h);
+#pragma unroll
+      for (int e = 0; e < V / 2; ++e) f[i * (V / 2) + e] = make_float2(h[2 * e], h[2 * e + 1]);
+    }
+  }
+};
+template <typename T>
+__device__ __forceinline__ void gn_put(T* p, const float2 (&f)[4]) {
+#pragma unroll
+  for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) {
+    constexpr int V = Vec16<T>::V;
+    float h[V];
+#pragma unroll
+    for (int e = 0; e < V / 2; ++e) {
+      h[2 * e] = f[i * (V / 2) + e].x;
+      h[2 * e + 1] = f[i * (V / 2) + e].y;
+    }
+    *(reinterpret_cast<uint4*>(p) + i) = Vec16<T>::pack(h);
+  }
+}
+
+// One level: its images, each cut into `chunks` runs of `per` pixels.
 struct GnRun {
   const void* x;
   const void* g;  // backward: grad_output
@@ -49,477 +133,948 @@ struct GnRun {
   float* mean;     // [N][groups]: written forward (null: not wanted), read backward
   float* rstd;
   long long pixels;  // of one image
-  long long per;
-  int n0, chunks;
-  int first_block;  // block of image n0, chunk 0
-  int row0;         // its row of partial results; a run's rows are [image][chunk]
+  int per, chunks;
+  int first_block;  // in its segment: block of the segment's first image, chunk 0
+  int row0;         // partial results of (image n, chunk c): row row0 + n * chunks + c
+};
+// Segments: either the images of several small levels together (one segment), or one level in
+// segments of `images` images.
+struct GnPhase {
+  int run0, runs;
+  int images, segments;
 };
 struct GnArgs {
   GnRun run[kGnMaxRuns];
-  int runs;
-  int C, groups, cg;
+  GnPhase phase[kGnMaxRuns];
+  int phases;
+  int N, C, groups, cg;
   int act;
+  int apply;  // 0: only the sums (backward without dx)
   float alpha, eps;
-  float2* part;   // [row][groups]: (mean, M2) forward, (sum w dz, sum w dz xhat) backward
+  float2* part;   // [row][groups]: (mean - pivot, M2) forward, (sum w dz, sum w dz xhat) backward
+  float* pivot;   // forward: [row of chunk 0][groups]
   float* part_c;  // backward: [row][2][C]: sum dz, sum dz xhat
-  float* pivot;   // fp32 forward: [row of chunk 0][groups]
+  unsigned* done;  // [segments] blocks whose sums are written, zero at launch
+  int* status;     // device status word
 };
-template <typename T>
-constexpr bool kGnPivot = sizeof(T) == 4;
 
-// exp and the division of the sigmoid: the fast forms (relative error about 2^-21) for 16-bit
-// maps, whose results are rounded to 2^-9 or 2^-12 anyway; the accurate ones for fp32.
+// 1 / (1 + exp(-z)) of a pair.  16-bit maps, whose results are rounded to 2^-9 or 2^-12, take the
+// fast exp and one fast reciprocal for both, 1 / a = b / (a b) (relative error about 2^-20; the
+// special-function unit sets their pace); exp(-z) is held below 2^60 for that, so z < -41 has a
+// sigmoid of 2^-60.  fp32 maps take the accurate exp and division.
 template <typename T>
-__device__ __forceinline__ float gn_sigmoid(float z) {
-  if constexpr (sizeof(T) == 2)
-    return __fdividef(1.f, 1.f + __expf(-z));
-  else
-    return 1.f / (1.f + expf(-z));
+__device__ __forceinline__ float2 gn_sigmoid(float2 z) {
+  if constexpr (sizeof(T) == 2) {
+    const float a = 1.f + fminf(__expf(-z.x), 1.152921504606846976e18f);
+    const float b = 1.f + fminf(__expf(-z.y), 1.152921504606846976e18f);
+    // (fminf returns the bound for a NaN, which so stays out of the other channel; z itself
+    // carries it on)
+    const float r = __fdividef(1.f, a * b);
+    return make_float2(b * r, a * r);
+  } else {
+    return make_float2(1.f / (1.f + expf(-z.x)), 1.f / (1.f + expf(-z.y)));
+  }
 }
-template <typename T>
-__device__ __forceinline__ float gn_act(float z, int act, float alpha) {
-  if (act == kGnRelu) return fmaxf(z, 0.f);
-  if (act == kGnLeaky) return z > 0.f ? z : alpha * z;
-  if (act == kGnSwish) return z * gn_sigmoid<T>(z);
+template <typename T, int kAct>
+__device__ __forceinline__ float2 gn_act(float2 z, float alpha) {
+  if constexpr (kAct == kGnRelu) return make_float2(max_nan(z.x, 0.f), max_nan(z.y, 0.f));
+  if constexpr (kAct == kGnLeaky)
+    return make_float2(z.x > 0.f ? z.x : alpha * z.x, z.y > 0.f ? z.y : alpha * z.y);
+  if constexpr (kAct == kGnSwish) return mul2(z, gn_sigmoid<T>(z));
   return z;
 }
-template <typename T>
-__device__ __forceinline__ float gn_act_grad(float z, int act, float alpha) {
-  if (act == kGnRelu) return z > 0.f ? 1.f : 0.f;
-  if (act == kGnLeaky) return z > 0.f ? 1.f : alpha;
-  if (act == kGnSwish) {
-    const float q = gn_sigmoid<T>(z);
-    return q * fmaf(z, 1.f - q, 1.f);
+// dy * act'(z)
+template <typename T, int kAct>
+__device__ __forceinline__ float2 gn_act_grad(float2 dy, float2 z, float alpha) {
+  if constexpr (kAct == kGnRelu) return make_float2(z.x > 0.f ? dy.x : 0.f, z.y > 0.f ? dy.y : 0.f);
+  if constexpr (kAct == kGnLeaky)
+    return make_float2(z.x > 0.f ? dy.x : alpha * dy.x, z.y > 0.f ? dy.y : alpha * dy.y);
+  if constexpr (kAct == kGnSwish) {
+    const float2 q = gn_sigmoid<T>(z);
+    return mul2(dy, mul2(q, fma2(z, fma2(q, both(-1.f), both(1.f)), both(1.f))));
   }
-  return 1.f;
-}
-// z from x in the one form that the forward and the backward share, each step rounded on its
-// own, so that both take the same side of an activation's kink.
-__device__ __forceinline__ float gn_xhat(float x, float mean, float rstd) {
-  return __fmul_rn(__fsub_rn(x, mean), rstd);
+  return dy;
 }
 
-// Which run, image, chunk and pixel range this block has.
-struct GnPlace {
-  int run, n, chunk;
-  long long p0, p1;
+struct GnSmem {
+  uint8_t stats_ring[kGnWarps][kGnStatsStages * kGnStage];
+  uint8_t apply_ring[kGnWarps][kGnApplyStages * kGnStage];
+  // statistics: the image's first pixel; a chunk's pixel lanes [lane][C] and their pixel counts
+  float first[kGnMaxChannels];
+  float a[kGnMaxChannels], b[kGnMaxChannels], d[kGnMaxChannels];
+  float cnt[kGnThreads];  // [warp][pixel lane of the warp]
+  // merge: per thread, then by group (mean, rstd; backward: the means of w dz and w dz xhat)
+  float m1[kGnMergeThreads], m2[kGnMergeThreads], m3[kGnMergeThreads];
+  float g1[kGnMaxChannels], g2[kGnMaxChannels];
+  uint64_t stats_full[kGnWarps][kGnStatsStages], apply_full[kGnWarps][kGnApplyStages];
+  uint64_t ready, taken;  // g1 and g2: written; in the apply warps' registers
+  int abort_flag;
+  int applied;  // the apply warps have finished every segment before this one
+  int go;
 };
-__device__ __forceinline__ GnPlace gn_place(const GnArgs& a) {
-  GnPlace p;
-  p.run = 0;
-  while (p.run + 1 < a.runs && static_cast<int>(blockIdx.x) >= a.run[p.run + 1].first_block) ++p.run;
-  const GnRun& r = a.run[p.run];
-  const int b = static_cast<int>(blockIdx.x) - r.first_block;
-  const int i = b / r.chunks;
-  p.chunk = b - i * r.chunks;
-  p.n = r.n0 + i;
-  p.p0 = p.chunk * r.per;
-  p.p1 = min(r.pixels, p.p0 + r.per);
-  return p;
+
+// What a warp and its threads have of a chunk.  The C / 8 vectors of a pixel are cut into `cbs`
+// blocks of at most 32; warp w has block w % cbs, and of the chunk's pixels every (8 / cbs)-th batch
+// of `sp`; a thread has one vector of every wl-th pixel of a batch.
+struct GnLanes {
+  int cbs, vb, nw, wl, sp;
+  int wi;         // the warp's first batch
+  int v, pl;      // vector of the pixel, pixel lane within the warp
+  int v0, nv;     // the warp's vectors
+  bool works, active;
+  __device__ __forceinline__ GnLanes(int C, int esz, int warp, int lane, int capacity) {
+    const int vc = C >> 3;
+    cbs = (vc + 31) / 32;
+    vb = (vc + cbs - 1) / cbs;
+    nw = kGnWarps / cbs;
+    wl = 32 / vb;
+    sp = capacity / (vb * 8 * esz * wl) * wl;
+    works = warp < cbs * nw;
+    const int cb = warp % cbs;
+    wi = warp / cbs;
+    v0 = cb * vb;
+    nv = min(vb, vc - v0);
+    pl = lane / vb;
+    v = v0 + lane - pl * vb;
+    active = works && pl < wl && v < v0 + nv;
+  }
+  // this thread's pixels of a chunk of p1
+  __device__ __forceinline__ int pixels(int p1) const {
+    const int round = nw * sp, full = p1 / round, rest = p1 - full * round - wi * sp;
+    const int part = min(max(rest, 0), sp);  // of the last round
+    return full * (sp / wl) + (part > pl ? (part - pl + wl - 1) / wl : 0);
+  }
+  __device__ __forceinline__ int lanes() const { return nw * wl; }  // pixel lanes of a channel
+  __device__ __forceinline__ int lane_index() const { return wi * wl + pl; }
+  // the count of pixel lane l of channel c (as written to `cnt`)
+  __device__ __forceinline__ int count_slot(int c, int l) const {
+    const int i = l / wl;
+    return ((c >> 3) / vb + cbs * i) * 32 + l - i * wl;
+  }
+};
+
+// A chunk of the work: level, image and pixels.
+struct GnPlace {
+  int run, n, chunk, row;
+  int p1;       // pixels of the chunk
+  size_t base;  // element of the chunk's first pixel
+  __device__ __forceinline__ int row_of_chunk0() const { return row - chunk; }
+};
+// This block's chunks in order, over all segments.
+struct GnCursor {
+  int phase = 0, seg = 0, block, blocks;
+  int k = 0;  // segment index over all phases
+  __device__ __forceinline__ explicit GnCursor(const GnArgs& a) {
+    block = static_cast<int>(blockIdx.x);
+    blocks = count(a);
+    settle(a);
+  }
+  __device__ __forceinline__ bool more(const GnArgs& a) const { return phase < a.phases; }
+  __device__ __forceinline__ void next(const GnArgs& a) {
+    block += static_cast<int>(gridDim.x);
+    settle(a);
+  }
+  __device__ __forceinline__ GnPlace place(const GnArgs& a) const {
+    const GnPhase& ph = a.phase[phase];
+    GnPlace p;
+    p.run = ph.run0;
+    while (p.run + 1 < ph.run0 + ph.runs && block >= a.run[p.run + 1].first_block) ++p.run;
+    const GnRun& r = a.run[p.run];
+    const int b = block - r.first_block;
+    const int img = b / r.chunks;
+    p.chunk = b - img * r.chunks;
+    p.n = seg * ph.images + img;
+    p.row = r.row0 + p.n * r.chunks + p.chunk;
+    const long long first = static_cast<long long>(p.chunk) * r.per;
+    p.base = (static_cast<size_t>(p.n) * r.pixels + first) * a.C;
+    p.p1 = static_cast<int>(min(static_cast<long long>(r.per), r.pixels - first));
+    return p;
+  }
+
+ private:
+  __device__ __forceinline__ int count(const GnArgs& a) const {
+    const GnPhase& ph = a.phase[phase];
+    const GnRun& last = a.run[ph.run0 + ph.runs - 1];
+    return last.first_block + min(ph.images, a.N - seg * ph.images) * last.chunks;
+  }
+  __device__ __forceinline__ void settle(const GnArgs& a) {  // to a segment that has this block
+    while (block >= blocks) {
+      block = static_cast<int>(blockIdx.x);
+      ++k;
+      if (++seg == a.phase[phase].segments) {
+        seg = 0;
+        if (++phase == a.phases) return;
+      }
+      blocks = count(a);
+    }
+  }
+};
+
+// A warp's ring of kStages copies and the batches of its chunks through it.
+template <typename T, bool kBackward, int kStages>
+struct GnRing {
+  static constexpr int kEsz = static_cast<int>(sizeof(T));
+  uint8_t* buf;
+  uint64_t* full;
+  int stage = 0;
+  uint32_t phase = 0;
+  int ahead = 0;   // batches of the coming chunk already in flight
+  int flying = 0;  // copies not yet waited for
+  // the coming chunk: its first batch's bytes, bytes from one batch to the next, batches, pixels of the
+  // last one
+  const uint8_t* x;
+  const uint8_t* dy;
+  uint32_t stride;
+  int nb, last;
+
+  __device__ __forceinline__ void aim(const GnArgs& a, const GnPlace& at, const GnLanes& ln) {
+    const int all = (at.p1 + ln.sp - 1) / ln.sp;
+    nb = ln.works && all > ln.wi ? (all - ln.wi + ln.nw - 1) / ln.nw : 0;
+    last = min(ln.sp, at.p1 - (ln.wi + (nb - 1) * ln.nw) * ln.sp);
+    stride = static_cast<uint32_t>(ln.nw * ln.sp * a.C * kEsz);
+    const GnRun& r = a.run[at.run];
+    const size_t off = (at.base + static_cast<size_t>(ln.wi * ln.sp) * a.C + ln.v0 * 8) * kEsz;
+    x = static_cast<const uint8_t*>(r.x) + off;
+    dy = static_cast<const uint8_t*>(r.g) + off;
+    ahead = 0;
+  }
+  // Starts batch i into a stage.
+  __device__ __forceinline__ void issue(const GnArgs& a, const GnLanes& ln, int i, int slot) {
+    const int lane = static_cast<int>(threadIdx.x) & 31;
+    ++flying;
+    if (ln.cbs == 1 && lane != 0) return;
+    const int n = i + 1 < nb ? ln.sp : last;
+    const int row = ln.nv * 8 * kEsz;
+    const size_t off = static_cast<size_t>(i) * stride;
+    uint8_t* const dst = buf + slot * kGnStage;
+    const uint32_t bytes = static_cast<uint32_t>(n * row);
+    if (lane == 0) mbar_arrive_expect_tx(&full[slot], kBackward ? 2 * bytes : bytes);
+    if (ln.cbs == 1) {  // whole pixels: contiguous
+      bulk_load(dst, x + off, bytes, &full[slot]);
+      if constexpr (kBackward) bulk_load(dst + kGnStage / 2, dy + off, bytes, &full[slot]);
+    } else {
+      __syncwarp();
+      for (int k = lane; k < n; k += 32) {
+        const size_t o = off + static_cast<size_t>(k) * (a.C * kEsz);
+        bulk_load(dst + k * row, x + o, static_cast<uint32_t>(row), &full[slot]);
+        if constexpr (kBackward)
+          bulk_load(dst + kGnStage / 2 + k * row, dy + o, static_cast<uint32_t>(row), &full[slot]);
+      }
+    }
+  }
+  // Starts the first copies of the chunk, behind those of the one before.
+  __device__ __forceinline__ void prefetch(const GnArgs& a, const GnLanes& ln) {
+    for (; ahead < kStages && ahead < nb; ++ahead) issue(a, ln, ahead, (stage + ahead) % kStages);
+  }
+  // The chunk's pixels in the ring: begin(a pixel of the thread) once, then f(its 8 channels of x (, of
+  // dy), where they go in `out`, the thread's first vector of the chunk's first pixel); K pixels are
+  // read before their arithmetic.
+  template <int K, typename B, typename F>
+  __device__ __forceinline__ void pixels(const GnArgs& a, const GnLanes& ln, GnSmem& s, T* out, B&& begin,
+                                         F&& f) {
+    prefetch(a, ln);
+    const int row = ln.nv * 8 * kEsz, step = ln.wl * row;
+    const uint32_t mine = smem_u32(buf) + static_cast<uint32_t>(ln.pl * row + (ln.v - ln.v0) * 8 * kEsz);
+    const int ostep = ln.wl * a.C;
+    T* o0 = out + static_cast<size_t>(ln.wi * ln.sp + ln.pl) * a.C;
+    const uint32_t ostride = stride / kEsz;
+    for (int i = 0; i < nb; ++i, o0 += ostride) {
+      const bool ok = mbar_wait(&full[stage], phase, &s.abort_flag, a.status, kDevTimeoutNorm);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      --flying;
+      const int n = i + 1 < nb ? ln.sp : last;
+      if (ln.active) {
+        uint32_t p = mine + stage * kGnStage;
+        T* o = o0;
+        int q = ln.pl;
+        if (i == 0 && q < n) {
+          Gn8<T> t;
+          t.load_shared(p);
+          begin(t);
+        }
+        for (; q + (K - 1) * ln.wl < n; q += K * ln.wl) {
+          Gn8<T> v[K], d[K];
+#pragma unroll
+          for (int k = 0; k < K; ++k) {
+            v[k].load_shared(p + k * step);
+            if constexpr (kBackward) d[k].load_shared(p + k * step + kGnStage / 2);
+          }
+#pragma unroll
+          for (int k = 0; k < K; ++k) f(v[k], d[k], o + k * ostep);
+          p += K * step;
+          o += K * ostep;
+        }
+#pragma unroll 1
+        for (; q < n; q += ln.wl, p += step, o += ostep) {
+          Gn8<T> v, d;
+          v.load_shared(p);
+          if constexpr (kBackward) d.load_shared(p + kGnStage / 2);
+          f(v, d, o);
+        }
+      }
+      __syncwarp();
+      if (i + kStages < nb) issue(a, ln, i + kStages, stage);
+      if (++stage == kStages) {
+        stage = 0;
+        phase ^= 1u;
+      }
+    }
+  }
+  // (matters only after a timeout: no copy may land after the block has gone)
+  __device__ __forceinline__ void drain() {
+    for (; flying > 0; --flying) {
+      mbar_wait_drain(&full[stage], phase);
+      if (++stage == kStages) {
+        stage = 0;
+        phase ^= 1u;
+      }
+    }
+  }
+};
+
+// Barriers of the statistics threads and of the merging threads.
+__device__ __forceinline__ void gn_stats_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kGnThreads) : "memory"); }
+__device__ __forceinline__ void gn_merge_sync() {
+  asm volatile("bar.sync 2, %0;" ::"n"(kGnMergeThreads) : "memory");
 }
 
-__device__ __forceinline__ float gn_group_sum(float v, int tpg) {
-  for (int o = tpg >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+
+__device__ __forceinline__ float gn_lane_sum(float v, int width) {
+  for (int o = width >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
-
-// Threads per group in a block's final sums over shared memory: a power of two up to a warp.
-__device__ __forceinline__ int gn_threads_per_group(int groups) {
+// Threads per group in a block's sums over channels: a power of two up to a warp.
+__device__ __forceinline__ int gn_group_width(const GnArgs& a) {
   int t = 32;
-  while (t > 1 && t * groups > kGnThreads) t >>= 1;
+  while (t > 1 && (t * a.groups > kGnThreads || t > a.cg)) t >>= 1;
   return t;
 }
 
-// Statistics of each block's pixels by group: part[row][g] = (mean, M2).  Thread t keeps
-// channel vector t % VC and takes every PL-th pixel.
-template <typename T>
-__global__ void __launch_bounds__(kGnThreads, 2) gn_stats_kernel(const __grid_constant__ GnArgs a) {
-  constexpr int V = Vec16<T>::V;
-  __shared__ float s_mean[kGnThreads * V];  // [pixel lane][C]
-  __shared__ float s_m2[kGnThreads * V];
-  __shared__ float s_cnt[kGnThreads];       // [pixel lane]
-  const GnPlace at = gn_place(a);
-  const GnRun& r = a.run[at.run];
-  const int vc = a.C / V, lanes = kGnThreads / vc;
-  const int v = threadIdx.x % vc, pl = threadIdx.x / vc;
-  griddep_wait();
-  if (pl < lanes) {
-    float mean[V], m2[V], pv[V];
-    float cnt = 0.f;
-    const T* x = static_cast<const T*>(r.x) + static_cast<size_t>(at.n) * r.pixels * a.C;
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-      mean[e] = m2[e] = 0.f;
-      if constexpr (kGnPivot<T>) pv[e] = static_cast<float>(x[(v * V + e) / a.cg * a.cg]);
-    }
-    for (long long p = at.p0 + pl; p < at.p1; p += static_cast<long long>(lanes) * kGnBatch) {
-      uint4 u[kGnBatch];
-      int k_n = 0;
-#pragma unroll
-      for (int k = 0; k < kGnBatch; ++k) {
-        const long long q = p + static_cast<long long>(k) * lanes;
-        u[k] = make_uint4(0u, 0u, 0u, 0u);
-        if (q < at.p1) {
-          u[k] = *(reinterpret_cast<const uint4*>(x + q * a.C) + v);
-          ++k_n;
-        }
-      }
-      // mean and squares of the k_n pixels (the zeros of missing ones add nothing to the sum and
-      // are left out of the squares), then one merge
-      float s[V], q2[V];
-#pragma unroll
-      for (int e = 0; e < V; ++e) s[e] = q2[e] = 0.f;
-#pragma unroll
-      for (int k = 0; k < kGnBatch; ++k) {
-        float f[V];
-        Vec16<T>::unpack(u[k], f);
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-          if constexpr (kGnPivot<T>)
-            s[e] += k < k_n ? f[e] - pv[e] : 0.f;
-          else
-            s[e] += f[e];
-        }
-      }
-      const float nb = static_cast<float>(k_n), inv = 1.f / nb;
-#pragma unroll
-      for (int e = 0; e < V; ++e) s[e] *= inv;
-#pragma unroll
-      for (int k = 0; k < kGnBatch; ++k) {
-        if (k < k_n) {
-          float f[V];
-          Vec16<T>::unpack(u[k], f);
-#pragma unroll
-          for (int e = 0; e < V; ++e) {
-            float d = f[e];
-            if constexpr (kGnPivot<T>) d -= pv[e];
-            d -= s[e];
-            q2[e] = fmaf(d, d, q2[e]);
-          }
-        }
-      }
-      const float w = nb / (cnt + nb), wn = w * cnt;
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const float d = s[e] - mean[e];
-        mean[e] = fmaf(d, w, mean[e]);
-        m2[e] += fmaf(d * d, wn, q2[e]);
-      }
-      cnt += nb;
-    }
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-      s_mean[pl * a.C + v * V + e] = mean[e];
-      s_m2[pl * a.C + v * V + e] = m2[e];
-    }
-    if (v == 0) s_cnt[pl] = cnt;
+// A thread's 8 channels of [pixel lane][C] (two 16-byte stores).
+__device__ __forceinline__ void gn_lane_store(float* dst, const float2 (&f)[4]) {
+  *reinterpret_cast<float4*>(dst) = make_float4(f[0].x, f[0].y, f[1].x, f[1].y);
+  *(reinterpret_cast<float4*>(dst) + 1) = make_float4(f[2].x, f[2].y, f[3].x, f[3].y);
+}
+
+// Statistics of a chunk by group: part[row][g] = (mean - pivot, M2); the pivots are the group's
+// first channel of the image's first pixel.
+template <typename T, typename Ring>
+__device__ __forceinline__ void gn_stats_sums(const GnArgs& a, const GnPlace& at, const GnLanes& ln,
+                                              GnSmem& s, Ring& ring) {
+  if (ln.active && ln.lane_index() == 0) {
+    const GnRun& r = a.run[at.run];
+    Gn8<T> t;
+    float2 f[4];
+    t.load(static_cast<const T*>(r.x) + static_cast<size_t>(at.n) * r.pixels * a.C + ln.v * 8);
+    t.get(f);
+    gn_lane_store(&s.first[ln.v * 8], f);
   }
-  __syncthreads();
-  griddep_launch_dependents();
-  // the group's channels and pixel lanes: their mean, then the squares about it
-  const int tpg = gn_threads_per_group(a.groups);
-  const int j = threadIdx.x % tpg;
-  const float inv_total = 1.f / (static_cast<float>(at.p1 - at.p0) * static_cast<float>(a.cg));
-  float2* out = a.part + static_cast<size_t>(r.row0 + (at.n - r.n0) * r.chunks + at.chunk) * a.groups;
-  for (int g0 = 0; g0 < a.groups; g0 += kGnThreads / tpg) {
-    const int g = g0 + threadIdx.x / tpg;
-    const bool in = g < a.groups;
-    const int entries = in ? lanes * a.cg : 0;
-    float s = 0.f;
-    for (int i = j; i < entries; i += tpg) {
-      const int l = i / a.cg, c = i - l * a.cg;
-      s = fmaf(s_cnt[l], s_mean[l * a.C + g * a.cg + c], s);
+  float2 np[4], s1[4], s2[4];  // minus the thread's first pixel; sums relative to it
+#pragma unroll
+  for (int i = 0; i < 4; ++i) np[i] = s1[i] = s2[i] = both(0.f);
+  ring.template pixels<kGnK>(
+      a, ln, s, static_cast<T*>(nullptr),
+      [&](const Gn8<T>& x) {
+        x.get(np);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) np[i] = make_float2(-np[i].x, -np[i].y);
+      },
+      [&](const Gn8<T>& x, const Gn8<T>&, T*) {
+        float2 f[4];
+        x.get(f);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 d = add2(f[i], np[i]);
+          s1[i] = add2(s1[i], d);
+          s2[i] = fma2(d, d, s2[i]);
+        }
+      });
+  const int cnt = ln.pixels(at.p1);
+  if (ln.active) {
+    const float inv = cnt > 0 ? 1.f / static_cast<float>(cnt) : 0.f;
+    float2 m[4], q[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      m[i] = mul2(s1[i], both(inv));
+      // (rounding may leave a constant's squares below 0)
+      q[i] = make_float2(max_nan(fmaf(-m[i].x, s1[i].x, s2[i].x), 0.f),
+                         max_nan(fmaf(-m[i].y, s1[i].y, s2[i].y), 0.f));
+      np[i] = make_float2(-np[i].x, -np[i].y);
     }
-    const float mean = gn_group_sum(s, tpg) * inv_total;
-    float m2 = 0.f;
-    for (int i = j; i < entries; i += tpg) {
-      const int l = i / a.cg, c = i - l * a.cg;
-      const float d = s_mean[l * a.C + g * a.cg + c] - mean;
-      m2 += fmaf(d * d, s_cnt[l], s_m2[l * a.C + g * a.cg + c]);
-    }
-    m2 = gn_group_sum(m2, tpg);
-    if (in && j == 0) {
-      out[g] = make_float2(mean, m2);
-      if constexpr (kGnPivot<T>) {
-        if (at.chunk == 0)
-          a.pivot[static_cast<size_t>(r.row0 + (at.n - r.n0) * r.chunks) * a.groups + g] =
-              static_cast<const float*>(r.x)[static_cast<size_t>(at.n) * r.pixels * a.C + g * a.cg];
+    const int o = ln.lane_index() * a.C + ln.v * 8;
+    gn_lane_store(&s.d[o], np);
+    gn_lane_store(&s.a[o], m);
+    gn_lane_store(&s.b[o], q);
+    if (ln.v == ln.v0) s.cnt[(threadIdx.x & ~31u) + ln.pl] = static_cast<float>(cnt);
+  }
+}
+__device__ __forceinline__ void gn_stats_reduce(const GnArgs& a, const GnPlace& at, const GnLanes& ln,
+                                                GnSmem& s) {
+  const float px = static_cast<float>(at.p1), inv_px = 1.f / px;
+  const int lanes = ln.lanes();
+  // a channel's lanes: (mean - pivot, M2)
+  auto channel = [&](int c, int g) {
+    const float pivot = s.first[g * a.cg];
+    float m = 0.f, q = 0.f;
+    if (lanes == kGnWarps && ln.wl == 1) {
+      float v[kGnWarps], n[kGnWarps];
+#pragma unroll
+      for (int l = 0; l < kGnWarps; ++l) {
+        n[l] = s.cnt[l * 32];
+        v[l] = (s.d[l * a.C + c] - pivot) + s.a[l * a.C + c];
+        if (n[l] > 0.f) m = fmaf(n[l], v[l], m);
       }
+      m *= inv_px;
+#pragma unroll
+      for (int l = 0; l < kGnWarps; ++l) {
+        const float d = v[l] - m;
+        if (n[l] > 0.f) q += fmaf(d * d, n[l], s.b[l * a.C + c]);
+      }
+      return make_float2(m, q);
+    }
+    for (int l = 0; l < lanes; ++l) {
+      const float n = s.cnt[ln.count_slot(c, l)];
+      if (n > 0.f) m = fmaf(n, (s.d[l * a.C + c] - pivot) + s.a[l * a.C + c], m);
+    }
+    m *= inv_px;
+    for (int l = 0; l < lanes; ++l) {
+      const float n = s.cnt[ln.count_slot(c, l)];
+      const float d = ((s.d[l * a.C + c] - pivot) + s.a[l * a.C + c]) - m;
+      if (n > 0.f) q += fmaf(d * d, n, s.b[l * a.C + c]);
+    }
+    return make_float2(m, q);
+  };
+  const size_t row = static_cast<size_t>(at.row) * a.groups;
+  const int t = static_cast<int>(threadIdx.x);
+  if (a.cg <= 32 && (a.cg & (a.cg - 1)) == 0) {
+    // adjacent threads have a group's channels: merged pairwise by shuffles (equal counts)
+    for (int c0 = 0; c0 < a.C; c0 += kGnThreads) {
+      const int c = c0 + t, g = c / a.cg;
+      float2 v = c < a.C ? channel(c, g) : both(0.f);
+      float n = px;
+      for (int o = 1; o < a.cg; o <<= 1, n += n) {
+        const float m = __shfl_xor_sync(0xffffffffu, v.x, o), q = __shfl_xor_sync(0xffffffffu, v.y, o);
+        const float d = m - v.x;
+        v.x = 0.5f * (v.x + m);
+        v.y = fmaf(0.5f * d * d, n, v.y + q);
+      }
+      if (c < a.C && c == g * a.cg) {
+        a.part[row + g] = v;
+        if (at.chunk == 0) a.pivot[row + g] = s.first[c];
+      }
+    }
+    return;
+  }
+  for (int c = t; c < a.C; c += kGnThreads) {
+    const float2 v = channel(c, c / a.cg);
+    s.a[c] = v.x;  // (column c of lane 0: this thread's own)
+    s.b[c] = v.y;
+  }
+  gn_stats_sync();
+  const int width = gn_group_width(a), j = t % width;
+  const float inv_cg = 1.f / static_cast<float>(a.cg);
+  for (int g0 = 0; g0 < a.groups; g0 += kGnThreads / width) {
+    const int g = g0 + t / width;
+    const int n = g < a.groups ? a.cg : 0;
+    float m = 0.f, q = 0.f;
+    for (int c = j; c < n; c += width) m += s.a[g * a.cg + c];
+    m = gn_lane_sum(m, width) * inv_cg;
+    for (int c = j; c < n; c += width) {
+      const float d = s.a[g * a.cg + c] - m;
+      q += fmaf(d * d, px, s.b[g * a.cg + c]);
+    }
+    q = gn_lane_sum(q, width);
+    if (n > 0 && j == 0) {
+      a.part[row + g] = make_float2(m, q);
+      if (at.chunk == 0) a.pivot[row + g] = s.first[g * a.cg];
     }
   }
 }
 
-// y = act(z).  Every block first merges its image's rows of partial statistics (chunk 0 also
-// writes them out), then streams its pixels.
-template <typename T>
-__global__ void __launch_bounds__(kGnThreads, 2) gn_apply_kernel(const __grid_constant__ GnArgs a) {
-  constexpr int V = Vec16<T>::V;
-  __shared__ float s_mean[kGnThreads], s_m2[kGnThreads], s_cnt[kGnThreads];
-  __shared__ float g_mean[kGnMaxChannels], g_rstd[kGnMaxChannels];
-  const GnPlace at = gn_place(a);
+// The image's statistics from its chunks' rows, by group: g1 = mean, g2 = rstd.  A thread sums its
+// rows relative to its first one.
+__device__ __forceinline__ void gn_merge_stats(const GnArgs& a, const GnPlace& at, GnSmem& s, int t) {
+  const size_t row0 = static_cast<size_t>(at.row_of_chunk0()) * a.groups;
   const GnRun& r = a.run[at.run];
-  griddep_wait();
-  griddep_launch_dependents();
-  const float2* rows = a.part + static_cast<size_t>(r.row0 + (at.n - r.n0) * r.chunks) * a.groups;
-  const int span = min(a.groups, kGnThreads);
-  const int per_g = kGnThreads / span;  // threads per group, each over every per_g-th row
+  const float2* rows = a.part + row0;
+  const int chunks = r.chunks;
+  const int span = min(a.groups, kGnMergeThreads);
+  const int per_g = kGnMergeThreads / span;  // threads per group, each over every per_g-th row
+  const int j = t / span, lane = t - j * span;
+  const float cg = static_cast<float>(a.cg), px = static_cast<float>(r.pixels);
+  const float per = static_cast<float>(r.per);
+  const float tail = static_cast<float>(r.pixels - static_cast<long long>(chunks - 1) * r.per);
+  constexpr int K = 20;
   for (int g0 = 0; g0 < a.groups; g0 += span) {
-    const int g = g0 + threadIdx.x % span, j = threadIdx.x / span;
-    float mean = 0.f, m2 = 0.f, cnt = 0.f;
-    if (j < per_g && g < a.groups) {
-      for (int i = j; i < r.chunks; i += per_g) {
-        const float2 t = rows[static_cast<size_t>(i) * a.groups + g];
-        const float nb = static_cast<float>(min(r.per, r.pixels - i * r.per));
-        const float d = t.x - mean, w = nb / (cnt + nb);
-        mean = fmaf(d, w, mean);
-        m2 += fmaf(d * d, w * cnt * static_cast<float>(a.cg), t.y);
-        cnt += nb;
+    const int g = g0 + lane;
+    const bool in = j < per_g && g < a.groups;
+    const float pivot = in && j == 0 ? __ldcg(a.pivot + row0 + g) : 0.f;
+    if (in) {
+      float ref = 0.f, sd = 0.f, sq = 0.f, m2 = 0.f, cnt = 0.f;
+      for (int i0 = j; i0 < chunks; i0 += K * per_g) {
+        float2 v[K];
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+          if (i0 + k * per_g < chunks) v[k] = __ldcg(rows + static_cast<size_t>(i0 + k * per_g) * a.groups + g);
+        if (i0 == j) ref = v[0].x;
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+          const int i = i0 + k * per_g;
+          if (i < chunks) {
+            const float n = i + 1 < chunks ? per : tail;
+            const float d = v[k].x - ref;
+            sd = fmaf(n, d, sd);
+            sq = fmaf(n * d, d, sq);
+            m2 += v[k].y;
+            cnt += n;
+          }
+        }
       }
-      s_mean[threadIdx.x] = mean;
-      s_m2[threadIdx.x] = m2;
-      s_cnt[threadIdx.x] = cnt;
+      const float m = cnt > 0.f ? sd / cnt : 0.f;
+      s.m1[t] = ref + m;
+      s.m2[t] = fmaf(cg, max_nan(fmaf(-m, sd, sq), 0.f), m2);
+      s.m3[t] = cnt;
     }
-    __syncthreads();
-    if (j == 0 && g < a.groups) {
-      const float px = static_cast<float>(r.pixels);
-      float s = 0.f;
-      for (int i = 0; i < per_g; ++i) s = fmaf(s_cnt[i * span + threadIdx.x], s_mean[i * span + threadIdx.x], s);
-      float mu = s / px;
-      float q = 0.f;
+    gn_merge_sync();
+    if (in && j == 0) {
+      float m = 0.f, q = 0.f;
+#pragma unroll 4
+      for (int i = 0; i < per_g; ++i)
+        if (s.m3[i * span + t] > 0.f) m = fmaf(s.m3[i * span + t], s.m1[i * span + t], m);
+      m /= px;
+#pragma unroll 4
       for (int i = 0; i < per_g; ++i) {
-        const float d = s_mean[i * span + threadIdx.x] - mu;
-        q += fmaf(d * d, s_cnt[i * span + threadIdx.x] * static_cast<float>(a.cg), s_m2[i * span + threadIdx.x]);
+        const float d = s.m1[i * span + t] - m;
+        if (s.m3[i * span + t] > 0.f) q += fmaf(d * d, s.m3[i * span + t] * cg, s.m2[i * span + t]);
       }
-      const float rs = 1.f / sqrtf(q / (px * static_cast<float>(a.cg)) + a.eps);
-      if constexpr (kGnPivot<T>)
-        mu += a.pivot[static_cast<size_t>(r.row0 + (at.n - r.n0) * r.chunks) * a.groups + g];
-      g_mean[g] = mu;
-      g_rstd[g] = rs;
+      const float mu = m + pivot;
+      const float rs = 1.f / sqrtf(q / (px * cg) + a.eps);
+      s.g1[g] = mu;
+      s.g2[g] = rs;
       if (at.chunk == 0 && r.mean != nullptr) {
         r.mean[static_cast<size_t>(at.n) * a.groups + g] = mu;
         r.rstd[static_cast<size_t>(at.n) * a.groups + g] = rs;
       }
     }
-    __syncthreads();
-  }
-  const int vc = a.C / V, lanes = kGnThreads / vc;
-  const int v = threadIdx.x % vc, pl = threadIdx.x / vc;
-  if (pl >= lanes) return;
-  float mean[V], rstd[V], w[V], b[V];
-#pragma unroll
-  for (int e = 0; e < V; ++e) {
-    const int c = v * V + e, g = c / a.cg;
-    mean[e] = g_mean[g];
-    rstd[e] = g_rstd[g];
-    w[e] = r.w != nullptr ? __ldg(r.w + c) : 1.f;
-    b[e] = r.b != nullptr ? __ldg(r.b + c) : 0.f;
-  }
-  const size_t base = static_cast<size_t>(at.n) * r.pixels * a.C;
-  const T* x = static_cast<const T*>(r.x) + base;
-  T* y = static_cast<T*>(r.y) + base;
-  constexpr int K = 4;
-  for (long long p = at.p0 + pl; p < at.p1; p += static_cast<long long>(lanes) * K) {
-    uint4 u[K];
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const long long q = p + static_cast<long long>(k) * lanes;
-      if (q < at.p1) u[k] = *(reinterpret_cast<const uint4*>(x + q * a.C) + v);
-    }
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const long long q = p + static_cast<long long>(k) * lanes;
-      if (q < at.p1) {
-        float f[V];
-        Vec16<T>::unpack(u[k], f);
-#pragma unroll
-        for (int e = 0; e < V; ++e)
-          f[e] = gn_act<T>(__fmaf_rn(gn_xhat(f[e], mean[e], rstd[e]), w[e], b[e]), a.act, a.alpha);
-        *(reinterpret_cast<uint4*>(y + q * a.C) + v) = Vec16<T>::pack(f);
-      }
-    }
+    gn_merge_sync();
   }
 }
 
-// Loads a thread's per-channel constants of the backward.
-template <int V>
-struct GnChannels {
-  float mean[V], rstd[V], w[V], b[V];
-  __device__ __forceinline__ void load(const GnArgs& a, const GnRun& r, int n, int v) {
+// A value per channel pair, of the channel's group: one for all 8 channels of a thread where groups
+// are whole vectors (kWhole: Cg % 8 == 0), else one per channel.
+template <bool kWhole>
+struct GnByGroup {
+  float2 v[kWhole ? 1 : 4];
+  __device__ __forceinline__ float2 operator[](int i) const { return v[kWhole ? 0 : i]; }
+  // f(group)
+  template <typename F>
+  __device__ __forceinline__ void set(const GnArgs& a, int vector, F&& f) {
+    int g = vector * 8 / a.cg;
+    if constexpr (kWhole) {
+      v[0] = both(f(g));
+    } else {
+      int rem = vector * 8 - g * a.cg;
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
-      const int c = v * V + e;
-      const size_t g = static_cast<size_t>(n) * a.groups + c / a.cg;
-      mean[e] = __ldg(r.mean + g);
-      rstd[e] = __ldg(r.rstd + g);
-      w[e] = r.w != nullptr ? __ldg(r.w + c) : 1.f;
-      b[e] = r.b != nullptr ? __ldg(r.b + c) : 0.f;
+      for (int i = 0; i < 4; ++i) {
+        float t[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          t[k] = f(g);
+          if (++rem == a.cg) {
+            rem = 0;
+            ++g;
+          }
+        }
+        v[i] = make_float2(t[0], t[1]);
+      }
     }
   }
 };
+// A thread's constants: z = (x - mean) * wr + b with wr = weight * rstd.  (x - mean first: no digits
+// of a large mean enter the product, and a constant group gives exactly b.  The backward forms z
+// with the same steps, so both take the same side of an activation's kink.)
+template <bool kWhole>
+struct GnChannels {
+  GnByGroup<kWhole> nm;  // -mean
+  float2 wr[4], b[4];
+  __device__ __forceinline__ void weights(const GnRun& r, int v) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      wr[i] = r.w != nullptr ? make_float2(__ldg(r.w + v * 8 + 2 * i), __ldg(r.w + v * 8 + 2 * i + 1)) : both(1.f);
+      b[i] = r.b != nullptr ? make_float2(__ldg(r.b + v * 8 + 2 * i), __ldg(r.b + v * 8 + 2 * i + 1)) : both(0.f);
+    }
+  }
+  // (after weights)
+  __device__ __forceinline__ void statistics(const GnArgs& a, int v, const float* mean, const float* rstd) {
+    nm.set(a, v, [&](int g) { return -mean[g]; });
+    GnByGroup<kWhole> rs;
+    rs.set(a, v, [&](int g) { return rstd[g]; });
+#pragma unroll
+    for (int i = 0; i < 4; ++i) wr[i] = mul2(wr[i], rs[i]);
+  }
+  __device__ __forceinline__ float2 centred(float2 x, int i) const { return add2(x, nm[i]); }
+  __device__ __forceinline__ float2 z(float2 d, int i) const { return fma2(d, wr[i], b[i]); }
+};
 
-// Backward sums of each block's pixels: by channel (part_c, for dweight / dbias) and, weighted,
-// by group (part, for dx).
-template <typename T>
-__global__ void __launch_bounds__(kGnThreads, 1) gn_bwd_stats_kernel(const __grid_constant__ GnArgs a) {
-  constexpr int V = Vec16<T>::V;
-  constexpr int K = 4;
-  __shared__ float s_dz[kGnThreads * V];  // [pixel lane][C], then row 0 = the block's sums
-  __shared__ float s_dx[kGnThreads * V];
-  const GnPlace at = gn_place(a);
-  const GnRun& r = a.run[at.run];
-  const int vc = a.C / V, lanes = kGnThreads / vc;
-  const int v = threadIdx.x % vc, pl = threadIdx.x / vc;
-  griddep_wait();
-  if (pl < lanes) {
-    GnChannels<V> ch;
-    ch.load(a, r, at.n, v);
-    float sz[V], sx[V];
+template <typename T, int kAct, bool kWhole, typename Ring>
+__device__ __forceinline__ void gn_apply_chunk(const GnArgs& a, const GnPlace& at, const GnLanes& ln, GnSmem& s,
+                                               Ring& ring, const GnChannels<kWhole>& ch) {
+  const float alpha = a.alpha;
+  ring.template pixels<kGnK / 2>(
+      a, ln, s, static_cast<T*>(a.run[at.run].y) + at.base + ln.v * 8, [](const Gn8<T>&) {},
+      [&](const Gn8<T>& x, const Gn8<T>&, T* y) {
+        float2 f[4];
+        x.get(f);
 #pragma unroll
-    for (int e = 0; e < V; ++e) sz[e] = sx[e] = 0.f;
-    const size_t base = static_cast<size_t>(at.n) * r.pixels * a.C;
-    const T* x = static_cast<const T*>(r.x) + base;
-    const T* dy = static_cast<const T*>(r.g) + base;
-    for (long long p = at.p0 + pl; p < at.p1; p += static_cast<long long>(lanes) * K) {
-      uint4 u[K], d[K];
-#pragma unroll
-      for (int k = 0; k < K; ++k) {
-        const long long q = p + static_cast<long long>(k) * lanes;
-        if (q < at.p1) {
-          u[k] = *(reinterpret_cast<const uint4*>(x + q * a.C) + v);
-          d[k] = *(reinterpret_cast<const uint4*>(dy + q * a.C) + v);
-        }
-      }
-#pragma unroll
-      for (int k = 0; k < K; ++k) {
-        if (p + static_cast<long long>(k) * lanes < at.p1) {
-          float f[V], h[V];
-          Vec16<T>::unpack(u[k], f);
-          Vec16<T>::unpack(d[k], h);
-#pragma unroll
-          for (int e = 0; e < V; ++e) {
-            const float xh = gn_xhat(f[e], ch.mean[e], ch.rstd[e]);
-            const float dz = h[e] * gn_act_grad<T>(__fmaf_rn(xh, ch.w[e], ch.b[e]), a.act, a.alpha);
-            sz[e] += dz;
-            sx[e] = fmaf(dz, xh, sx[e]);
-          }
-        }
-      }
-    }
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-      s_dz[pl * a.C + v * V + e] = sz[e];
-      s_dx[pl * a.C + v * V + e] = sx[e];
-    }
-  }
-  __syncthreads();
-  griddep_launch_dependents();
-  const size_t row = r.row0 + static_cast<size_t>(at.n - r.n0) * r.chunks + at.chunk;
-  float* pc = a.part_c + row * 2 * a.C;
-  for (int c = threadIdx.x; c < a.C; c += kGnThreads) {
-    float z = 0.f, x = 0.f;
-    for (int l = 0; l < lanes; ++l) {
-      z += s_dz[l * a.C + c];
-      x += s_dx[l * a.C + c];
-    }
-    pc[c] = z;
-    pc[a.C + c] = x;
-    const float w = r.w != nullptr ? __ldg(r.w + c) : 1.f;
-    s_dz[c] = w * z;  // (only this thread reads and writes column c)
-    s_dx[c] = w * x;
-  }
-  __syncthreads();
-  for (int g = threadIdx.x; g < a.groups; g += kGnThreads) {
-    float z = 0.f, x = 0.f;
-    for (int c = 0; c < a.cg; ++c) {
-      z += s_dz[g * a.cg + c];
-      x += s_dx[g * a.cg + c];
-    }
-    a.part[row * a.groups + g] = make_float2(z, x);
+        for (int i = 0; i < 4; ++i) f[i] = gn_act<T, kAct>(ch.z(ch.centred(f[i], i), i), alpha);
+        gn_put<T>(y, f);
+      });
+}
+template <typename T, bool kWhole, typename Ring>
+__device__ __forceinline__ void gn_apply(const GnArgs& a, const GnPlace& at, const GnLanes& ln, GnSmem& s,
+                                         Ring& ring, const GnChannels<kWhole>& ch) {
+  switch (a.act) {
+    case kGnRelu: return gn_apply_chunk<T, kGnRelu>(a, at, ln, s, ring, ch);
+    case kGnLeaky: return gn_apply_chunk<T, kGnLeaky>(a, at, ln, s, ring, ch);
+    case kGnSwish: return gn_apply_chunk<T, kGnSwish>(a, at, ln, s, ring, ch);
+    default: return gn_apply_chunk<T, kGnNone>(a, at, ln, s, ring, ch);
   }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kGnThreads, 1) gn_bwd_apply_kernel(const __grid_constant__ GnArgs a) {
-  constexpr int V = Vec16<T>::V;
-  constexpr int K = 4;
-  __shared__ float s_z[kGnThreads], s_x[kGnThreads];
-  __shared__ float g_z[kGnMaxChannels], g_x[kGnMaxChannels];
-  const GnPlace at = gn_place(a);
-  const GnRun& r = a.run[at.run];
-  griddep_wait();
-  griddep_launch_dependents();
-  const float2* rows = a.part + static_cast<size_t>(r.row0 + (at.n - r.n0) * r.chunks) * a.groups;
-  const int span = min(a.groups, kGnThreads);
-  const int per_g = kGnThreads / span;
-  const float inv_m = 1.f / (static_cast<float>(r.pixels) * static_cast<float>(a.cg));
-  for (int g0 = 0; g0 < a.groups; g0 += span) {
-    const int g = g0 + threadIdx.x % span, j = threadIdx.x / span;
-    float z = 0.f, x = 0.f;
-    if (j < per_g && g < a.groups) {
-      for (int i = j; i < r.chunks; i += per_g) {
-        const float2 t = rows[static_cast<size_t>(i) * a.groups + g];
-        z += t.x;
-        x += t.y;
-      }
-      s_z[threadIdx.x] = z;
-      s_x[threadIdx.x] = x;
-    }
-    __syncthreads();
-    if (j == 0 && g < a.groups) {
-      z = x = 0.f;
-      for (int i = 0; i < per_g; ++i) {
-        z += s_z[i * span + threadIdx.x];
-        x += s_x[i * span + threadIdx.x];
-      }
-      g_z[g] = __fmul_rn(z, inv_m);
-      g_x[g] = __fmul_rn(x, inv_m);
-    }
-    __syncthreads();
-  }
-  const int vc = a.C / V, lanes = kGnThreads / vc;
-  const int v = threadIdx.x % vc, pl = threadIdx.x / vc;
-  if (pl >= lanes) return;
-  GnChannels<V> ch;
-  ch.load(a, r, at.n, v);
-  float mz[V], mx[V];
+// Backward sums of a chunk: by channel (part_c, for dweight / dbias) and, weighted, by group
+// (part, for dx).  The pixels' sums are of dz and dz (x - mean); rstd follows at their end.
+template <typename T, int kAct, bool kWhole, typename Ring>
+__device__ __forceinline__ void gn_bwd_chunk_sums(const GnArgs& a, const GnPlace& at, const GnLanes& ln,
+                                                  GnSmem& s, Ring& ring, const GnChannels<kWhole>& ch,
+                                                  float2 (&sz)[4], float2 (&sx)[4]) {
+  const float alpha = a.alpha;
+  ring.template pixels<kGnK / 2>(
+      a, ln, s, static_cast<T*>(nullptr), [](const Gn8<T>&) {},
+      [&](const Gn8<T>& x, const Gn8<T>& d, T*) {
+        float2 f[4], h[4];
+        x.get(f);
+        d.get(h);
 #pragma unroll
-  for (int e = 0; e < V; ++e) {
-    const int g = (v * V + e) / a.cg;
-    mz[e] = g_z[g];
-    mx[e] = g_x[g];
-  }
-  const size_t base = static_cast<size_t>(at.n) * r.pixels * a.C;
-  const T* x = static_cast<const T*>(r.x) + base;
-  const T* dy = static_cast<const T*>(r.g) + base;
-  T* dx = static_cast<T*>(r.y) + base;
-  for (long long p = at.p0 + pl; p < at.p1; p += static_cast<long long>(lanes) * K) {
-    uint4 u[K], d[K];
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const long long q = p + static_cast<long long>(k) * lanes;
-      if (q < at.p1) {
-        u[k] = *(reinterpret_cast<const uint4*>(x + q * a.C) + v);
-        d[k] = *(reinterpret_cast<const uint4*>(dy + q * a.C) + v);
-      }
-    }
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const long long q = p + static_cast<long long>(k) * lanes;
-      if (q < at.p1) {
-        float f[V], h[V];
-        Vec16<T>::unpack(u[k], f);
-        Vec16<T>::unpack(d[k], h);
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-          const float xh = gn_xhat(f[e], ch.mean[e], ch.rstd[e]);
-          const float dz = h[e] * gn_act_grad<T>(__fmaf_rn(xh, ch.w[e], ch.b[e]), a.act, a.alpha);
-          // (the product w dz rounded on its own, as in the sums: over one value it cancels
-          // against its mean exactly)
-          const float t = __fsub_rn(__fmul_rn(ch.w[e], dz), mz[e]);
-          f[e] = ch.rstd[e] * fmaf(-xh, mx[e], t);
+        for (int i = 0; i < 4; ++i) {
+          const float2 e = ch.centred(f[i], i);
+          const float2 dz = gn_act_grad<T, kAct>(h[i], ch.z(e, i), alpha);
+          sz[i] = add2(sz[i], dz);
+          sx[i] = fma2(dz, e, sx[i]);
         }
-        *(reinterpret_cast<uint4*>(dx + q * a.C) + v) = Vec16<T>::pack(f);
+      });
+}
+template <typename T, bool kWhole, typename Ring>
+__device__ __forceinline__ void gn_bwd_sums(const GnArgs& a, const GnPlace& at, const GnLanes& ln, GnSmem& s,
+                                            Ring& ring) {
+  GnChannels<kWhole> ch;
+  const GnRun& r = a.run[at.run];
+  if (ln.active) {
+    ch.weights(r, ln.v);
+    ch.statistics(a, ln.v, r.mean + static_cast<size_t>(at.n) * a.groups,
+                  r.rstd + static_cast<size_t>(at.n) * a.groups);
+  }
+  float2 sz[4], sx[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) sz[i] = sx[i] = both(0.f);
+  switch (a.act) {
+    case kGnRelu: gn_bwd_chunk_sums<T, kGnRelu>(a, at, ln, s, ring, ch, sz, sx); break;
+    case kGnLeaky: gn_bwd_chunk_sums<T, kGnLeaky>(a, at, ln, s, ring, ch, sz, sx); break;
+    case kGnSwish: gn_bwd_chunk_sums<T, kGnSwish>(a, at, ln, s, ring, ch, sz, sx); break;
+    default: gn_bwd_chunk_sums<T, kGnNone>(a, at, ln, s, ring, ch, sz, sx);
+  }
+  if (ln.active) {
+    GnByGroup<kWhole> rs;
+    rs.set(a, ln.v, [&](int g) { return r.rstd[static_cast<size_t>(at.n) * a.groups + g]; });
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sx[i] = mul2(sx[i], rs[i]);
+    const int o = ln.lane_index() * a.C + ln.v * 8;
+    gn_lane_store(&s.a[o], sz);
+    gn_lane_store(&s.b[o], sx);
+  }
+}
+__device__ __forceinline__ void gn_bwd_reduce(const GnArgs& a, const GnPlace& at, const GnLanes& ln, GnSmem& s) {
+  float* pc = a.part_c + static_cast<size_t>(at.row) * 2 * a.C;
+  const float* w = a.run[at.run].w;
+  const int t = static_cast<int>(threadIdx.x), lanes = ln.lanes();
+  for (int c = t; c < a.C; c += kGnThreads) {
+    float z = 0.f, x = 0.f;
+#pragma unroll 8
+    for (int l = 0; l < lanes; ++l) {
+      z += s.a[l * a.C + c];
+      x += s.b[l * a.C + c];
+    }
+    pc[c] = z;
+    pc[a.C + c] = x;
+    const float wc = w != nullptr ? __ldg(w + c) : 1.f;
+    s.first[c] = wc * z;
+    s.d[c] = wc * x;
+  }
+  gn_stats_sync();
+  const int width = gn_group_width(a), j = t % width;
+  for (int g0 = 0; g0 < a.groups; g0 += kGnThreads / width) {
+    const int g = g0 + t / width;
+    const int n = g < a.groups ? a.cg : 0;
+    float z = 0.f, x = 0.f;
+    for (int c = j; c < n; c += width) {
+      z += s.first[g * a.cg + c];
+      x += s.d[g * a.cg + c];
+    }
+    z = gn_lane_sum(z, width);
+    x = gn_lane_sum(x, width);
+    if (n > 0 && j == 0) a.part[static_cast<size_t>(at.row) * a.groups + g] = make_float2(z, x);
+  }
+}
+// The image's sums over its chunks' rows, by group: g1 = mean of w dz, g2 = mean of w dz xhat.
+__device__ __forceinline__ void gn_bwd_merge(const GnArgs& a, const GnPlace& at, GnSmem& s, int t) {
+  const GnRun& r = a.run[at.run];
+  const float2* rows = a.part + static_cast<size_t>(at.row_of_chunk0()) * a.groups;
+  const int chunks = r.chunks;
+  const int span = min(a.groups, kGnMergeThreads);
+  const int per_g = kGnMergeThreads / span;
+  const int j = t / span, lane = t - j * span;
+  const float inv_m = 1.f / (static_cast<float>(r.pixels) * static_cast<float>(a.cg));
+  constexpr int K = 20;
+  for (int g0 = 0; g0 < a.groups; g0 += span) {
+    const int g = g0 + lane;
+    const bool in = j < per_g && g < a.groups;
+    if (in) {
+      float z = 0.f, x = 0.f;
+      for (int i0 = j; i0 < chunks; i0 += K * per_g) {
+        float2 v[K];
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+          v[k] = i0 + k * per_g < chunks ? __ldcg(rows + static_cast<size_t>(i0 + k * per_g) * a.groups + g)
+                                         : both(0.f);
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+          z += v[k].x;
+          x += v[k].y;
+        }
       }
+      s.m1[t] = z;
+      s.m2[t] = x;
+    }
+    gn_merge_sync();
+    if (in && j == 0) {
+      float z = 0.f, x = 0.f;
+      for (int i = 0; i < per_g; ++i) {
+        z += s.m1[i * span + t];
+        x += s.m2[i * span + t];
+      }
+      s.g1[g] = __fmul_rn(z, inv_m);
+      s.g2[g] = __fmul_rn(x, inv_m);
+    }
+    gn_merge_sync();
+  }
+}
+
+// A thread's constants of dx = rstd (w dz - m1 - (x - mean) rstd m2), with the group's means m1 of w
+// dz and m2 of w dz xhat.  (w dz - m1 first: over one value it cancels.)
+template <bool kWhole>
+struct GnGradient {
+  float2 w[4];
+  GnByGroup<kWhole> rs, n1, n2;  // rstd, -m1, -rstd m2
+  __device__ __forceinline__ void set(const GnArgs& a, const GnRun& r, int n, int v, const float* m1,
+                                      const float* m2) {
+    const float* rstd = r.rstd + static_cast<size_t>(n) * a.groups;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      w[i] = r.w != nullptr ? make_float2(__ldg(r.w + v * 8 + 2 * i), __ldg(r.w + v * 8 + 2 * i + 1)) : both(1.f);
+    rs.set(a, v, [&](int g) { return rstd[g]; });
+    n1.set(a, v, [&](int g) { return -m1[g]; });
+    n2.set(a, v, [&](int g) { return -rstd[g] * m2[g]; });
+  }
+  __device__ __forceinline__ float2 dx(float2 e, float2 dz, int i) const {
+    return mul2(rs[i], fma2(e, n2[i], fma2(w[i], dz, n1[i])));
+  }
+};
+template <typename T, int kAct, bool kWhole, typename Ring>
+__device__ __forceinline__ void gn_bwd_apply_chunk(const GnArgs& a, const GnPlace& at, const GnLanes& ln,
+                                                   GnSmem& s, Ring& ring, const GnChannels<kWhole>& ch,
+                                                   const GnGradient<kWhole>& gr) {
+  const float alpha = a.alpha;
+  ring.template pixels<kGnK / 4>(
+      a, ln, s, static_cast<T*>(a.run[at.run].y) + at.base + ln.v * 8, [](const Gn8<T>&) {},
+      [&](const Gn8<T>& x, const Gn8<T>& d, T* dx) {
+        float2 f[4], h[4];
+        x.get(f);
+        d.get(h);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 e = ch.centred(f[i], i);
+          f[i] = gr.dx(e, gn_act_grad<T, kAct>(h[i], ch.z(e, i), alpha), i);
+        }
+        gn_put<T>(dx, f);
+      });
+}
+template <typename T, bool kWhole, typename Ring>
+__device__ __forceinline__ void gn_bwd_apply(const GnArgs& a, const GnPlace& at, const GnLanes& ln, GnSmem& s,
+                                             Ring& ring, const GnChannels<kWhole>& ch,
+                                             const GnGradient<kWhole>& gr) {
+  switch (a.act) {
+    case kGnRelu: return gn_bwd_apply_chunk<T, kGnRelu>(a, at, ln, s, ring, ch, gr);
+    case kGnLeaky: return gn_bwd_apply_chunk<T, kGnLeaky>(a, at, ln, s, ring, ch, gr);
+    case kGnSwish: return gn_bwd_apply_chunk<T, kGnSwish>(a, at, ln, s, ring, ch, gr);
+    default: return gn_bwd_apply_chunk<T, kGnNone>(a, at, ln, s, ring, ch, gr);
+  }
+}
+
+// Gives up the launch: every bounded wait of the block ends.
+__device__ __forceinline__ void gn_abort(const GnArgs& a, GnSmem& s) {
+  *static_cast<volatile int*>(&s.abort_flag) = 1;
+  if (a.status) atomicCAS(a.status, 0, kDevTimeoutNorm);
+}
+__device__ __forceinline__ bool gn_aborted(GnSmem& s) { return *static_cast<volatile int*>(&s.abort_flag) != 0; }
+
+// One thread: waits until every block's sums of segment k are written.
+__device__ __forceinline__ bool gn_wait_segment(const GnArgs& a, GnSmem& s, int k, int blocks) {
+  const unsigned want = static_cast<unsigned>(blocks);
+  const uint64_t t0 = globaltimer_ns();
+  while (true) {
+    unsigned v;
+    asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(a.done + k) : "memory");
+    if (v >= want) break;
+    if (gn_aborted(s)) return false;
+    if (globaltimer_ns() - t0 > kWaitTimeoutNs) {
+      gn_abort(a, s);
+      return false;
+    }
+  }
+  __threadfence();
+  return true;
+}
+// Whether the statistics of segment k may be read already: at most four segments ahead of the apply
+// warps, so that these find theirs in L2 (two ahead left them waiting: 134 us instead of 119 us for 8 x
+// 200 x 304 x 256 bf16).
+__device__ __forceinline__ bool gn_may_read(const GnArgs& a, GnSmem& s, int k) {
+  return !a.apply || *static_cast<volatile int*>(&s.applied) >= k - 3;
+}
+
+// Warps 0-7: statistics; 8-15: apply; 16-19: merge.
+template <typename T, bool kBackward, bool kWhole>
+__global__ void __launch_bounds__(2 * kGnThreads + kGnMergeThreads, 1)
+    gn_kernel(const __grid_constant__ GnArgs a) {
+  extern __shared__ __align__(128) uint8_t gn_smem[];
+  GnSmem& s = *reinterpret_cast<GnSmem*>(gn_smem);
+  constexpr int kCapacity = kBackward ? kGnStage / 2 : kGnStage;
+  const int warp = static_cast<int>(threadIdx.x) >> 5, lane = static_cast<int>(threadIdx.x) & 31;
+  if (threadIdx.x == 0) {
+    for (int w = 0; w < kGnWarps; ++w) {
+      for (int i = 0; i < kGnStatsStages; ++i) mbar_init(&s.stats_full[w][i], 1);
+      for (int i = 0; i < kGnApplyStages; ++i) mbar_init(&s.apply_full[w][i], 1);
+    }
+    mbar_init(&s.ready, 1);
+    mbar_init(&s.taken, kGnWarps);
+    s.abort_flag = 0;
+    s.applied = 0;
+    fence_barrier_init();
+  }
+  __syncthreads();
+  if (warp < kGnWarps) {
+    const GnLanes ln(a.C, static_cast<int>(sizeof(T)), warp, lane, kCapacity);
+    GnRing<T, kBackward, kGnStatsStages> ring;
+    ring.buf = s.stats_ring[warp];
+    ring.full = s.stats_full[warp];
+    GnCursor cur(a);
+    GnPlace at;
+    if (cur.more(a)) {
+      at = cur.place(a);
+      ring.aim(a, at, ln);
+    }
+    while (cur.more(a)) {
+      const uint64_t t0 = globaltimer_ns();
+      while (!__all_sync(0xffffffffu, gn_may_read(a, s, cur.k) || gn_aborted(s))) {
+        __nanosleep(32);
+        if (globaltimer_ns() - t0 > kWaitTimeoutNs) gn_abort(a, s);
+      }
+      if constexpr (kBackward)
+        gn_bwd_sums<T, kWhole>(a, at, ln, s, ring);
+      else
+        gn_stats_sums<T>(a, at, ln, s, ring);
+      GnCursor nxt = cur;
+      nxt.next(a);
+      GnPlace then = at;
+      if (nxt.more(a)) {
+        then = nxt.place(a);
+        ring.aim(a, then, ln);
+        if (__all_sync(0xffffffffu, gn_may_read(a, s, nxt.k))) ring.prefetch(a, ln);
+      }
+      gn_stats_sync();
+      if constexpr (kBackward)
+        gn_bwd_reduce(a, at, ln, s);
+      else
+        gn_stats_reduce(a, at, ln, s);
+      gn_stats_sync();
+      if (threadIdx.x == 0) {
+        __threadfence();
+        atomicAdd(a.done + cur.k, 1u);
+      }
+      cur = nxt;
+      at = then;
+    }
+    ring.drain();
+  } else if (!a.apply) {
+    return;
+  } else if (warp < 2 * kGnWarps) {
+    const GnLanes ln(a.C, static_cast<int>(sizeof(T)), warp - kGnWarps, lane, kCapacity);
+    GnRing<T, kBackward, kGnApplyStages> ring;
+    ring.buf = s.apply_ring[warp - kGnWarps];
+    ring.full = s.apply_full[warp - kGnWarps];
+    uint32_t phase = 0;
+    for (GnCursor cur(a); cur.more(a); cur.next(a), phase ^= 1u) {
+      const GnPlace at = cur.place(a);
+      const GnRun& r = a.run[at.run];
+      if (warp == kGnWarps && lane == 0) *static_cast<volatile int*>(&s.applied) = cur.k;
+      // (what does not depend on the other blocks, before the wait for them)
+      ring.aim(a, at, ln);
+      if (r.y != nullptr) ring.prefetch(a, ln);
+      GnChannels<kWhole> ch;
+      if (ln.active) {
+        ch.weights(r, ln.v);
+        if constexpr (kBackward)
+          ch.statistics(a, ln.v, r.mean + static_cast<size_t>(at.n) * a.groups,
+                        r.rstd + static_cast<size_t>(at.n) * a.groups);
+      }
+      const bool ok = mbar_wait(&s.ready, phase, &s.abort_flag, a.status, kDevTimeoutNorm);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      GnGradient<kWhole> gr;
+      if (ln.active) {
+        if constexpr (kBackward)
+          gr.set(a, r, at.n, ln.v, s.g1, s.g2);
+        else
+          ch.statistics(a, ln.v, s.g1, s.g2);
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&s.taken);
+      if constexpr (kBackward) {
+        if (r.y != nullptr) gn_bwd_apply<T>(a, at, ln, s, ring, ch, gr);
+      } else {
+        gn_apply<T>(a, at, ln, s, ring, ch);
+      }
+    }
+    ring.drain();
+  } else {
+    const int t = static_cast<int>(threadIdx.x) - 2 * kGnThreads;
+    uint32_t phase = 0;
+    int waited = -1;
+    for (GnCursor cur(a); cur.more(a); cur.next(a), phase ^= 1u) {
+      const GnPlace at = cur.place(a);
+      if (t == 0) {
+        bool ok = !gn_aborted(s);
+        if (ok && cur.k != waited) ok = gn_wait_segment(a, s, cur.k, cur.blocks);
+        // (g1 and g2 of the chunk before are in registers)
+        ok = ok && mbar_wait(&s.taken, phase ^ 1u, &s.abort_flag, a.status, kDevTimeoutNorm);
+        s.go = ok;
+      }
+      waited = cur.k;
+      gn_merge_sync();
+      const bool ok = *static_cast<volatile int*>(&s.go) != 0;
+      if (!ok) break;
+      if constexpr (kBackward)
+        gn_bwd_merge(a, at, s, t);
+      else
+        gn_merge_stats(a, at, s, t);
+      if (t == 0) mbar_arrive(&s.ready);
     }
   }
 }
@@ -544,6 +1099,7 @@ __global__ void __launch_bounds__(1024) gn_bwd_sum_kernel(const __grid_constant_
   griddep_wait();
   float z = 0.f, x = 0.f;
   if (c < a.C) {
+#pragma unroll 4
     for (int i = row; i < sp.rows; i += 32) {
       const float* p = a.part_c + static_cast<size_t>(sp.row0 + i) * 2 * a.C;
       z += p[c];
@@ -563,96 +1119,79 @@ __global__ void __launch_bounds__(1024) gn_bwd_sum_kernel(const __grid_constant_
 }
 
 // ------------------------------------------------------------------------------ host side
-// The launches of one call: runs of images whose maps together stay within `budget` bytes (one
-// image at least), at most kGnMaxRuns of them per launch.
-struct GnLaunch {
-  std::vector<GnRun> runs;  // (x, g, y, ... filled by the caller)
-  std::vector<int> level;
-  int blocks = 0;
-};
 struct GnSchedule {
-  std::vector<GnLaunch> launches;
-  int rows = 0;
+  GnRun run[kGnMaxRuns];  // sizes only
+  GnPhase phase[kGnMaxRuns];
+  int phases = 0, segments = 0, blocks = 0;  // blocks: of the largest segment
+  long long rows = 0;
 };
 
-// Cuts the launch's images into chunks: about `target` blocks of equal bytes (the levels of a
-// launch share them in proportion), none below 16 KB.
-void gn_cut(GnLaunch& l, const std::vector<int>& images, long long pixel_bytes, int target) {
+// Cuts the images of a segment into chunks: about `target` blocks of equal bytes (the levels share
+// them in proportion), none below 8 KB.
+void gn_cut(GnRun* run, int runs, int images, long long pixel_bytes, int target) {
   long long total = 0;
-  for (size_t i = 0; i < l.runs.size(); ++i) total += l.runs[i].pixels * pixel_bytes * images[i];
-  long long per_block = std::max<long long>((total + target - 1) / target, 16384);
+  for (int i = 0; i < runs; ++i) total += run[i].pixels * pixel_bytes * images;
+  long long per_block = std::max<long long>((total + target - 1) / target, 8192);
   for (;;) {
     long long blocks = 0;
-    for (size_t i = 0; i < l.runs.size(); ++i) {
-      GnRun& r = l.runs[i];
-      long long per = std::max<long long>(1, per_block / pixel_bytes);
-      r.chunks = static_cast<int>((r.pixels + per - 1) / per);
-      r.per = (r.pixels + r.chunks - 1) / r.chunks;
+    for (int i = 0; i < runs; ++i) {
+      GnRun& r = run[i];
+      const long long per = std::min<long long>(std::max<long long>(1, per_block / pixel_bytes), 1 << 30);
+      long long chunks = (r.pixels + per - 1) / per;
+      r.per = static_cast<int>((r.pixels + chunks - 1) / chunks);
       r.chunks = static_cast<int>((r.pixels + r.per - 1) / r.per);  // (none empty)
-      blocks += static_cast<long long>(r.chunks) * images[i];
+      r.first_block = static_cast<int>(blocks);
+      blocks += static_cast<long long>(r.chunks) * images;
     }
-    long long at_least = 0;
-    for (int n : images) at_least += n;
-    if (blocks <= std::max<long long>(target, at_least) || per_block > total) break;
-    per_block += per_block / 8;  // rounding left a second, nearly empty wave
+    if (blocks <= std::max<long long>(target, static_cast<long long>(images) * runs) || per_block > total) break;
+    per_block += per_block / 16 + 1;  // rounding left a few chunks for a second round
   }
 }
 
-GnSchedule gn_schedule(int levels, int N, int C, int esz, const long long* pixels, long long budget,
-                       int per_sm) {
+GnSchedule gn_schedule(DType dt, int levels, int N, int C, const long long* pixels, long long budget) {
   GnSchedule s;
-  const long long pixel_bytes = static_cast<long long>(C) * esz;
-  const int target = sm_count() * per_sm;
-  std::vector<int> images;
-  long long used = 0;
-  auto close = [&] {
-    if (s.launches.empty() || images.empty()) return;
-    GnLaunch& l = s.launches.back();
-    gn_cut(l, images, pixel_bytes, target);
-    for (size_t i = 0; i < l.runs.size(); ++i) {
-      l.runs[i].first_block = l.blocks;
-      l.runs[i].row0 = s.rows;
-      l.blocks += l.runs[i].chunks * images[i];
-      s.rows += l.runs[i].chunks * images[i];
+  std::memset(s.run, 0, sizeof(s.run));
+  const long long pixel_bytes = static_cast<long long>(C) * dtype_size(dt);
+  const int target = sm_count();
+  for (int lv = 0; lv < levels;) {
+    GnPhase& p = s.phase[s.phases++];
+    p.run0 = lv;
+    long long used = 0;
+    int end = lv;
+    while (end < levels && used + pixels[end] * pixel_bytes * N <= budget) used += pixels[end++] * pixel_bytes * N;
+    if (end > lv) {  // whole levels together
+      p.runs = end - lv;
+      p.images = N;
+    } else {
+      p.runs = 1;
+      p.images = static_cast<int>(std::max<long long>(1, budget / (pixels[lv] * pixel_bytes)));
+      // (segments of equal size)
+      const int count = (N + p.images - 1) / p.images;
+      p.images = (N + count - 1) / count;
     }
-    images.clear();
-    used = 0;
-  };
-  for (int lv = 0; lv < levels; ++lv) {
-    const long long bytes = pixels[lv] * pixel_bytes;
-    for (int n = 0; n < N;) {
-      if (s.launches.empty() || images.empty()) s.launches.emplace_back();
-      GnLaunch& l = s.launches.back();
-      const long long room = (budget - used) / bytes;
-      int take = static_cast<int>(std::min<long long>(N - n, room));
-      if (take < 1 && !images.empty()) {
-        close();
-        continue;
-      }
-      take = std::max(take, 1);
-      GnRun r;
-      std::memset(&r, 0, sizeof(r));
-      r.pixels = pixels[lv];
-      r.n0 = n;
-      l.runs.push_back(r);
-      l.level.push_back(lv);
-      images.push_back(take);
-      used += bytes * take;
-      n += take;
-      if (static_cast<int>(l.runs.size()) == kGnMaxRuns) close();
+    p.segments = (N + p.images - 1) / p.images;
+    for (int i = 0; i < p.runs; ++i) s.run[lv + i].pixels = pixels[lv + i];
+    gn_cut(s.run + lv, p.runs, p.images, pixel_bytes, target);
+    for (int i = 0; i < p.runs; ++i) {
+      s.run[lv + i].row0 = static_cast<int>(s.rows);
+      s.rows += static_cast<long long>(s.run[lv + i].chunks) * N;
     }
+    const GnRun& last = s.run[lv + p.runs - 1];
+    s.blocks = std::max(s.blocks, last.first_block + p.images * last.chunks);
+    s.segments += p.segments;
+    lv += p.runs;
   }
-  close();
   return s;
 }
 
-// Bytes of input that a run of launches keeps in L2 between its two passes.
-constexpr long long kGnForwardBudget = 48LL << 20;
-constexpr long long kGnBackwardBudget = 32LL << 20;  // of x; dy doubles it
+// Segment size: bytes of x (the backward's come with dy).  A segment is read again from L2 while the
+// next ones stream in, so a few of them have to fit its 126 MB; half the size costs more waits than it
+// saves (R50 pyramid 47 -> 50 us).
+constexpr long long kGnForwardBudget = 64LL << 20;
+constexpr long long kGnBackwardBudget = 32LL << 20;
 
 GnSchedule gn_schedule_for(DType dt, int levels, int N, int C, const long long* pixels, bool backward) {
-  return gn_schedule(levels, N, C, dtype_size(dt), pixels, backward ? kGnBackwardBudget : kGnForwardBudget,
-                     backward ? 1 : 2);
+  return gn_schedule(dt, levels, N, C, pixels, backward ? kGnBackwardBudget : kGnForwardBudget);
 }
 
 size_t gn_align(size_t n) { return (n + 255) / 256 * 256; }
@@ -666,95 +1205,75 @@ bool gn_sizes_ok(int levels, int N, int C, const long long* pixels, int groups) 
   return true;
 }
 
-template <typename T>
-cudaError_t gn_forward_t(const GnSchedule& sc, GnArgs& a, const GroupNormLevel* lv, cudaStream_t s) {
-  LaunchOpts first, next;
-  next.pdl = true;
-  bool started = false;
-  for (const GnLaunch& l : sc.launches) {
-    a.runs = static_cast<int>(l.runs.size());
-    for (int i = 0; i < a.runs; ++i) {
-      GnRun r = l.runs[i];
-      const GroupNormLevel& v = lv[l.level[i]];
-      r.x = v.x;
-      r.y = v.y;
-      r.w = v.weight;
-      r.b = v.bias;
-      r.mean = v.mean;
-      r.rstd = v.rstd;
-      a.run[i] = r;
-    }
-    cudaError_t e = launch_ex(gn_stats_kernel<T>, dim3(l.blocks), dim3(kGnThreads), 0, s,
-                              started ? next : first, 1, a);
-    if (e != cudaSuccess) return e;
-    started = true;
-    if ((e = launch_ex(gn_apply_kernel<T>, dim3(l.blocks), dim3(kGnThreads), 0, s, next, 1, a)) !=
-        cudaSuccess)
-      return e;
-  }
-  return cudaSuccess;
+// Workspace: counters, rows by group, then pivots (forward) or rows by channel (backward).
+struct GnWorkspace {
+  size_t part, extra, total;
+};
+GnWorkspace gn_workspace(const GnSchedule& sc, int C, int groups, bool backward) {
+  const size_t rows = static_cast<size_t>(sc.rows);
+  GnWorkspace w;
+  w.part = gn_align(sc.segments * sizeof(unsigned));
+  w.extra = w.part + gn_align(rows * groups * sizeof(float2));
+  w.total = w.extra + gn_align(rows * (backward ? 2 * C : groups) * sizeof(float));
+  return w;
 }
 
-template <typename T>
-cudaError_t gn_backward_t(const GnSchedule& sc, GnArgs& a, const GroupNormLevel* lv, int levels, int N,
-                          cudaStream_t s) {
-  LaunchOpts first, next;
-  next.pdl = true;
-  bool started = false;
+template <typename T, bool kBackward, bool kWhole>
+cudaError_t gn_launch(const GnSchedule& sc, const GnArgs& a, cudaStream_t s) {
+  const auto kernel = gn_kernel<T, kBackward, kWhole>;
+  constexpr int kSmem = static_cast<int>(sizeof(GnSmem));
+  static_assert(kSmem <= 232448, "group norm smem");
+  static std::atomic<bool> configured[64];
+  cudaError_t e = once_per_device(configured, [&] {
+    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+  });
+  if (e != cudaSuccess) return e;
+  if ((e = cudaMemsetAsync(a.done, 0, sc.segments * sizeof(unsigned), s)) != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(std::min(sc.blocks, sm_count())));
+  cfg.blockDim = dim3(2 * kGnThreads + kGnMergeThreads);
+  cfg.dynamicSmemBytes = kSmem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeCooperative;  // blocks wait for one another: all resident or none
+  attr[0].val.cooperative = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, a);
+}
+
+// dweight and dbias from the rows: a level's rows follow one another, and so do the levels; one
+// with null dweight and dbias adds its rows to the level before it.
+cudaError_t gn_sum_rows(const GnSchedule& sc, const GnArgs& a, const GroupNormLevel* lv, int levels,
+                        cudaStream_t s) {
   GnSumArgs sum;
   std::memset(&sum, 0, sizeof(sum));
   sum.part_c = a.part_c;
   sum.C = a.C;
-  bool want_sums = false;
-  for (const GnLaunch& l : sc.launches) {
-    a.runs = static_cast<int>(l.runs.size());
-    bool want_dx = false;
-    for (int i = 0; i < a.runs; ++i) {
-      GnRun r = l.runs[i];
-      const GroupNormLevel& v = lv[l.level[i]];
-      r.x = v.x;
-      r.g = v.grad;
-      r.y = v.y;
-      r.w = v.weight;
-      r.b = v.bias;
-      r.mean = v.mean;
-      r.rstd = v.rstd;
-      a.run[i] = r;
-      want_dx = want_dx || v.y != nullptr;
-    }
-    cudaError_t e = launch_ex(gn_bwd_stats_kernel<T>, dim3(l.blocks), dim3(kGnThreads), 0, s,
-                              started ? next : first, 1, a);
-    if (e != cudaSuccess) return e;
-    started = true;
-    if (want_dx && (e = launch_ex(gn_bwd_apply_kernel<T>, dim3(l.blocks), dim3(kGnThreads), 0, s, next,
-                                  1, a)) != cudaSuccess)
-      return e;
-  }
-  // Rows of a level's images follow one another over the launches, and so do the levels: a level
-  // with null dweight and dbias adds its rows to the level before it.
+  bool wanted = false;
   int spans = 0;
-  int row = 0;
   for (int v = 0; v < levels; ++v) {
-    int rows = 0;
-    for (const GnLaunch& l : sc.launches)
-      for (size_t i = 0; i < l.runs.size(); ++i)
-        if (l.level[i] == v) {
-          const int end = i + 1 < l.runs.size() ? l.runs[i + 1].row0 : l.runs[0].row0 + l.blocks;
-          rows += end - l.runs[i].row0;
-        }
     if (v == 0 || lv[v].dweight != nullptr || lv[v].dbias != nullptr) {
       GnSumSpan& sp = sum.span[spans++];
       sp.dw = lv[v].dweight;
       sp.db = lv[v].dbias;
-      sp.row0 = row;
-      sp.rows = 0;
-      want_sums = want_sums || sp.dw != nullptr || sp.db != nullptr;
+      sp.row0 = sc.run[v].row0;
+      wanted = wanted || sp.dw != nullptr || sp.db != nullptr;
     }
-    sum.span[spans - 1].rows += rows;
-    row += rows;
+    sum.span[spans - 1].rows += sc.run[v].chunks * a.N;
   }
-  if (!want_sums) return cudaSuccess;
-  return launch_ex(gn_bwd_sum_kernel, dim3(spans * ((a.C + 31) / 32)), dim3(1024), 0, s, next, 1, sum);
+  if (!wanted) return cudaSuccess;
+  return launch_ex(gn_bwd_sum_kernel, dim3(spans * ((a.C + 31) / 32)), dim3(1024), 0, s, LaunchOpts(), 1,
+                   sum);
+}
+
+template <typename T>
+cudaError_t gn_run(const GnSchedule& sc, const GnArgs& a, const GroupNormLevel* lv, int levels,
+                   bool backward, cudaStream_t s) {
+  const bool whole = a.cg % 8 == 0;
+  if (!backward) return whole ? gn_launch<T, false, true>(sc, a, s) : gn_launch<T, false, false>(sc, a, s);
+  const cudaError_t e = whole ? gn_launch<T, true, true>(sc, a, s) : gn_launch<T, true, false>(sc, a, s);
+  return e == cudaSuccess ? gn_sum_rows(sc, a, lv, levels, s) : e;
 }
 
 }  // namespace
@@ -763,38 +1282,52 @@ size_t group_norm_workspace_bytes(DType dt, int levels, int N, int C, const long
                                   int groups, bool backward) {
   if (!gn_sizes_ok(levels, N, C, pixels, groups)) return 0;
   const GnSchedule sc = gn_schedule_for(dt, levels, N, C, pixels, backward);
-  const size_t rows = static_cast<size_t>(sc.rows);
-  const size_t extra = backward ? rows * 2 * C : dt == DType::F32 ? rows * groups : 0;
-  return gn_align(rows * groups * sizeof(float2)) + gn_align(extra * sizeof(float));
+  return sc.rows < (1LL << 31) ? gn_workspace(sc, C, groups, backward).total : 0;
 }
 
 cudaError_t launch_group_norm(DType dt, const GroupNormLevel* lv, int levels, int N, int C,
                               const long long* pixels, int groups, float eps, int act, float alpha,
-                              bool backward, void* ws, size_t ws_bytes, cudaStream_t s) {
+                              bool backward, void* ws, size_t ws_bytes, int* status,
+                              cudaStream_t s) {
   if (!gn_sizes_ok(levels, N, C, pixels, groups)) return cudaErrorInvalidValue;
   const GnSchedule sc = gn_schedule_for(dt, levels, N, C, pixels, backward);
-  const size_t rows = static_cast<size_t>(sc.rows);
-  const size_t part = gn_align(rows * groups * sizeof(float2));
-  const size_t extra = backward ? rows * 2 * C : dt == DType::F32 ? rows * groups : 0;
-  if (part + gn_align(extra * sizeof(float)) > ws_bytes) return cudaErrorInvalidValue;
+  if (sc.rows >= (1LL << 31)) return cudaErrorInvalidValue;
+  const GnWorkspace w = gn_workspace(sc, C, groups, backward);
+  if (w.total > ws_bytes) return cudaErrorInvalidValue;
   GnArgs a;
   std::memset(&a, 0, sizeof(a));
+  for (int l = 0; l < levels; ++l) {
+    a.run[l] = sc.run[l];
+    a.run[l].x = lv[l].x;
+    a.run[l].g = lv[l].grad;
+    a.run[l].y = lv[l].y;
+    a.run[l].w = lv[l].weight;
+    a.run[l].b = lv[l].bias;
+    a.run[l].mean = lv[l].mean;
+    a.run[l].rstd = lv[l].rstd;
+    a.apply |= lv[l].y != nullptr;
+  }
+  std::memcpy(a.phase, sc.phase, sizeof(a.phase));
+  a.phases = sc.phases;
+  a.N = N;
   a.C = C;
   a.groups = groups;
   a.cg = C / groups;
   a.act = act;
   a.alpha = alpha;
   a.eps = eps;
-  a.part = static_cast<float2*>(ws);
-  (backward ? a.part_c : a.pivot) = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + part);
+  a.status = status;
+  uint8_t* base = static_cast<uint8_t*>(ws);
+  a.done = reinterpret_cast<unsigned*>(base);
+  a.part = reinterpret_cast<float2*>(base + w.part);
+  (backward ? a.part_c : a.pivot) = reinterpret_cast<float*>(base + w.extra);
   switch (dt) {
     case DType::BF16:
-      return backward ? gn_backward_t<__nv_bfloat16>(sc, a, lv, levels, N, s)
-                      : gn_forward_t<__nv_bfloat16>(sc, a, lv, s);
+      return gn_run<__nv_bfloat16>(sc, a, lv, levels, backward, s);
     case DType::F16:
-      return backward ? gn_backward_t<__half>(sc, a, lv, levels, N, s) : gn_forward_t<__half>(sc, a, lv, s);
+      return gn_run<__half>(sc, a, lv, levels, backward, s);
     case DType::F32:
-      return backward ? gn_backward_t<float>(sc, a, lv, levels, N, s) : gn_forward_t<float>(sc, a, lv, s);
+      return gn_run<float>(sc, a, lv, levels, backward, s);
     default:
       return cudaErrorInvalidValue;
   }

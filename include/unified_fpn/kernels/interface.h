@@ -122,7 +122,8 @@ size_t group_norm_workspace_bytes(DType dt, int levels, int N, int C, const long
                                   int groups, bool backward);
 cudaError_t launch_group_norm(DType dt, const GroupNormLevel* lv, int levels, int N, int C,
                               const long long* pixels, int groups, float eps, int act, float alpha,
-                              bool backward, void* ws, size_t ws_bytes, cudaStream_t s);
+                              bool backward, void* ws, size_t ws_bytes, int* status,
+                              cudaStream_t s);
 
 // ---- tensor-core kernels (tc_kernels.cu)
 // Spatial tiling of the 3x3 implicit GEMM: tile_w * tile_h = 128 output pixels.
