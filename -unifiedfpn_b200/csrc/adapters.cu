@@ -14,9 +14,12 @@
 // back into shared memory as the A operand of a last MMA against up[a], on the accumulator that
 // already holds x W^T.  So an adapter costs R / 256 more tensor work and no further pass.
 //
-// h is kept in two 16-bit parts, hi = round(h) and lo = round(h - hi), 16 (bf16) or 22 (fp16) bits
-// together: one rounding to bf16 would be the largest error of the fp32 weight gradients, and of
-// an adapter's share of out, for one k-step more.  The backward reads both parts.
+// h is kept in 16-bit parts, hi = round(h), the next = round(h - hi) and so on: three of bf16 or two
+// of fp16 carry 22 bits and more.  One rounding to bf16 would be the largest error of the fp32 weight
+// gradients, and of an adapter's share of out; the further parts cost one k-step of the last MMA each,
+// and columns of the gradients' GEMM.  The tensor cores' fp32 accumulation rounds every step
+// downwards, an error that grows with the number of steps: the products behind h are split over up to
+// four accumulators (32 steps each at K = 2048: dup 3.1e-6 -> 0.8e-6 off at fp16).
 #include "kernels.h"
 #include "tc_gemm.cuh"
 
@@ -29,21 +32,50 @@ namespace ufpn {
 namespace {
 
 constexpr int kAdMaxRank = 64;
-constexpr int kAdThreads = kTcThreads;  // TMA warp, MMA warp, 8 epilogue warps
+constexpr int kAdEpiWarps = 8;
+// TMA warp, MMA warp, 8 epilogue warps (at 168 registers a thread: each keeps a row of 128 accumulators)
+constexpr int kAdThreads = 64 + 32 * kAdEpiWarps;
 constexpr int kDevTimeoutAdapter = 0x107;
 
+template <typename T>
+constexpr int kAdParts = TcElem<T>::kFmt == 1 ? 3 : 2;  // of h: bf16, fp16
+
+// K-major operand rows of RB = 32, 64 or 128 bytes under the swizzle of that width (16-byte chunk c of
+// row r at c ^ (r * RB / 128 % (RB / 16))), 8-row atoms of 8 RB bytes.
+template <int RB>
+__device__ __forceinline__ uint64_t sdesc_kmajor_rows(uint32_t saddr) {
+  constexpr uint64_t layout = RB == 128 ? 2 : RB == 64 ? 4 : 6;
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((saddr & 0x3FFFFu) >> 4);
+  d |= static_cast<uint64_t>(1) << 16;
+  d |= static_cast<uint64_t>(8 * RB >> 4) << 32;
+  d |= static_cast<uint64_t>(1) << 46;
+  d |= layout << 61;
+  return d;
+}
+template <int RB>
+__device__ __forceinline__ uint32_t row_chunk(int row, int chunk) {
+  return static_cast<uint32_t>(row * RB + ((chunk ^ ((row * RB / 128) & (RB / 16 - 1))) << 4));
+}
+
 // Shared memory of fpn_adapter_kernel for ranks up to RP.
-template <int RP>
+template <int RP, int kParts>
 struct AdCfg {
-  static constexpr int kU = RP * 128;  // one k-block of down[a]
+  static constexpr int kRow = RP * 2;   // bytes of a row of h or up
+  static constexpr int kU = RP * 128;   // one k-block of down[a]
   static constexpr int kStage = kTcAStage + kTcBStage + kU;
   static constexpr int kStages = RP <= 32 ? 3 : 2;  // (three of 56 KB would not fit)
-  static constexpr int kOffV = kStages * kStage;         // up[a]: 256 rows of 128 bytes
-  static constexpr int kOffT = kOffV + kTcBStage;        // h: hi, lo; then the output's staging
-  static constexpr int kOffBars = kOffT + 2 * kTcAStage;
+  static constexpr int kPart = kTcBlockM * kRow;
+  // h's parts; before them, in the same place, the top-down weights (their MMA is over when h is)
+  static constexpr int kT = kParts * kPart > kTcAStage ? kParts * kPart : kTcAStage;
+  static constexpr int kStaging = RP <= 16 ? 4096 : 2048;  // per storing warp: 32 pixels
+  static constexpr int kOffV = kStages * kStage;           // up[a]: 256 rows
+  static constexpr int kOffT = kOffV + kTcBlockN * kRow;
+  static constexpr int kOffStaging = kOffT + kT;
+  static constexpr int kOffBias = kOffStaging + kAdEpiWarps * kStaging;
+  static constexpr int kOffBars = kOffBias + kTcBlockN * 4;
   static constexpr int kSmemBytes = kOffBars + 256 + 1024 /*alignment slack*/;
-  static_assert(kU % 1024 == 0 && kSmemBytes <= 232448, "adapter smem");
-  static_assert(2 * kTcAStage == kTcEpiWarps * kTcStagingPerWarp, "staging takes h's place");
+  static_assert(kU % 1024 == 0 && kPart % 1024 == 0 && kT % 1024 == 0 && kSmemBytes <= 232448, "adapter smem");
 };
 
 struct AdArgs {
@@ -56,24 +88,29 @@ struct AdArgs {
   long long va, vc, vr;
   int v_rows;    // output channels
   int v_vec;     // vr == 1 and every row is whole 16-byte vectors
-  void* hidden;  // [pixels][2][rank_pad] hi, lo; or null
+  void* hidden;  // [pixels][parts][rank_pad], or null
   int rank_pad;  // rank rounded up to 8
   int want_out;  // 0: only hidden
+  int h_accs;    // accumulators that h's k-blocks alternate over
 };
+constexpr int kAdMaxHAccs = 4;
+int ad_h_accs(int num_kb) { return std::min(kAdMaxHAccs, (num_kb + 7) / 8); }
 
 __device__ __forceinline__ int ad_adapter(const AdArgs& a, int n) {
   const int i = __ldg(a.index + n);
   return i >= 0 && i < a.adapters ? i : -1;
 }
 
-// h in two parts: v ~ hi + lo.  (fp16: a value beyond its range keeps the rest in lo.)
+// v ~ the sum of its parts.  (fp16: a value beyond its range keeps the rest in the second.)
 template <typename T>
-__device__ __forceinline__ void ad_split(float v, uint16_t& hi, uint16_t& lo) {
-  float c = v;
-  if constexpr (TcElem<T>::kFmt == 0) c = v > 65504.f ? 65504.f : (v < -65504.f ? -65504.f : v);
-  hi = Pack<T>::bits(c);
-  const float h = Pack<T>::unpack(static_cast<uint32_t>(hi)).x;
-  lo = Pack<T>::bits(v - h);
+__device__ __forceinline__ void ad_split(float v, uint16_t (&part)[kAdParts<T>]) {
+#pragma unroll
+  for (int i = 0; i < kAdParts<T>; ++i) {
+    float c = v;
+    if constexpr (TcElem<T>::kFmt == 0) c = v > 65504.f ? 65504.f : (v < -65504.f ? -65504.f : v);
+    part[i] = Pack<T>::bits(c);
+    v -= Pack<T>::unpack(static_cast<uint32_t>(part[i])).x;
+  }
 }
 
 template <typename T, int RP>
@@ -84,7 +121,8 @@ __global__ void __launch_bounds__(kAdThreads, 1)
                        const __grid_constant__ CUtensorMap map_coarse,
                        const __grid_constant__ CUtensorMap map_u, const TcGemmArgs args,
                        const AdArgs ad) {
-  using Cfg = AdCfg<RP>;
+  constexpr int kParts = kAdParts<T>;
+  using Cfg = AdCfg<RP, kParts>;
   constexpr int S = Cfg::kStages;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_addr = smem_u32(smem_raw);
@@ -96,7 +134,7 @@ __global__ void __launch_bounds__(kAdThreads, 1)
   uint64_t* acce_bar = accf_bar + 1;   // ... and read
   uint64_t* hfull_bar = accf_bar + 2;  // h accumulator final
   uint64_t* tfull_bar = accf_bar + 3;  // h and up in shared memory
-  uint64_t* sfree_bar = accf_bar + 4;  // every warp's stores have left the staging
+  uint64_t* wfull_bar = accf_bar + 4;  // the top-down weights in shared memory
   uint64_t* done_bar = accf_bar + 5;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done_bar + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -104,7 +142,7 @@ __global__ void __launch_bounds__(kAdThreads, 1)
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   const bool bil_mma = args.coarse != nullptr && args.cbox_w > 0;
-  constexpr uint32_t kHCol = kTcBlockN;  // h accumulator: TMEM columns [256, 256 + RP)
+  constexpr uint32_t kHCol = kTcBlockN;  // h accumulators: TMEM columns from 256, RP each
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < S; ++s) {
@@ -112,10 +150,10 @@ __global__ void __launch_bounds__(kAdThreads, 1)
       mbar_init(&empty_bar[s], 1);
     }
     mbar_init(accf_bar, 1);
-    mbar_init(acce_bar, kTcEpiWarps * 32);
+    mbar_init(acce_bar, 32 * kAdEpiWarps);
     mbar_init(hfull_bar, 1);
-    mbar_init(tfull_bar, kTcEpiWarps * 32);
-    mbar_init(sfree_bar, kTcEpiWarps);
+    mbar_init(tfull_bar, kAdEpiWarps * 32);
+    mbar_init(wfull_bar, kTcBlockM);
     mbar_init(done_bar, 1);
     *abort_flag = 0;
     fence_barrier_init();
@@ -167,9 +205,8 @@ __global__ void __launch_bounds__(kAdThreads, 1)
               tma_load_4d(su, &map_u, &full_bar[stage], kb * 64, 0, 0, adapter, kPolicyEvictLast);
           }
         } else {
-          // top-down k-block, as in the plain lateral
-          tc_build_bilinear<T>(sa, sb, lane, x0, y0, args.tile_w, args.H, args.W, args.Hc, args.Wc,
-                               args.scale_y, args.scale_x, args.cbox_w, args.cbox_h);
+          // top-down k-block: the tile's coarse box as the B operand (the weights: the h warps)
+          tc_zero_btail(sb, lane, args.cbox_w * args.cbox_h, 4);
           fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) {
@@ -207,6 +244,7 @@ __global__ void __launch_bounds__(kAdThreads, 1)
       constexpr uint32_t idesc_bmn = make_idesc(kTcBlockM, kTcBlockN, kFmt, kFmt, 1u);
       int stage = 0;
       uint32_t phase = 0, tile_phase = 0, h_phase = 0;
+      const uint32_t t_addr = smem_u32(smem + Cfg::kOffT);
       bool ok = true;
       for (int tile = blockIdx.x; ok && tile < args.num_tiles; tile += gridDim.x) {
         int n, x0, y0, slice;
@@ -216,6 +254,7 @@ __global__ void __launch_bounds__(kAdThreads, 1)
         if (!mbar_wait(acce_bar, tile_phase ^ 1u, abort_flag, args.status, kDevTimeoutAdapter)) break;
         tc_fence_after();
         const int nkb = args.num_kb + (bil_mma ? 1 : 0);
+        int hset = 0;  // kb modulo h_accs
         for (int kb = 0; kb < nkb; ++kb) {
           if (!mbar_wait(&full_bar[stage], phase, abort_flag, args.status, kDevTimeoutAdapter)) {
             ok = false;
@@ -227,17 +266,28 @@ __global__ void __launch_bounds__(kAdThreads, 1)
           if (kb < args.num_kb) {
             const uint64_t bdesc = sdesc_kmajor_sw128(sa + kTcAStage);
             const uint64_t udesc = sdesc_kmajor_sw128(sa + kTcAStage + kTcBStage);
+            // (the two products' steps alternate: the small ones, each waiting for the one before on its
+            // accumulator, run behind the large ones)
+            const uint32_t hacc = tmem_base + kHCol + static_cast<uint32_t>(hset * RP);
+            const bool h_more = kb >= ad.h_accs;
+            if (++hset == ad.h_accs) hset = 0;
 #pragma unroll
             for (int k = 0; k < kMmaPerKb; ++k) {
-              const uint32_t acc = (kb > 0 || k > 0) ? 1u : 0u;
-              if (ad.want_out) tc_mma_f16(tmem_base, adesc + 2u * k, bdesc + 2u * k, idesc, acc);
-              if (has) tc_mma_f16(tmem_base + kHCol, adesc + 2u * k, udesc + 2u * k, idesc_u, acc);
+              if (ad.want_out)
+                tc_mma_f16(tmem_base, adesc + 2u * k, bdesc + 2u * k, idesc, (kb > 0 || k > 0) ? 1u : 0u);
+              if (has) tc_mma_f16(hacc, adesc + 2u * k, udesc + 2u * k, idesc_u, (h_more || k > 0) ? 1u : 0u);
             }
           } else {
+            if (!mbar_wait(wfull_bar, tile_phase, abort_flag, args.status, kDevTimeoutAdapter)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            const uint64_t wdesc = sdesc_kmajor_sw128(t_addr);
             const uint64_t bdesc = sdesc_mnmajor_sw128(sa + kTcAStage, kTcCoarseMaxPix * 128);
 #pragma unroll
             for (int k = 0; k < kMmaPerKb; ++k)
-              tc_mma_f16(tmem_base, adesc + 2u * k, bdesc + 128u * k, idesc_bmn, 1u);
+              tc_mma_f16(tmem_base, wdesc + 2u * k, bdesc + 128u * k, idesc_bmn, 1u);
           }
           tc_commit(&empty_bar[stage]);
           if (++stage == S) {
@@ -251,11 +301,10 @@ __global__ void __launch_bounds__(kAdThreads, 1)
           if (ad.want_out) {
             if (!mbar_wait(tfull_bar, h_phase, abort_flag, args.status, kDevTimeoutAdapter)) break;
             tc_fence_after();
-            const uint32_t t = smem_u32(smem + Cfg::kOffT);
-            const uint64_t vdesc = sdesc_kmajor_sw128(smem_u32(smem + Cfg::kOffV));
+            const uint64_t vdesc = sdesc_kmajor_rows<Cfg::kRow>(smem_u32(smem + Cfg::kOffV));
 #pragma unroll
-            for (int part = 0; part < 2; ++part) {
-              const uint64_t tdesc = sdesc_kmajor_sw128(t + part * kTcAStage);
+            for (int part = 0; part < kParts; ++part) {
+              const uint64_t tdesc = sdesc_kmajor_rows<Cfg::kRow>(t_addr + part * Cfg::kPart);
 #pragma unroll
               for (int k = 0; k < RP / 16; ++k)
                 tc_mma_f16(tmem_base, tdesc + 2u * k, vdesc + 2u * k, idesc, 1u);
@@ -273,14 +322,21 @@ __global__ void __launch_bounds__(kAdThreads, 1)
     // ------------------------------------------------------------ epilogue
     const int ew = warp - 2;
     const int quarter = warp & 3;  // TMEM lanes 32 * quarter .. + 31
-    const int chalf = ew >> 2;     // output channels 128 * chalf .. + 127
+    const int chalf = ew >> 2;     // output channels 128 * chalf .. + 127; of h: 0 converts, 1 brings up
     const int row = quarter * 32 + lane;
     const uint32_t lane_addr = static_cast<uint32_t>(quarter * 32) << 16;
-    uint8_t* const my_stage = smem + Cfg::kOffT + ew * kTcStagingPerWarp;
+    const uint32_t t_addr = smem_u32(smem + Cfg::kOffT), v_addr = smem_u32(smem + Cfg::kOffV);
+    constexpr int kCols = Cfg::kStaging / 64;  // channels of 32 pixels that the staging holds
+    uint8_t* const my_stage = smem + Cfg::kOffStaging + ew * Cfg::kStaging;
+    float* const bias_s = reinterpret_cast<float*>(smem + Cfg::kOffBias) + chalf * 128;
     const int tw = args.tile_w;
     const bool taps_global = args.coarse != nullptr && !bil_mma;
     uint32_t tile_phase = 0, h_phase = 0;
     int v_adapter = -1, v_slice = -1;  // what the up region holds
+    // (every warp of a half writes the same values; with channel slices there is no bias)
+    for (int i = lane; i < 128; i += 32)
+      bias_s[i] = args.bias != nullptr ? __ldg(args.bias + chalf * 128 + i) : 0.f;
+    __syncwarp();
     for (int tile = blockIdx.x; tile < args.num_tiles; tile += gridDim.x) {
       int n, x0, y0, slice;
       tc_tile_origin(args, tile, n, x0, y0, slice);
@@ -288,25 +344,48 @@ __global__ void __launch_bounds__(kAdThreads, 1)
       const bool has = adapter >= 0;
       const int py = y0 + row / tw, px = x0 + row % tw;
       const bool valid = py < args.H && px < args.W;
-      uint4* hid = nullptr;  // this thread's pixel of `hidden`: 2 * rank_pad elements
+      // Here the tile before is through: its MMAs have read h, up and the top-down weights.
+      if (bil_mma && chalf == 0) {
+        // this pixel's row of the top-down weights: four of 64 coarse pixels
+        const uint4 z = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) st_shared_v4(t_addr + row * 128 + j * 16, z);
+        const TcTaps tp = tc_taps(py, px, args.H, args.W, args.Hc, args.Wc, args.scale_y, args.scale_x);
+        const int cy0 = static_cast<int>(tc_src(y0, args.scale_y, args.Hc));
+        const int cx0 = static_cast<int>(tc_src(x0, args.scale_x, args.Wc));
+        int k[4] = {(tp.ya - cy0) * args.cbox_w + tp.xa - cx0, (tp.ya - cy0) * args.cbox_w + tp.xb - cx0,
+                    (tp.yb - cy0) * args.cbox_w + tp.xa - cx0, (tp.yb - cy0) * args.cbox_w + tp.xb - cx0};
+        float w[4] = {tp.w00, tp.w01, tp.w10, tp.w11};
+        // (corners that coincide at the map's border add their weights)
+#pragma unroll
+        for (int i = 1; i < 4; ++i)
+#pragma unroll
+          for (int j = 0; j < i; ++j)
+            if (k[i] == k[j] && w[j] != 0.f) {
+              w[j] += w[i];
+              w[i] = 0.f;
+            }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (w[i] == 0.f || k[i] < 0 || k[i] >= args.cbox_w * args.cbox_h) continue;
+          const uint32_t byte = static_cast<uint32_t>(k[i]) * 2u;
+          st_shared_u16(t_addr + row * 128 + ((((byte >> 4) ^ (row & 7)) & 7) << 4) + (byte & 15),
+                        Pack<T>::bits(w[i]));
+        }
+        fence_proxy_async_smem();
+        mbar_arrive(wfull_bar);
+      }
+      uint4* hid = nullptr;  // this thread's pixel of `hidden`: kParts * rank_pad elements
       if (ad.hidden != nullptr && slice == 0 && valid && chalf == 0)
         hid = reinterpret_cast<uint4*>(
             static_cast<uint8_t*>(ad.hidden) +
-            ((static_cast<size_t>(n) * args.H + py) * args.W + px) * ad.rank_pad * 4);
+            ((static_cast<size_t>(n) * args.H + py) * args.W + px) * ad.rank_pad * (2 * kParts));
       if (has) {
-        if (lane == 0) {
-          bulk_wait_group_read<0>();
-          mbar_arrive(sfree_bar);
-        }
-        __syncwarp();
         if (chalf == 1 && ad.want_out && (adapter != v_adapter || slice != v_slice)) {
-          // up[a] (this slice's 256 rows): the MMA that read the last one has completed (this
-          // thread has waited for its accumulator)
+          // up[a] (this slice's 256 rows)
           const uint16_t* v = static_cast<const uint16_t*>(ad.v) + adapter * ad.va;
-          const uint32_t dst = smem_u32(smem + Cfg::kOffV);
-          const int e = (ew - 4) * 32 + lane;
 #pragma unroll 1
-          for (int c = e; c < kTcBlockN; c += 128) {
+          for (int c = row; c < kTcBlockN; c += kTcBlockM) {
             const int ch = slice * kTcBlockN + c;
             const uint16_t* src = v + ch * ad.vc;
 #pragma unroll
@@ -327,62 +406,60 @@ __global__ void __launch_bounds__(kAdThreads, 1)
                   q = make_uint4(w[0], w[1], w[2], w[3]);
                 }
               }
-              st_shared_v4(dst + c * 128 + ((j ^ (c & 7)) << 4), q);
+              st_shared_v4(v_addr + row_chunk<Cfg::kRow>(c, j), q);
             }
           }
-        }
-        if (chalf == 1) {
           v_adapter = adapter;
           v_slice = slice;
         }
         // (every warp waits for the tile's h, so that none runs ahead on the barriers below)
         bool ok = mbar_wait(hfull_bar, h_phase, abort_flag, args.status, kDevTimeoutAdapter);
-        if (chalf == 0)
-          ok = ok && mbar_wait(sfree_bar, h_phase, abort_flag, args.status, kDevTimeoutAdapter);
-        ok = __all_sync(0xffffffffu, ok);
+        if (!__all_sync(0xffffffffu, ok)) break;
         if (chalf == 0) {
-          if (ok) {
-            tc_fence_after();
-            const float s = ad.scale * (ad.scales != nullptr ? __ldg(ad.scales + adapter) : 1.f);
-            const uint32_t t = smem_u32(smem + Cfg::kOffT) + row * 128;
+          const float s = ad.scale * (ad.scales != nullptr ? __ldg(ad.scales + adapter) : 1.f);
+          tc_fence_after();
+          const uint32_t hacc = tmem_base + kHCol + (static_cast<uint32_t>(quarter * 32) << 16);
 #pragma unroll
-            for (int j = 0; j < RP / 8; ++j) {
-              uint32_t r[8];
-              __syncwarp();
-              tmem_ld8(tmem_base + kHCol + j * 8 + lane_addr, r);
+          for (int j = 0; j < RP / 8; ++j) {
+            uint32_t r[8];
+            float h[8];
+            __syncwarp();
+            tmem_ld8(hacc + j * 8, r);
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 8; ++i) h[i] = __uint_as_float(r[i]);
+            for (int q = 1; q < ad.h_accs; ++q) {
+              tmem_ld8(hacc + q * RP + j * 8, r);
               tmem_wait_ld();
-              uint32_t hi[4], lo[4];
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                uint16_t h0, l0, h1, l1;
-                const int c = j * 8 + 2 * i;
-                ad_split<T>(c < ad.rank ? s * __uint_as_float(r[2 * i]) : 0.f, h0, l0);
-                ad_split<T>(c + 1 < ad.rank ? s * __uint_as_float(r[2 * i + 1]) : 0.f, h1, l1);
-                hi[i] = h0 | (static_cast<uint32_t>(h1) << 16);
-                lo[i] = l0 | (static_cast<uint32_t>(l1) << 16);
-              }
-              const uint4 qh = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-              const uint4 ql = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-              const uint32_t off = static_cast<uint32_t>((j ^ (row & 7)) << 4);
-              if (ad.want_out) {
-                st_shared_v4(t + off, qh);
-                st_shared_v4(t + kTcAStage + off, ql);
-              }
-              if (hid != nullptr && j * 8 < ad.rank_pad) {
-                hid[j] = qh;
-                hid[ad.rank_pad / 8 + j] = ql;
-              }
+              for (int i = 0; i < 8; ++i) h[i] += __uint_as_float(r[i]);
+            }
+            uint32_t w[kParts][4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              uint16_t p0[kParts], p1[kParts];
+              const int c = j * 8 + 2 * i;
+              ad_split<T>(c < ad.rank ? s * h[2 * i] : 0.f, p0);
+              ad_split<T>(c + 1 < ad.rank ? s * h[2 * i + 1] : 0.f, p1);
+#pragma unroll
+              for (int part = 0; part < kParts; ++part)
+                w[part][i] = p0[part] | (static_cast<uint32_t>(p1[part]) << 16);
+            }
+#pragma unroll
+            for (int part = 0; part < kParts; ++part) {
+              const uint4 q = make_uint4(w[part][0], w[part][1], w[part][2], w[part][3]);
+              if (ad.want_out) st_shared_v4(t_addr + part * Cfg::kPart + row_chunk<Cfg::kRow>(row, j), q);
+              if (hid != nullptr && j * 8 < ad.rank_pad) hid[(part * ad.rank_pad >> 3) + j] = q;
             }
           }
         }
-        if (!ok) break;
         fence_proxy_async_smem();
         tc_fence_before();
         mbar_arrive(tfull_bar);
         h_phase ^= 1u;
         if (!ad.want_out) mbar_arrive(acce_bar);
       } else if (hid != nullptr) {
-        for (int j = 0; j < ad.rank_pad / 4; ++j) hid[j] = make_uint4(0u, 0u, 0u, 0u);
+        for (int j = 0; j < ad.rank_pad * kParts / 8; ++j) hid[j] = make_uint4(0u, 0u, 0u, 0u);
       }
       if (!ad.want_out) continue;
 
@@ -416,29 +493,27 @@ __global__ void __launch_bounds__(kAdThreads, 1)
       }
       const int ox = x0 + (quarter * 32) % tw, oy = y0 + (quarter * 32) / tw;
       const int scol = slice * kTcBlockN;
-      const uint32_t stage_addr = smem_u32(my_stage) + lane * 128;
+      const uint32_t stage_addr = smem_u32(my_stage);
 #pragma unroll
-      for (int step = 0; step < 2; ++step) {
-        const int col0 = chalf * 128 + step * 64;
+      for (int step = 0; step < 128 / kCols; ++step) {
+        const int col0 = chalf * 128 + step * kCols;
         if (lane == 0) bulk_wait_group_read<0>();
         __syncwarp();
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
+        for (int j = 0; j < kCols / 8; ++j) {
           float v[8];
-          const int c = col0 + j * 8;
+          const int c = step * kCols + j * 8;  // of the warp's 128
+          const float4 b0 = *reinterpret_cast<const float4*>(bias_s + c);
+          const float4 b1 = *(reinterpret_cast<const float4*>(bias_s + c) + 1);
+          const float bb[8] = {b0.x, b0.y, b0.z, b0.w, b1.x, b1.y, b1.z, b1.w};
 #pragma unroll
-          for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(rr[step * 64 + j * 8 + i]);
-          if (args.bias != nullptr) {
-            const float4 b0 = __ldg(reinterpret_cast<const float4*>(args.bias + scol + c));
-            const float4 b1 = __ldg(reinterpret_cast<const float4*>(args.bias + scol + c) + 1);
-            v[0] += b0.x, v[1] += b0.y, v[2] += b0.z, v[3] += b0.w;
-            v[4] += b1.x, v[5] += b1.y, v[6] += b1.z, v[7] += b1.w;
-          }
+          for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(rr[c + i]) + bb[i];
           if (taps_global) {
-            const uint4 q[4] = {__ldg(reinterpret_cast<const uint4*>(cb + o00 + c * 2)),
-                                __ldg(reinterpret_cast<const uint4*>(cb + o01 + c * 2)),
-                                __ldg(reinterpret_cast<const uint4*>(cb + o10 + c * 2)),
-                                __ldg(reinterpret_cast<const uint4*>(cb + o11 + c * 2))};
+            const int o = (chalf * 128 + c) * 2;
+            const uint4 q[4] = {__ldg(reinterpret_cast<const uint4*>(cb + o00 + o)),
+                                __ldg(reinterpret_cast<const uint4*>(cb + o01 + o)),
+                                __ldg(reinterpret_cast<const uint4*>(cb + o10 + o)),
+                                __ldg(reinterpret_cast<const uint4*>(cb + o11 + o))};
             const float w[4] = {tp.w00, tp.w01, tp.w10, tp.w11};
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
@@ -451,7 +526,7 @@ __global__ void __launch_bounds__(kAdThreads, 1)
               }
             }
           }
-          st_shared_v4(stage_addr + ((j ^ (lane & 7)) << 4),
+          st_shared_v4(stage_addr + row_chunk<kCols * 2>(lane, j),
                        make_uint4(Pack<T>::pack(v[0], v[1]), Pack<T>::pack(v[2], v[3]),
                                   Pack<T>::pack(v[4], v[5]), Pack<T>::pack(v[6], v[7])));
         }
@@ -478,14 +553,15 @@ __global__ void __launch_bounds__(kAdThreads, 1)
 }
 
 // ------------------------------------------------------------------ adapter gradients
-// part[unit][r][c] = sum over the unit's pixels of h[p][r] q[p][c], h = hi + lo: for the channel
-// blocks of x with h = dh (ddown), and for dy with h (dup).  A tcgen05 GEMM over pixels (both
-// operands MN-major 64-pixel boxes): M = 256 channels in two accumulators, N = 2 rank_pad columns,
-// the hi and lo parts side by side, added when the accumulators are read.
+// part[unit][r][c] = sum over the unit's pixels of h[p][r] q[p][c]: for the channel blocks of x with
+// h = dh (ddown), and for dy with h (dup).  A tcgen05 GEMM over pixels (both operands MN-major
+// 64-pixel boxes): M = 256 channels in two accumulators, N = parts x rank_pad columns, the parts of
+// h side by side, added when the accumulators are read.  Where TMEM has room (N <= 128), the k-blocks
+// alternate over two pairs of accumulators: at most 64 steps on one (see the rounding above).
 constexpr int kAgChunk = 64 * 128;
 constexpr int kAgStages = 4;
 constexpr int kAgQ = 4 * kAgChunk;                 // 256 channels
-constexpr int kAgStage = kAgQ + 2 * kAgChunk;      // + up to 128 columns of h
+constexpr int kAgStage = kAgQ + 3 * kAgChunk;      // + up to 192 columns of h
 constexpr int kAgOffBars = kAgStages * kAgStage;
 constexpr int kAgSmemBytes = kAgOffBars + 256 + 1024;
 static_assert(kAgSmemBytes <= 232448, "adapter gradient smem");
@@ -502,7 +578,7 @@ struct AgArgs {
 };
 
 template <typename T>
-__global__ void __launch_bounds__(kAdThreads, 1)
+__global__ void __launch_bounds__(kTcThreads, 1)
     fpn_adapter_grad_kernel(const __grid_constant__ CUtensorMap map_x,
                             const __grid_constant__ CUtensorMap map_dy,
                             const __grid_constant__ CUtensorMap map_dh,
@@ -532,8 +608,10 @@ __global__ void __launch_bounds__(kAdThreads, 1)
   const CUtensorMap* mh = is_x ? &map_dh : &map_h;
   const int c0 = is_x ? block * 256 : 0;
   const int kb0 = split * a.per, kb1 = min(a.num_kb, kb0 + a.per);  // non-empty (host)
-  const int cols = 2 * a.rank_pad;
+  constexpr int kParts = kAdParts<T>;
+  const int cols = (kParts * a.rank_pad + 15) / 16 * 16;  // (columns past the parts are zeros)
   const int hchunks = (cols + 63) / 64;
+  const int sets = cols <= 128 ? 2 : 1;  // accumulators at columns 256 * half + 128 * set
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < S; ++s) {
@@ -547,7 +625,7 @@ __global__ void __launch_bounds__(kAdThreads, 1)
     prefetch_tmap(mh);
   }
   if (warp == 1) {
-    tmem_alloc(tmem_slot, 256);
+    tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
   tc_fence_before();
@@ -603,9 +681,10 @@ __global__ void __launch_bounds__(kAdThreads, 1)
         const uint64_t b = sdesc_mnmajor_sw128(q + kAgQ, kAgChunk);
 #pragma unroll
         for (int k = 0; k < kMmaPerKb; ++k) {  // 16 pixels per step
-          const uint32_t acc = (kb > kb0 || k > 0) ? 1u : 0u;
-          tc_mma_f16(tmem_base, a0 + 128u * k, b + 128u * k, idesc, acc);
-          tc_mma_f16(tmem_base + 128, a1 + 128u * k, b + 128u * k, idesc, acc);
+          const uint32_t set = (kb - kb0) % sets, d = tmem_base + 128u * set;
+          const uint32_t acc = (kb - kb0 >= sets || k > 0) ? 1u : 0u;
+          tc_mma_f16(d, a0 + 128u * k, b + 128u * k, idesc, acc);
+          tc_mma_f16(d + 256, a1 + 128u * k, b + 128u * k, idesc, acc);
         }
         tc_commit(&empty_bar[stage]);
         if (++stage == S) {
@@ -622,19 +701,25 @@ __global__ void __launch_bounds__(kAdThreads, 1)
     const bool ok = mbar_wait(accf_bar, 0, abort_flag, a.status, kDevTimeoutAdapter);
     if (__all_sync(0xffffffffu, ok)) {
       tc_fence_after();
-      const uint32_t acc = tmem_base + half * 128 + (static_cast<uint32_t>(quarter * 32) << 16);
+      const uint32_t acc = tmem_base + half * 256 + (static_cast<uint32_t>(quarter * 32) << 16);
+      const int used = min(sets, kb1 - kb0);
       float* dst = a.part + ((static_cast<size_t>(n - a.n0) * a.splits + split) * a.blocks + block) *
                                 a.rank_pad * 256 +
                    half * 128 + quarter * 32 + lane;
       for (int r = 0; r < a.rank_pad; r += 8) {
-        uint32_t hi[8], lo[8];
-        __syncwarp();
-        tmem_ld8(acc + r, hi);
-        tmem_ld8(acc + a.rank_pad + r, lo);
-        tmem_wait_ld();
+        float sum[8] = {};
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          dst[(r + i) * 256] = __uint_as_float(hi[i]) + __uint_as_float(lo[i]);
+        for (int part = kParts - 1; part >= 0; --part)  // the smallest first
+          for (int set = 0; set < used; ++set) {
+            uint32_t v[8];
+            __syncwarp();
+            tmem_ld8(acc + 128 * set + part * a.rank_pad + r, v);
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sum[i] += __uint_as_float(v[i]);
+          }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) dst[(r + i) * 256] = sum[i];
       }
     }
   }
@@ -643,7 +728,7 @@ __global__ void __launch_bounds__(kAdThreads, 1)
   if (warp == 1) {
     __syncwarp();
     tc_fence_after();
-    tmem_dealloc(tmem_base, 256);
+    tmem_dealloc(tmem_base, 512);
   }
 }
 
@@ -708,8 +793,9 @@ __global__ void __launch_bounds__(256) adapter_transpose_kernel(const uint16_t* 
 
 // ------------------------------------------------------------------ host side
 template <typename T, int RP>
-cudaError_t launch_adapter_rp(const TcPlan& p, const CUtensorMap& map_u, const AdArgs& ad, cudaStream_t s) {
-  using Cfg = AdCfg<RP>;
+cudaError_t launch_adapter_rp(const TcPlan& p, const CUtensorMap& map_u, const AdArgs& ad, void* out,
+                              cudaStream_t s) {
+  using Cfg = AdCfg<RP, kAdParts<T>>;
   auto kern = fpn_adapter_kernel<T, RP>;
   static std::atomic<bool> configured[64];
   cudaError_t e = once_per_device(configured, [&] {
@@ -718,17 +804,26 @@ cudaError_t launch_adapter_rp(const TcPlan& p, const CUtensorMap& map_u, const A
   if (e != cudaSuccess) return e;
   TcGemmArgs a;
   std::memcpy(&a, p.args, sizeof(a));
+  CUtensorMap map_out = p.map_out;
+  if (Cfg::kStaging != 4096 && ad.want_out) {  // stores of 32 channels
+    const int sw = a.tile_w < 32 ? a.tile_w : 32;
+    const int C = a.out_cols ? a.out_cols : kTcBlockN;
+    e = encode_nhwc_cols_map(&map_out, p.dtype, out, a.N_img, a.H, a.W, C, sw, 32 / sw, 32);
+    if (e != cudaSuccess) return e;
+  }
   return launch_ex(kern, dim3(p.grid), dim3(kAdThreads), Cfg::kSmemBytes, s, LaunchOpts(), 1, p.map_a,
-                   p.map_b, p.map_out, p.map_coarse, map_u, a, ad);
+                   p.map_b, map_out, p.map_coarse, map_u, a, ad);
 }
 template <typename T>
-cudaError_t launch_adapter_t(const TcPlan& p, const CUtensorMap& map_u, const AdArgs& ad, cudaStream_t s) {
-  if (ad.rank <= 16) return launch_adapter_rp<T, 16>(p, map_u, ad, s);
-  if (ad.rank <= 32) return launch_adapter_rp<T, 32>(p, map_u, ad, s);
-  return launch_adapter_rp<T, 64>(p, map_u, ad, s);
+cudaError_t launch_adapter_t(const TcPlan& p, const CUtensorMap& map_u, const AdArgs& ad, void* out,
+                             cudaStream_t s) {
+  if (ad.rank <= 16) return launch_adapter_rp<T, 16>(p, map_u, ad, out, s);
+  if (ad.rank <= 32) return launch_adapter_rp<T, 32>(p, map_u, ad, out, s);
+  return launch_adapter_rp<T, 64>(p, map_u, ad, out, s);
 }
 
 int pad8(int v) { return (v + 7) / 8 * 8; }
+int parts_of(DType dt) { return dt == DType::BF16 ? kAdParts<__nv_bfloat16> : kAdParts<__half>; }
 int rank_tile(int rank) { return rank <= 16 ? 16 : rank <= 32 ? 32 : 64; }
 size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 
@@ -773,7 +868,8 @@ AgPlan adapter_grad_plan(const AdapterProblem& p) {
   const long long units = static_cast<long long>(p.N) * g.blocks;
   int k = static_cast<int>(std::max<long long>(1, sm_count() / units));
   k = std::min(k, std::max(1, g.num_kb / 4));
-  g.per = (g.num_kb + k - 1) / k;
+  const int most = (parts_of(p.dtype) * pad8(p.rank) + 15) / 16 * 16 <= 128 ? 32 : 16;  // k-blocks
+  g.per = std::min(most, (g.num_kb + k - 1) / k);
   g.splits = (g.num_kb + g.per - 1) / g.per;
   g.image_bytes = static_cast<size_t>(g.splits) * g.blocks * pad8(p.rank) * 256 * sizeof(float);
   g.images = static_cast<int>(std::min<size_t>(p.N, std::max<size_t>(1, (256u << 20) / g.image_bytes)));
@@ -788,7 +884,7 @@ AdWorkspace adapter_workspace(const AdapterProblem& p, bool own_w_t) {
   w.up_t = 0;
   w.w_t = w.up_t + align256(static_cast<size_t>(p.adapters) * p.rank * 256 * 2);
   w.dh = w.w_t + (own_w_t ? static_cast<size_t>((p.Cin + 255) / 256) * 256 * 256 * 2 : 0);
-  w.part = w.dh + align256(static_cast<size_t>(p.N) * p.H * p.W * 2 * pad8(p.rank) * 2);
+  w.part = w.dh + align256(static_cast<size_t>(p.N) * p.H * p.W * parts_of(p.dtype) * pad8(p.rank) * 2);
   const AgPlan g = adapter_grad_plan(p);
   w.total = w.part + g.images * g.image_bytes;
   return w;
@@ -799,7 +895,7 @@ cudaError_t adapter_grads_t(const AdapterProblem& p, const void* x, const void* 
                             const void* h, float* part, float* ddown, float* dup, int* status,
                             cudaStream_t s) {
   const AgPlan g = adapter_grad_plan(p);
-  const int hw = p.H * p.W, hc = 2 * pad8(p.rank);
+  const int hw = p.H * p.W, hc = parts_of(p.dtype) * pad8(p.rank);
   CUtensorMap mx, my, mdh, mh;
   cudaError_t e = encode_nhwc_map(&mx, p.dtype, x, p.N, 1, hw, p.Cin, p.Cin, 64, 1);
   if (e == cudaSuccess) e = encode_nhwc_map(&my, p.dtype, dy, p.N, 1, hw, 256, 256, 64, 1);
@@ -829,7 +925,7 @@ cudaError_t adapter_grads_t(const AdapterProblem& p, const void* x, const void* 
     a.rank_pad = pad8(p.rank);
     a.part = part;
     a.status = status;
-    e = launch_ex(kern, dim3(static_cast<unsigned>(images) * g.splits * g.blocks), dim3(kAdThreads),
+    e = launch_ex(kern, dim3(static_cast<unsigned>(images) * g.splits * g.blocks), dim3(kTcThreads),
                   kAgSmemBytes, s, LaunchOpts(), 1, mx, my, mdh, mh, a);
     if (e != cudaSuccess) return e;
     ArArgs r;
@@ -885,8 +981,9 @@ cudaError_t launch_lateral_adapters(const AdapterProblem& p, const void* x, cons
   ad.hidden = hidden;
   ad.rank_pad = pad8(p.rank);
   ad.want_out = 1;
-  return p.dtype == DType::BF16 ? launch_adapter_t<__nv_bfloat16>(plan, map_u, ad, s)
-                                : launch_adapter_t<__half>(plan, map_u, ad, s);
+  ad.h_accs = ad_h_accs((p.Cin + 63) / 64);
+  return p.dtype == DType::BF16 ? launch_adapter_t<__nv_bfloat16>(plan, map_u, ad, out, s)
+                                : launch_adapter_t<__half>(plan, map_u, ad, out, s);
 }
 
 size_t lateral_adapters_workspace_bytes(const AdapterProblem& p, bool has_w_t, bool need_dx) {
@@ -938,8 +1035,9 @@ cudaError_t launch_lateral_adapters_backward(const AdapterProblem& p, const void
   ad.hidden = dh;
   ad.rank_pad = pad8(p.rank);
   ad.want_out = dx != nullptr;
-  e = p.dtype == DType::BF16 ? launch_adapter_t<__nv_bfloat16>(plan, map_u, ad, s)
-                             : launch_adapter_t<__half>(plan, map_u, ad, s);
+  ad.h_accs = ad_h_accs(4);
+  e = p.dtype == DType::BF16 ? launch_adapter_t<__nv_bfloat16>(plan, map_u, ad, dx, s)
+                             : launch_adapter_t<__half>(plan, map_u, ad, dx, s);
   if (e != cudaSuccess) return e;
   float* part = reinterpret_cast<float*>(base + wl.part);
   return p.dtype == DType::BF16

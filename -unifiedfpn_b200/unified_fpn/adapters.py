@@ -19,6 +19,7 @@ from .ops import _DT
 
 _CL = torch.channels_last
 MAX_RANK = 64
+_PARTS = {torch.bfloat16: 3, torch.float16: 2}  # 16-bit values that make up one of h
 
 
 def _cl(t: torch.Tensor) -> torch.Tensor:
@@ -90,8 +91,8 @@ def fpn_lateral_adapters(input: torch.Tensor, weight: torch.Tensor, bias: torch.
     ``index``: one integer per image on the device, values outside 0 .. L - 1 (-1 by convention) run
     without an adapter; ``scale``: a number, or [L] on the device.  ``weight`` [256, Cin] or [256,
     Cin, 1, 1], ``bias`` [256], Cin a multiple of 8, at most 2048.  Sums are fp32 and rounded once;
-    h is carried in two 16-bit parts.  With ``return_hidden`` also returns h in that form (opaque,
-    [N, H, W, 2, R rounded up to 8]) for :func:`fpn_lateral_adapters_backward`."""
+    h is carried in 16-bit parts, 3 of bf16 or 2 of fp16.  With ``return_hidden`` also returns h in that
+    form (opaque, [N, H, W, parts, R rounded up to 8]) for :func:`fpn_lateral_adapters_backward`."""
     down, up, index, scales, scale = _check(input, down, up, index, scale)
     x = _cl(input)
     n, cin, h, w = x.shape
@@ -109,7 +110,8 @@ def fpn_lateral_adapters(input: torch.Tensor, weight: torch.Tensor, bias: torch.
         hc, wc = coarse.shape[2:]
     rank = down.shape[1]
     out = torch.empty((n, 256, h, w), dtype=x.dtype, device=dev, memory_format=_CL)
-    hidden = torch.empty((n, h, w, 2, (rank + 7) // 8 * 8), dtype=x.dtype, device=dev) if return_hidden else None
+    hidden = torch.empty((n, h, w, _PARTS[x.dtype], (rank + 7) // 8 * 8), dtype=x.dtype,
+                         device=dev) if return_hidden else None
 
     def call():
         return lib.ufpn_lateral_adapters(
@@ -141,7 +143,7 @@ def fpn_lateral_adapters_backward(input: torch.Tensor, weight: torch.Tensor | No
         raise ValueError("grad_output must be [N, 256, H, W] in the input's dtype")
     g = _cl(grad_output)
     count, rank = down.shape[:2]
-    if hidden.dtype is not x.dtype or tuple(hidden.shape) != (n, h, w, 2, (rank + 7) // 8 * 8) \
+    if hidden.dtype is not x.dtype or tuple(hidden.shape) != (n, h, w, _PARTS[x.dtype], (rank + 7) // 8 * 8) \
             or hidden.device != dev or not hidden.is_contiguous():
         raise ValueError("hidden must be what the forward returned")
     wt = wtt = None

@@ -276,6 +276,9 @@ bool tc_use_wide_epilogue(TcPlan& plan);
 // elements (>= C), box (one 128-byte row of channels, bw, bh, 1).
 cudaError_t encode_nhwc_map(CUtensorMap* map, DType dt, const void* base, int N, int H, int W,
                             int C, int pix_stride, int bw, int bh);
+// The same with boxes of `cols` channels of 64 or 128 bytes, under the swizzle of that width.
+cudaError_t encode_nhwc_cols_map(CUtensorMap* map, DType dt, const void* base, int N, int H, int W,
+                                 int C, int bw, int bh, int cols);
 // 16-bit lateral plans only: store the output into channels [0, C) of a map whose pixels are
 // pix_stride elements apart (out = that channel slice's first element).  Used to write the
 // 256-channel slices of a wider tensor (the input gradient of a Cin > 256 lateral).
@@ -434,7 +437,7 @@ struct AdapterProblem {
   float scale;          // times scales[a]
 };
 // out = x w^T + bias + h up[a]^T [+ bilinear(coarse)], h = scale x down[a]^T; hidden (optional):
-// [pixels][2][rank padded to 8] 16-bit, h as hi + lo.
+// [pixels][parts][rank padded to 8], h as the sum of 3 (bf16) or 2 (fp16) parts.
 cudaError_t launch_lateral_adapters(const AdapterProblem& p, const void* x, const void* w,
                                     const float* bias, const void* down, const void* up,
                                     const void* coarse, int Hc, int Wc, void* out, void* hidden,

@@ -284,8 +284,9 @@ int ufpn_conv3x3_act(int dtype, const void* x, const void* w, const float* bias,
  * every tensor 16-byte aligned.  No reference counterpart.
  *   down [adapters][rank][Cin], up [adapters][256][rank], index int32 [N] on the device, scales fp32
  *   [adapters] on the device or NULL (1); coarse as ufpn_lateral_conv, or NULL.
- *   hidden: NULL, or [N * H * W][2][rank rounded up to 8] elements that receive h for the backward
- *   (the 16-bit value nearest to h, then the nearest to what is left; zeros without an adapter). */
+ *   hidden: NULL, or [N * H * W][parts][rank rounded up to 8] elements that receive h for the
+ *   backward, in 3 parts (BF16) or 2 (F16): the 16-bit value nearest to h, then the nearest to what
+ *   is left; zeros without an adapter. */
 int ufpn_lateral_adapters(int dtype, const void* x, const void* w, const float* bias,
                           const void* down, const void* up, const int* index, const float* scales,
                           float scale, const void* coarse, void* out, void* hidden, int N, int Cin,
