@@ -32,9 +32,11 @@ namespace ufpn {
 namespace {
 
 constexpr int kAdMaxRank = 64;
-constexpr int kAdEpiWarps = 8;
-// TMA warp, MMA warp, 8 epilogue warps (at 168 registers a thread: each keeps a row of 128 accumulators)
+// TMA warp, MMA warp, 16 epilogue warps: what the epilogue does for a tile is one long chain of
+// instructions, so that twice the warps halve its time (8 warps: about 6000 cycles a tile).
+constexpr int kAdEpiWarps = 16;
 constexpr int kAdThreads = 64 + 32 * kAdEpiWarps;
+constexpr int kAdWarpCols = kTcBlockN / (kAdEpiWarps / 4);  // output channels of a warp
 constexpr int kDevTimeoutAdapter = 0x107;
 
 template <typename T>
@@ -58,18 +60,20 @@ __device__ __forceinline__ uint32_t row_chunk(int row, int chunk) {
   return static_cast<uint32_t>(row * RB + ((chunk ^ ((row * RB / 128) & (RB / 16 - 1))) << 4));
 }
 
-// Shared memory of fpn_adapter_kernel for ranks up to RP.
+// Shared memory of fpn_adapter_kernel for ranks up to RP.  (Keeping 256 x 256 weights resident instead
+// of streaming them with every tile changed nothing: 148 against 146 us on P2 of eight images.)
 template <int RP, int kParts>
 struct AdCfg {
   static constexpr int kRow = RP * 2;   // bytes of a row of h or up
   static constexpr int kU = RP * 128;   // one k-block of down[a]
-  static constexpr int kStage = kTcAStage + kTcBStage + kU;
+  static constexpr int kOffU = kTcAStage + kTcBStage;
+  static constexpr int kStage = kOffU + kU;
   static constexpr int kStages = RP <= 32 ? 3 : 2;  // (three of 56 KB would not fit)
   static constexpr int kPart = kTcBlockM * kRow;
   // h's parts; before them, in the same place, the top-down weights (their MMA is over when h is)
   static constexpr int kT = kParts * kPart > kTcAStage ? kParts * kPart : kTcAStage;
-  static constexpr int kStaging = RP <= 16 ? 4096 : 2048;  // per storing warp: 32 pixels
-  static constexpr int kOffV = kStages * kStage;           // up[a]: 256 rows
+  static constexpr int kStaging = 1024;  // per epilogue warp: 32 pixels x 16 channels
+  static constexpr int kOffV = kStages * kStage;  // up[a]: 256 rows
   static constexpr int kOffT = kOffV + kTcBlockN * kRow;
   static constexpr int kOffStaging = kOffT + kT;
   static constexpr int kOffBias = kOffStaging + kAdEpiWarps * kStaging;
@@ -92,6 +96,8 @@ struct AdArgs {
   int rank_pad;  // rank rounded up to 8
   int want_out;  // 0: only hidden
   int h_accs;    // accumulators that h's k-blocks alternate over
+  void* out;     // NHWC, out_c channels
+  int out_c;
 };
 constexpr int kAdMaxHAccs = 4;
 int ad_h_accs(int num_kb) { return std::min(kAdMaxHAccs, (num_kb + 7) / 8); }
@@ -113,11 +119,11 @@ __device__ __forceinline__ void ad_split(float v, uint16_t (&part)[kAdParts<T>])
   }
 }
 
-template <typename T, int RP>
+// kTaps: the top-down taps are added from global memory in the epilogue (their box exceeds 64 pixels).
+template <typename T, int RP, bool kTaps>
 __global__ void __launch_bounds__(kAdThreads, 1)
     fpn_adapter_kernel(const __grid_constant__ CUtensorMap map_a,
                        const __grid_constant__ CUtensorMap map_b,
-                       const __grid_constant__ CUtensorMap map_out,
                        const __grid_constant__ CUtensorMap map_coarse,
                        const __grid_constant__ CUtensorMap map_u, const TcGemmArgs args,
                        const AdArgs ad) {
@@ -136,12 +142,13 @@ __global__ void __launch_bounds__(kAdThreads, 1)
   uint64_t* tfull_bar = accf_bar + 3;  // h and up in shared memory
   uint64_t* wfull_bar = accf_bar + 4;  // the top-down weights in shared memory
   uint64_t* done_bar = accf_bar + 5;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done_bar + 1);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(accf_bar + 6);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
-  const bool bil_mma = args.coarse != nullptr && args.cbox_w > 0;
+  const bool bil_mma = !kTaps && args.coarse != nullptr;
+  const int nkb = args.num_kb + (bil_mma ? 1 : 0);  // k-blocks of a tile: the products', the top-down add's
   constexpr uint32_t kHCol = kTcBlockN;  // h accumulators: TMEM columns from 256, RP each
 
   if (threadIdx.x == 0) {
@@ -160,7 +167,6 @@ __global__ void __launch_bounds__(kAdThreads, 1)
     prefetch_tmap(&map_a);
     prefetch_tmap(&map_b);
     prefetch_tmap(&map_u);
-    prefetch_tmap(&map_out);
     if (bil_mma) prefetch_tmap(&map_coarse);
   }
   if (warp == 1) {
@@ -178,13 +184,12 @@ __global__ void __launch_bounds__(kAdThreads, 1)
     int stage = 0, issued = 0;
     uint32_t phase = 0;
     bool ok = true;
-    const uint32_t coarse_bytes = static_cast<uint32_t>(args.cbox_w * args.cbox_h * 128 * 4);
+    const uint32_t box_bytes = static_cast<uint32_t>(args.cbox_w * args.cbox_h * 128);  // 64 channels
     for (int tile = blockIdx.x; ok && tile < args.num_tiles; tile += gridDim.x) {
       int n, x0, y0, slice;
       tc_tile_origin(args, tile, n, x0, y0, slice);
       const int adapter = ad_adapter(ad, n);
       if (!ad.want_out && adapter < 0) continue;
-      const int nkb = args.num_kb + (bil_mma ? 1 : 0);
       for (int kb = 0; kb < nkb; ++kb) {
         ok = mbar_wait(&empty_bar[stage], phase ^ 1u, abort_flag, args.status, kDevTimeoutAdapter);
         if (!__all_sync(0xffffffffu, ok)) {
@@ -192,27 +197,28 @@ __global__ void __launch_bounds__(kAdThreads, 1)
           break;
         }
         uint8_t* const sa = smem + stage * Cfg::kStage;
-        uint8_t* const sb = sa + kTcAStage;
-        uint8_t* const su = sb + kTcBStage;
+        uint8_t* const su = sa + Cfg::kOffU;
         if (kb < args.num_kb) {
           if (lane == 0) {
             mbar_arrive_expect_tx(&full_bar[stage], kTcAStage + (ad.want_out ? kTcBStage : 0) +
                                                         (adapter >= 0 ? Cfg::kU : 0));
             tma_load_4d(sa, &map_a, &full_bar[stage], kb * 64, x0, y0, n, kPolicyEvictFirst);
             if (ad.want_out)
-              tma_load_2d(sb, &map_b, &full_bar[stage], kb * 64, slice * kTcBlockN, kPolicyEvictLast);
+              tma_load_2d(sa + kTcAStage, &map_b, &full_bar[stage], kb * 64, slice * kTcBlockN,
+                          kPolicyEvictLast);
             if (adapter >= 0)
               tma_load_4d(su, &map_u, &full_bar[stage], kb * 64, 0, 0, adapter, kPolicyEvictLast);
           }
         } else {
-          // top-down k-block: the tile's coarse box as the B operand (the weights: the h warps)
+          // top-down k-block: the tile's coarse box as the B operand (the weights: the epilogue)
+          uint8_t* const sb = sa + kTcAStage;
           tc_zero_btail(sb, lane, args.cbox_w * args.cbox_h, 4);
           fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) {
             const int cy = static_cast<int>(tc_src(y0, args.scale_y, args.Hc));
             const int cx = static_cast<int>(tc_src(x0, args.scale_x, args.Wc));
-            mbar_arrive_expect_tx(&full_bar[stage], coarse_bytes);
+            mbar_arrive_expect_tx(&full_bar[stage], box_bytes * 4);
             for (int b = 0; b < 4; ++b)
               tma_load_4d(sb + b * (kTcCoarseMaxPix * 128), &map_coarse, &full_bar[stage], b * 64, cx,
                           cy, n, kPolicyEvictLast);
@@ -253,7 +259,6 @@ __global__ void __launch_bounds__(kAdThreads, 1)
         if (!ad.want_out && !has) continue;
         if (!mbar_wait(acce_bar, tile_phase ^ 1u, abort_flag, args.status, kDevTimeoutAdapter)) break;
         tc_fence_after();
-        const int nkb = args.num_kb + (bil_mma ? 1 : 0);
         int hset = 0;  // kb modulo h_accs
         for (int kb = 0; kb < nkb; ++kb) {
           if (!mbar_wait(&full_bar[stage], phase, abort_flag, args.status, kDevTimeoutAdapter)) {
@@ -265,7 +270,7 @@ __global__ void __launch_bounds__(kAdThreads, 1)
           const uint64_t adesc = sdesc_kmajor_sw128(sa);
           if (kb < args.num_kb) {
             const uint64_t bdesc = sdesc_kmajor_sw128(sa + kTcAStage);
-            const uint64_t udesc = sdesc_kmajor_sw128(sa + kTcAStage + kTcBStage);
+            const uint64_t udesc = sdesc_kmajor_sw128(sa + Cfg::kOffU);
             // (the two products' steps alternate: the small ones, each waiting for the one before on its
             // accumulator, run behind the large ones)
             const uint32_t hacc = tmem_base + kHCol + static_cast<uint32_t>(hset * RP);
@@ -322,34 +327,32 @@ __global__ void __launch_bounds__(kAdThreads, 1)
     // ------------------------------------------------------------ epilogue
     const int ew = warp - 2;
     const int quarter = warp & 3;  // TMEM lanes 32 * quarter .. + 31
-    const int chalf = ew >> 2;     // output channels 128 * chalf .. + 127; of h: 0 converts, 1 brings up
+    const int cq = ew >> 2;        // output channels 64 * cq .. + 63
     const int row = quarter * 32 + lane;
     const uint32_t lane_addr = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t t_addr = smem_u32(smem + Cfg::kOffT), v_addr = smem_u32(smem + Cfg::kOffV);
-    constexpr int kCols = Cfg::kStaging / 64;  // channels of 32 pixels that the staging holds
-    uint8_t* const my_stage = smem + Cfg::kOffStaging + ew * Cfg::kStaging;
-    float* const bias_s = reinterpret_cast<float*>(smem + Cfg::kOffBias) + chalf * 128;
-    const int tw = args.tile_w;
-    const bool taps_global = args.coarse != nullptr && !bil_mma;
+    const uint32_t stage_addr = smem_u32(smem + Cfg::kOffStaging + ew * Cfg::kStaging);
+    float* const bias_s = reinterpret_cast<float*>(smem + Cfg::kOffBias) + cq * kAdWarpCols;
+    const int tw_shift = 31 - __clz(args.tile_w), tw_mask = args.tile_w - 1;  // (a power of two)
     uint32_t tile_phase = 0, h_phase = 0;
     int v_adapter = -1, v_slice = -1;  // what the up region holds
-    // (every warp of a half writes the same values; with channel slices there is no bias)
-    for (int i = lane; i < 128; i += 32)
-      bias_s[i] = args.bias != nullptr ? __ldg(args.bias + chalf * 128 + i) : 0.f;
+    // (each of the four warps writes the same values; with channel slices there is no bias)
+    for (int i = lane; i < kAdWarpCols; i += 32)
+      bias_s[i] = args.bias != nullptr ? __ldg(args.bias + cq * kAdWarpCols + i) : 0.f;
     __syncwarp();
     for (int tile = blockIdx.x; tile < args.num_tiles; tile += gridDim.x) {
       int n, x0, y0, slice;
       tc_tile_origin(args, tile, n, x0, y0, slice);
       const int adapter = ad_adapter(ad, n);
       const bool has = adapter >= 0;
-      const int py = y0 + row / tw, px = x0 + row % tw;
+      const int py = y0 + (row >> tw_shift), px = x0 + (row & tw_mask);
       const bool valid = py < args.H && px < args.W;
       // Here the tile before is through: its MMAs have read h, up and the top-down weights.
-      if (bil_mma && chalf == 0) {
+      if (bil_mma && cq == 0) {
         // this pixel's row of the top-down weights: four of 64 coarse pixels
         const uint4 z = make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) st_shared_v4(t_addr + row * 128 + j * 16, z);
+        for (int j = 0; j < 8; ++j) st_shared_v4(t_addr + row * 128 + ((j ^ (row & 7)) << 4), z);
         const TcTaps tp = tc_taps(py, px, args.H, args.W, args.Hc, args.Wc, args.scale_y, args.scale_x);
         const int cy0 = static_cast<int>(tc_src(y0, args.scale_y, args.Hc));
         const int cx0 = static_cast<int>(tc_src(x0, args.scale_x, args.Wc));
@@ -376,81 +379,77 @@ __global__ void __launch_bounds__(kAdThreads, 1)
         mbar_arrive(wfull_bar);
       }
       uint4* hid = nullptr;  // this thread's pixel of `hidden`: kParts * rank_pad elements
-      if (ad.hidden != nullptr && slice == 0 && valid && chalf == 0)
+      if (ad.hidden != nullptr && slice == 0 && valid)
         hid = reinterpret_cast<uint4*>(
             static_cast<uint8_t*>(ad.hidden) +
             ((static_cast<size_t>(n) * args.H + py) * args.W + px) * ad.rank_pad * (2 * kParts));
       if (has) {
-        if (chalf == 1 && ad.want_out && (adapter != v_adapter || slice != v_slice)) {
-          // up[a] (this slice's 256 rows)
-          const uint16_t* v = static_cast<const uint16_t*>(ad.v) + adapter * ad.va;
-#pragma unroll 1
-          for (int c = row; c < kTcBlockN; c += kTcBlockM) {
-            const int ch = slice * kTcBlockN + c;
-            const uint16_t* src = v + ch * ad.vc;
-#pragma unroll
-            for (int j = 0; j < RP / 8; ++j) {
-              uint4 q = make_uint4(0u, 0u, 0u, 0u);
-              if (ch < ad.v_rows && j * 8 < ad.rank) {
-                if (ad.v_vec) {
-                  q = __ldg(reinterpret_cast<const uint4*>(src) + j);
-                } else {
-                  uint32_t w[4];
-#pragma unroll
-                  for (int i = 0; i < 4; ++i) {
-                    const int r = j * 8 + 2 * i;
-                    const uint32_t lo = r < ad.rank ? __ldg(src + r * ad.vr) : 0;
-                    const uint32_t hi = r + 1 < ad.rank ? __ldg(src + (r + 1) * ad.vr) : 0;
-                    w[i] = lo | (hi << 16);
-                  }
-                  q = make_uint4(w[0], w[1], w[2], w[3]);
-                }
-              }
-              st_shared_v4(v_addr + row_chunk<Cfg::kRow>(c, j), q);
-            }
-          }
-          v_adapter = adapter;
-          v_slice = slice;
-        }
-        // (every warp waits for the tile's h, so that none runs ahead on the barriers below)
-        bool ok = mbar_wait(hfull_bar, h_phase, abort_flag, args.status, kDevTimeoutAdapter);
-        if (!__all_sync(0xffffffffu, ok)) break;
-        if (chalf == 0) {
-          const float s = ad.scale * (ad.scales != nullptr ? __ldg(ad.scales + adapter) : 1.f);
-          tc_fence_after();
-          const uint32_t hacc = tmem_base + kHCol + (static_cast<uint32_t>(quarter * 32) << 16);
+        if (ad.want_out && cq >= 2 && (adapter != v_adapter || slice != v_slice)) {
+          // up[a] (this slice's 256 rows): one row a thread of the upper two quarters
+          const int c = (cq - 2) * kTcBlockM + row;
+          const int ch = slice * kTcBlockN + c;
+          const uint16_t* src = static_cast<const uint16_t*>(ad.v) + adapter * ad.va + ch * ad.vc;
 #pragma unroll
           for (int j = 0; j < RP / 8; ++j) {
-            uint32_t r[8];
-            float h[8];
-            __syncwarp();
-            tmem_ld8(hacc + j * 8, r);
+            uint4 q = make_uint4(0u, 0u, 0u, 0u);
+            if (ch < ad.v_rows && j * 8 < ad.rank) {
+              if (ad.v_vec) {
+                q = __ldg(reinterpret_cast<const uint4*>(src) + j);
+              } else {
+                uint32_t w[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  const int r = j * 8 + 2 * i;
+                  const uint32_t lo = r < ad.rank ? __ldg(src + r * ad.vr) : 0;
+                  const uint32_t hi = r + 1 < ad.rank ? __ldg(src + (r + 1) * ad.vr) : 0;
+                  w[i] = lo | (hi << 16);
+                }
+                q = make_uint4(w[0], w[1], w[2], w[3]);
+              }
+            }
+            st_shared_v4(v_addr + row_chunk<Cfg::kRow>(c, j), q);
+          }
+        }
+        v_adapter = adapter;
+        v_slice = slice;
+        const float s = ad.scale * (ad.scales != nullptr ? __ldg(ad.scales + adapter) : 1.f);
+        // (every warp waits for the tile's h, so that none runs ahead on the barriers below)
+        const bool ok = mbar_wait(hfull_bar, h_phase, abort_flag, args.status, kDevTimeoutAdapter);
+        if (!__all_sync(0xffffffffu, ok)) break;
+        tc_fence_after();
+        const uint32_t hacc = tmem_base + kHCol + lane_addr;
+        // 8 columns at a time, by the quarters in turn
+#pragma unroll 1
+        for (int j = cq; j < RP / 8; j += 4) {
+          uint32_t r[8];
+          float h[8];
+          __syncwarp();
+          tmem_ld8(hacc + j * 8, r);
+          tmem_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 8; ++i) h[i] = __uint_as_float(r[i]);
+          for (int q = 1; q < ad.h_accs; ++q) {
+            tmem_ld8(hacc + q * RP + j * 8, r);
             tmem_wait_ld();
 #pragma unroll
-            for (int i = 0; i < 8; ++i) h[i] = __uint_as_float(r[i]);
-            for (int q = 1; q < ad.h_accs; ++q) {
-              tmem_ld8(hacc + q * RP + j * 8, r);
-              tmem_wait_ld();
+            for (int i = 0; i < 8; ++i) h[i] += __uint_as_float(r[i]);
+          }
+          uint32_t w[kParts][4];
 #pragma unroll
-              for (int i = 0; i < 8; ++i) h[i] += __uint_as_float(r[i]);
-            }
-            uint32_t w[kParts][4];
+          for (int i = 0; i < 4; ++i) {
+            uint16_t p0[kParts], p1[kParts];
+            const int c = j * 8 + 2 * i;
+            ad_split<T>(c < ad.rank ? s * h[2 * i] : 0.f, p0);
+            ad_split<T>(c + 1 < ad.rank ? s * h[2 * i + 1] : 0.f, p1);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              uint16_t p0[kParts], p1[kParts];
-              const int c = j * 8 + 2 * i;
-              ad_split<T>(c < ad.rank ? s * h[2 * i] : 0.f, p0);
-              ad_split<T>(c + 1 < ad.rank ? s * h[2 * i + 1] : 0.f, p1);
+            for (int part = 0; part < kParts; ++part)
+              w[part][i] = p0[part] | (static_cast<uint32_t>(p1[part]) << 16);
+          }
 #pragma unroll
-              for (int part = 0; part < kParts; ++part)
-                w[part][i] = p0[part] | (static_cast<uint32_t>(p1[part]) << 16);
-            }
-#pragma unroll
-            for (int part = 0; part < kParts; ++part) {
-              const uint4 q = make_uint4(w[part][0], w[part][1], w[part][2], w[part][3]);
-              if (ad.want_out) st_shared_v4(t_addr + part * Cfg::kPart + row_chunk<Cfg::kRow>(row, j), q);
-              if (hid != nullptr && j * 8 < ad.rank_pad) hid[(part * ad.rank_pad >> 3) + j] = q;
-            }
+          for (int part = 0; part < kParts; ++part) {
+            const uint4 q = make_uint4(w[part][0], w[part][1], w[part][2], w[part][3]);
+            if (ad.want_out) st_shared_v4(t_addr + part * Cfg::kPart + row_chunk<Cfg::kRow>(row, j), q);
+            if (hid != nullptr && j * 8 < ad.rank_pad) hid[(part * ad.rank_pad >> 3) + j] = q;
           }
         }
         fence_proxy_async_smem();
@@ -458,7 +457,7 @@ __global__ void __launch_bounds__(kAdThreads, 1)
         mbar_arrive(tfull_bar);
         h_phase ^= 1u;
         if (!ad.want_out) mbar_arrive(acce_bar);
-      } else if (hid != nullptr) {
+      } else if (hid != nullptr && cq == 0) {
         for (int j = 0; j < ad.rank_pad * kParts / 8; ++j) hid[j] = make_uint4(0u, 0u, 0u, 0u);
       }
       if (!ad.want_out) continue;
@@ -467,80 +466,86 @@ __global__ void __launch_bounds__(kAdThreads, 1)
       if (!__all_sync(0xffffffffu, ok)) break;
       tile_phase ^= 1u;
       tc_fence_after();
-      // The whole accumulator row goes to registers at once, so that the next tile's MMAs start
-      // while this one is converted and stored.
-      uint32_t rr[128];
+      // The warp's accumulators go to registers at once, so that the next tile's MMAs start while
+      // they are converted and stored.
+      uint32_t rr[kAdWarpCols];
       __syncwarp();
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
-        tmem_ld32(tmem_base + chalf * 128 + q * 32 + lane_addr,
+      for (int q = 0; q < kAdWarpCols / 32; ++q)
+        tmem_ld32(tmem_base + cq * kAdWarpCols + q * 32 + lane_addr,
                   *reinterpret_cast<uint32_t(*)[32]>(&rr[q * 32]));
       tmem_wait_ld();
       tc_fence_before();
       mbar_arrive(acce_bar);
 
-      TcTaps tp{};
-      const uint8_t* cb = nullptr;
-      size_t o00 = 0, o01 = 0, o10 = 0, o11 = 0;
-      if (taps_global) {
-        tp = tc_taps(py, px, args.H, args.W, args.Hc, args.Wc, args.scale_y, args.scale_x);
-        constexpr size_t rowb = kTcBlockN * 2;
-        cb = static_cast<const uint8_t*>(args.coarse) + static_cast<size_t>(n) * args.Hc * args.Wc * rowb;
-        o00 = (static_cast<size_t>(tp.ya) * args.Wc + tp.xa) * rowb;
-        o01 = (static_cast<size_t>(tp.ya) * args.Wc + tp.xb) * rowb;
-        o10 = (static_cast<size_t>(tp.yb) * args.Wc + tp.xa) * rowb;
-        o11 = (static_cast<size_t>(tp.yb) * args.Wc + tp.xb) * rowb;
+      // 16 channels of the warp's 32 pixels at a time through 1 KB of shared memory, so that two lanes
+      // write a pixel's 32 bytes: lane l stores half l % 2 of pixels l / 2 and l / 2 + 16.
+      const int scol = slice * kTcBlockN + cq * kAdWarpCols;
+      T* dst[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int r = quarter * 32 + (lane >> 1) + 16 * i;
+        const int sy = y0 + (r >> tw_shift), sx = x0 + (r & tw_mask);
+        dst[i] = sy < args.H && sx < args.W
+                     ? static_cast<T*>(ad.out) + ((static_cast<size_t>(n) * args.H + sy) * args.W + sx) * ad.out_c +
+                           scol + (lane & 1) * 8
+                     : nullptr;
       }
-      const int ox = x0 + (quarter * 32) % tw, oy = y0 + (quarter * 32) / tw;
-      const int scol = slice * kTcBlockN;
-      const uint32_t stage_addr = smem_u32(my_stage);
+      TcTaps tp{};
+      const T* tap[4];
+      if constexpr (kTaps) {
+        tp = tc_taps(py, px, args.H, args.W, args.Hc, args.Wc, args.scale_y, args.scale_x);
+        const T* c = static_cast<const T*>(args.coarse) +
+                     static_cast<size_t>(n) * args.Hc * args.Wc * kTcBlockN + cq * kAdWarpCols;
+        tap[0] = c + (static_cast<size_t>(tp.ya) * args.Wc + tp.xa) * kTcBlockN;
+        tap[1] = c + (static_cast<size_t>(tp.ya) * args.Wc + tp.xb) * kTcBlockN;
+        tap[2] = c + (static_cast<size_t>(tp.yb) * args.Wc + tp.xa) * kTcBlockN;
+        tap[3] = c + (static_cast<size_t>(tp.yb) * args.Wc + tp.xb) * kTcBlockN;
+      }
 #pragma unroll
-      for (int step = 0; step < 128 / kCols; ++step) {
-        const int col0 = chalf * 128 + step * kCols;
-        if (lane == 0) bulk_wait_group_read<0>();
-        __syncwarp();
+      for (int step = 0; step < kAdWarpCols / 16; ++step) {
+        float v[16];
 #pragma unroll
-        for (int j = 0; j < kCols / 8; ++j) {
-          float v[8];
-          const int c = step * kCols + j * 8;  // of the warp's 128
-          const float4 b0 = *reinterpret_cast<const float4*>(bias_s + c);
-          const float4 b1 = *(reinterpret_cast<const float4*>(bias_s + c) + 1);
-          const float bb[8] = {b0.x, b0.y, b0.z, b0.w, b1.x, b1.y, b1.z, b1.w};
+        for (int i = 0; i < 4; ++i) {
+          const float4 b = *reinterpret_cast<const float4*>(bias_s + step * 16 + 4 * i);
+          v[4 * i + 0] = __uint_as_float(rr[step * 16 + 4 * i + 0]) + b.x;
+          v[4 * i + 1] = __uint_as_float(rr[step * 16 + 4 * i + 1]) + b.y;
+          v[4 * i + 2] = __uint_as_float(rr[step * 16 + 4 * i + 2]) + b.z;
+          v[4 * i + 3] = __uint_as_float(rr[step * 16 + 4 * i + 3]) + b.w;
+        }
+        if constexpr (kTaps) {
+          const float w[4] = {tp.w00, tp.w01, tp.w10, tp.w11};
 #pragma unroll
-          for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(rr[c + i]) + bb[i];
-          if (taps_global) {
-            const int o = (chalf * 128 + c) * 2;
-            const uint4 q[4] = {__ldg(reinterpret_cast<const uint4*>(cb + o00 + o)),
-                                __ldg(reinterpret_cast<const uint4*>(cb + o01 + o)),
-                                __ldg(reinterpret_cast<const uint4*>(cb + o10 + o)),
-                                __ldg(reinterpret_cast<const uint4*>(cb + o11 + o))};
-            const float w[4] = {tp.w00, tp.w01, tp.w10, tp.w11};
+          for (int k = 0; k < 4; ++k)
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const uint32_t u[4] = {q[k].x, q[k].y, q[k].z, q[k].w};
+            for (int h = 0; h < 2; ++h) {
+              const uint4 q = __ldg(reinterpret_cast<const uint4*>(tap[k] + step * 16) + h);
+              const uint32_t u[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
                 const float2 f = Pack<T>::unpack(u[e]);
-                v[2 * e] = fmaf(w[k], f.x, v[2 * e]);
-                v[2 * e + 1] = fmaf(w[k], f.y, v[2 * e + 1]);
+                v[8 * h + 2 * e] = fmaf(w[k], f.x, v[8 * h + 2 * e]);
+                v[8 * h + 2 * e + 1] = fmaf(w[k], f.y, v[8 * h + 2 * e + 1]);
               }
             }
-          }
-          st_shared_v4(stage_addr + row_chunk<kCols * 2>(lane, j),
-                       make_uint4(Pack<T>::pack(v[0], v[1]), Pack<T>::pack(v[2], v[3]),
-                                  Pack<T>::pack(v[4], v[5]), Pack<T>::pack(v[6], v[7])));
         }
-        fence_proxy_async_smem();
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          st_shared_v4(stage_addr + row_chunk<32>(lane, h),
+                       make_uint4(Pack<T>::pack(v[8 * h + 0], v[8 * h + 1]), Pack<T>::pack(v[8 * h + 2], v[8 * h + 3]),
+                                  Pack<T>::pack(v[8 * h + 4], v[8 * h + 5]), Pack<T>::pack(v[8 * h + 6], v[8 * h + 7])));
         __syncwarp();
-        if (lane == 0) {
-          if (args.out_cols == 0 || scol + col0 < args.out_cols)
-            tma_store_4d(&map_out, my_stage, scol + col0, ox, oy, n);
-          bulk_commit_group();
+        uint4 o[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) o[i] = ld_shared_v4(stage_addr + row_chunk<32>((lane >> 1) + 16 * i, lane & 1));
+        __syncwarp();
+        if (scol + step * 16 + (lane & 1) * 8 < ad.out_c) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            if (dst[i] != nullptr) *reinterpret_cast<uint4*>(dst[i] + step * 16) = o[i];
         }
       }
     }
-    if (lane == 0) bulk_wait_group<0>();
-    __syncwarp();
   }
 
   tc_fence_before();
@@ -792,11 +797,10 @@ __global__ void __launch_bounds__(256) adapter_transpose_kernel(const uint16_t* 
 }
 
 // ------------------------------------------------------------------ host side
-template <typename T, int RP>
-cudaError_t launch_adapter_rp(const TcPlan& p, const CUtensorMap& map_u, const AdArgs& ad, void* out,
-                              cudaStream_t s) {
+template <typename T, int RP, bool kTaps>
+cudaError_t launch_adapter_rp(const TcPlan& p, const CUtensorMap& map_u, const AdArgs& ad, cudaStream_t s) {
   using Cfg = AdCfg<RP, kAdParts<T>>;
-  auto kern = fpn_adapter_kernel<T, RP>;
+  auto kern = fpn_adapter_kernel<T, RP, kTaps>;
   static std::atomic<bool> configured[64];
   cudaError_t e = once_per_device(configured, [&] {
     return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmemBytes);
@@ -804,22 +808,21 @@ cudaError_t launch_adapter_rp(const TcPlan& p, const CUtensorMap& map_u, const A
   if (e != cudaSuccess) return e;
   TcGemmArgs a;
   std::memcpy(&a, p.args, sizeof(a));
-  CUtensorMap map_out = p.map_out;
-  if (Cfg::kStaging != 4096 && ad.want_out) {  // stores of 32 channels
-    const int sw = a.tile_w < 32 ? a.tile_w : 32;
-    const int C = a.out_cols ? a.out_cols : kTcBlockN;
-    e = encode_nhwc_cols_map(&map_out, p.dtype, out, a.N_img, a.H, a.W, C, sw, 32 / sw, 32);
-    if (e != cudaSuccess) return e;
-  }
   return launch_ex(kern, dim3(p.grid), dim3(kAdThreads), Cfg::kSmemBytes, s, LaunchOpts(), 1, p.map_a,
-                   p.map_b, map_out, p.map_coarse, map_u, a, ad);
+                   p.map_b, p.map_coarse, map_u, a, ad);
+}
+template <typename T, bool kTaps>
+cudaError_t launch_adapter_rank(const TcPlan& p, const CUtensorMap& map_u, const AdArgs& ad, cudaStream_t s) {
+  return ad.rank <= 16   ? launch_adapter_rp<T, 16, kTaps>(p, map_u, ad, s)
+         : ad.rank <= 32 ? launch_adapter_rp<T, 32, kTaps>(p, map_u, ad, s)
+                         : launch_adapter_rp<T, 64, kTaps>(p, map_u, ad, s);
 }
 template <typename T>
-cudaError_t launch_adapter_t(const TcPlan& p, const CUtensorMap& map_u, const AdArgs& ad, void* out,
-                             cudaStream_t s) {
-  if (ad.rank <= 16) return launch_adapter_rp<T, 16>(p, map_u, ad, out, s);
-  if (ad.rank <= 32) return launch_adapter_rp<T, 32>(p, map_u, ad, out, s);
-  return launch_adapter_rp<T, 64>(p, map_u, ad, out, s);
+cudaError_t launch_adapter_t(const TcPlan& p, const CUtensorMap& map_u, const AdArgs& ad, cudaStream_t s) {
+  TcGemmArgs a;
+  std::memcpy(&a, p.args, sizeof(a));
+  return a.coarse != nullptr && a.cbox_w <= 0 ? launch_adapter_rank<T, true>(p, map_u, ad, s)
+                                              : launch_adapter_rank<T, false>(p, map_u, ad, s);
 }
 
 int pad8(int v) { return (v + 7) / 8 * 8; }
@@ -982,8 +985,10 @@ cudaError_t launch_lateral_adapters(const AdapterProblem& p, const void* x, cons
   ad.rank_pad = pad8(p.rank);
   ad.want_out = 1;
   ad.h_accs = ad_h_accs((p.Cin + 63) / 64);
-  return p.dtype == DType::BF16 ? launch_adapter_t<__nv_bfloat16>(plan, map_u, ad, out, s)
-                                : launch_adapter_t<__half>(plan, map_u, ad, out, s);
+  ad.out = out;
+  ad.out_c = 256;
+  return p.dtype == DType::BF16 ? launch_adapter_t<__nv_bfloat16>(plan, map_u, ad, s)
+                                : launch_adapter_t<__half>(plan, map_u, ad, s);
 }
 
 size_t lateral_adapters_workspace_bytes(const AdapterProblem& p, bool has_w_t, bool need_dx) {
@@ -1036,8 +1041,10 @@ cudaError_t launch_lateral_adapters_backward(const AdapterProblem& p, const void
   ad.rank_pad = pad8(p.rank);
   ad.want_out = dx != nullptr;
   ad.h_accs = ad_h_accs(4);
-  e = p.dtype == DType::BF16 ? launch_adapter_t<__nv_bfloat16>(plan, map_u, ad, dx, s)
-                             : launch_adapter_t<__half>(plan, map_u, ad, dx, s);
+  ad.out = dx;
+  ad.out_c = p.Cin;
+  e = p.dtype == DType::BF16 ? launch_adapter_t<__nv_bfloat16>(plan, map_u, ad, s)
+                             : launch_adapter_t<__half>(plan, map_u, ad, s);
   if (e != cudaSuccess) return e;
   float* part = reinterpret_cast<float*>(base + wl.part);
   return p.dtype == DType::BF16

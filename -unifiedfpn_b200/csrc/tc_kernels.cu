@@ -520,13 +520,6 @@ cudaError_t encode_nhwc_map(CUtensorMap* map, DType dt, const void* base, int N,
   return encode(map, dt, 4, base, dims, strides, box);
 }
 
-cudaError_t encode_nhwc_cols_map(CUtensorMap* map, DType dt, const void* base, int N, int H, int W,
-                                 int C, int bw, int bh, int cols) {
-  const int bytes = cols * dtype_size(dt);
-  if (N <= 0 || H <= 0 || W <= 0 || C <= 0 || (bytes != 64 && bytes != 128)) return cudaErrorInvalidValue;
-  return encode_nhwc(map, dt, base, N, H, W, C, bw, bh, bytes);
-}
-
 cudaError_t encode_rows_map(CUtensorMap* map, DType dt, const void* base, int cols, long long rows,
                             int box_cols, int box_rows) {
   if (cols <= 0 || rows <= 0 || box_cols * dtype_size(dt) != 128) return cudaErrorInvalidValue;

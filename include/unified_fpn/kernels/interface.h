@@ -276,9 +276,6 @@ bool tc_use_wide_epilogue(TcPlan& plan);
 // elements (>= C), box (one 128-byte row of channels, bw, bh, 1).
 cudaError_t encode_nhwc_map(CUtensorMap* map, DType dt, const void* base, int N, int H, int W,
                             int C, int pix_stride, int bw, int bh);
-// The same with boxes of `cols` channels of 64 or 128 bytes, under the swizzle of that width.
-cudaError_t encode_nhwc_cols_map(CUtensorMap* map, DType dt, const void* base, int N, int H, int W,
-                                 int C, int bw, int bh, int cols);
 // 16-bit lateral plans only: store the output into channels [0, C) of a map whose pixels are
 // pix_stride elements apart (out = that channel slice's first element).  Used to write the
 // 256-channel slices of a wider tensor (the input gradient of a Cin > 256 lateral).
