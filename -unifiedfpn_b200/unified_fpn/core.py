@@ -27,7 +27,8 @@ import torch
 
 from . import _lib
 from ._lib import check, lib
-from .ops import _DT, E4M3, _stream
+from .groupnorm import fpn_group_norm
+from .ops import _ACTIVATIONS, _DT, E4M3, _stream, fpn_p6
 
 _ACT = {"none": 0, "relu": 1, "leaky_relu": 2, "swish": 3}
 
@@ -56,6 +57,7 @@ class UnifiedFPN:
         self._weight_refs = []      # keeps host/device weight tensors alive until copied
         self._config = None
         self._scale_buf = None      # e4m3 input scales, a stable device address per engine
+        self._norm = None           # group norm of the outputs: (weights, biases, groups, eps, act, alpha)
 
     def __del__(self):
         h = getattr(self, "_h", None)
@@ -120,6 +122,40 @@ class UnifiedFPN:
                 torch.cuda.current_stream(self.device).synchronize()
             check(lib.ufpn_core_set_weights(self._h, l, *[t.data_ptr() for t in ts]), "set_weights")
         self._weights_ready = True
+
+    def set_group_norm(self, weights: Sequence[torch.Tensor] | None, biases: Sequence[torch.Tensor] | None = None,
+                       groups: int = 32, eps: float = 1e-5, activation: str | None = None,
+                       alpha: float = 0.01) -> None:
+        """A group norm with an activation behind every level's 3x3 (:func:`fpn_group_norm` over P2..P5
+        in one call, in place); P6 then comes from the normed P5.  ``weights`` / ``biases``: four [256]
+        vectors, for P2..P5 (``biases`` None = 0); ``weights=None`` takes the norm away again.  An
+        activation set by :meth:`set_activation` acts before the norm."""
+        if weights is None:
+            self._norm = None
+            return
+        if activation not in _ACTIVATIONS:
+            raise ValueError(f"unknown activation {activation!r}")
+        if groups < 1 or 256 % groups:
+            raise ValueError("groups must divide 256")
+        if not eps >= 0:
+            raise ValueError("eps must not be negative")
+        params = []
+        for name, seq in (("weights", weights), ("biases", biases)):
+            if seq is not None and (len(seq) != 4 or any(t.numel() != 256 for t in seq)):
+                raise ValueError(f"{name} must be four vectors of 256 (P2-P5)")
+            params.append(None if seq is None else
+                          [t.detach().reshape(-1).to(self.device, torch.float32).clone() for t in seq])
+        self._norm = (*params, groups, eps, activation, alpha)
+
+    def _apply_norm(self, outs, p6):
+        w, b, groups, eps, act, alpha = self._norm
+        if all(t.is_contiguous(memory_format=torch.channels_last) for t in outs):
+            fpn_group_norm(outs, w, b, groups, eps, act, alpha, out=outs)
+        else:
+            for t, normed in zip(outs, fpn_group_norm(outs, w, b, groups, eps, act, alpha)):
+                t.copy_(normed)
+        if p6 is not None:
+            p6.copy_(fpn_p6(outs[3]))
 
     def _default_weights(self, chans):
         g = torch.Generator().manual_seed(0)
@@ -234,16 +270,16 @@ class UnifiedFPN:
             outs, p6 = self._alloc_outputs(feats, mf, return_p6)
         ins = _ptr_array([t.data_ptr() for t in feats])
         os_ = _ptr_array([t.data_ptr() for t in outs])
+        raw_p6 = p6.data_ptr() if p6 is not None and self._norm is None else None
         if feats[0].dtype == E4M3:
             sp = self._scale_ptrs(input_scales)
-            check(lib.ufpn_core_forward_e4m3(self._h, ins, sp, os_,
-                                             p6.data_ptr() if p6 is not None else None,
-                                             _stream(feats[0])), "forward")
+            check(lib.ufpn_core_forward_e4m3(self._h, ins, sp, os_, raw_p6, _stream(feats[0])), "forward")
         else:
             if input_scales is not None:
                 raise ValueError("input_scales apply to float8_e4m3fn inputs only")
-            check(lib.ufpn_core_forward(self._h, ins, os_, p6.data_ptr() if p6 is not None else None,
-                                        _stream(feats[0])), "forward")
+            check(lib.ufpn_core_forward(self._h, ins, os_, raw_p6, _stream(feats[0])), "forward")
+        if self._norm is not None:
+            self._apply_norm(outs, p6)
         return outs + [p6] if return_p6 else outs
 
     __call__ = forward

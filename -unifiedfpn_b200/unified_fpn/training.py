@@ -14,7 +14,9 @@ backward needs; ``fpn_neck_backward`` returns the gradients of every input, weig
 Each half is one call into the library's native driver (``ufpn_neck_train_forward`` /
 ``ufpn_neck_train_backward``), which issues its kernels on the caller's stream; Python only
 allocates the results.  ``FPNNeck`` wraps both in a ``torch.nn.Module`` with fp32 master weights
-(the kernels compute in the features' 16-bit dtype) for use under autograd.
+(the kernels compute in the features' 16-bit dtype) for use under autograd; it can also carry a
+group norm with an activation behind every 3x3 (``norm_groups``) and low-rank adapters on its
+laterals, one per image of a batch (``adapters``).
 """
 from __future__ import annotations
 
@@ -25,7 +27,10 @@ import torch
 
 from . import _lib
 from ._lib import check, lib
-from .ops import _DT
+from .adapters import fpn_lateral_adapters, fpn_lateral_adapters_backward
+from .groupnorm import fpn_group_norm, fpn_group_norm_backward
+from .ops import (_ACTIVATIONS, _DT, fpn_conv3x3, fpn_conv3x3_backward, fpn_lateral_conv_backward, fpn_p6,
+                  fpn_p6_backward, fpn_upsample_add_backward)
 
 _CL = torch.channels_last
 
@@ -196,17 +201,120 @@ class _NeckFunction(torch.autograd.Function):
                 *gl, *gbl, *gw3, *gb3)
 
 
+class _NormFunction(torch.autograd.Function):
+    """Group norm and activation of P2..P5, and P6 from the normed P5."""
+
+    @staticmethod
+    def forward(ctx, groups, eps, activation, alpha, return_p6, *args):
+        maps, w, b = list(args[:4]), list(args[4:8]), list(args[8:12])
+        outs, mean, rstd = fpn_group_norm(maps, w, b, groups, eps, activation, alpha, return_stats=True)
+        ctx.save_for_backward(*maps, *mean, *rstd, *w, *b)
+        ctx.act = (activation, alpha)
+        return (*outs, fpn_p6(outs[3])) if return_p6 else tuple(outs)
+
+    @staticmethod
+    def backward(ctx, *grads):
+        t = ctx.saved_tensors
+        maps, mean, rstd, w, b = (list(t[i:i + 4]) for i in range(0, 20, 4))
+        dt = maps[0].dtype
+        g = [torch.zeros_like(m, memory_format=_CL) if d is None else _layout(d, dt, m.device)
+             for d, m in zip(grads, maps)]
+        if len(grads) > 4 and grads[4] is not None:
+            if g[3] is grads[3]:  # (the caller's tensor stays as it is)
+                g[3] = g[3].clone(memory_format=_CL)
+            fpn_p6_backward(grads[4], g[3])
+        gx, gw, gb = fpn_group_norm_backward(maps, g, mean, rstd, w, b, *ctx.act,
+                                             need_input_grad=any(ctx.needs_input_grad[5:9]))
+        return (None,) * 5 + (*(gx or [None] * 4), *[v.to(p.dtype).view_as(p) for v, p in zip(gw, w)],
+                              *[v.to(p.dtype).view_as(p) for v, p in zip(gb, b)])
+
+
+class _AdapterNeckFunction(torch.autograd.Function):
+    """The neck with an adapter per image on every lateral: M_l = lateral_l(C_l) + adapter + up(M_{l+1}),
+    P_l = conv3x3_l(M_l), P6 = P5[::2, ::2]."""
+
+    @staticmethod
+    def forward(ctx, return_p6, scale, index, c2, c3, c4, c5, *params):
+        feats = [c2, c3, c4, c5]
+        lw, lb, ow, ob, down, up = (list(params[i:i + 4]) for i in range(0, 24, 4))
+        dt = c2.dtype
+        x = [f.contiguous(memory_format=_CL) for f in feats]
+        merged, hidden = [None] * 4, [None] * 4
+        for l in (3, 2, 1, 0):
+            merged[l], hidden[l] = fpn_lateral_adapters(
+                x[l], lw[l], lb[l], down[l], up[l], index, scale, coarse=merged[l + 1] if l < 3 else None,
+                return_hidden=True)
+        outs = [fpn_conv3x3(m, w, b) for m, w, b in zip(merged, ow, ob)]
+        ctx.save_for_backward(index, *x, *merged, *hidden, *lw, *ow, *down, *up)
+        ctx.scale = scale
+        ctx.params = [(p.dtype, p.shape) for p in params]
+        ctx.dtype = dt
+        return (*outs, fpn_p6(outs[3])) if return_p6 else tuple(outs)
+
+    @staticmethod
+    def backward(ctx, *grads):
+        t = ctx.saved_tensors
+        index = t[0]
+        x, merged, hidden, lw, ow, down, up = (list(t[i:i + 4]) for i in range(1, 29, 4))
+        need = ctx.needs_input_grad
+        need_x, need_lat, need_out = need[3:7], need[7:15], need[15:23]
+        g = [torch.zeros_like(m, memory_format=_CL) if d is None else _layout(d, ctx.dtype, m.device)
+             for d, m in zip(grads, merged)]
+        if len(grads) > 4 and grads[4] is not None:
+            if g[3] is grads[3]:
+                g[3] = g[3].clone(memory_format=_CL)
+            fpn_p6_backward(grads[4], g[3])
+        gx, glw, glb, gow, gob, gd, gu = ([None] * 4 for _ in range(7))
+        dm = None
+        for l in range(4):  # finest first: the top-down adjoint
+            w = any(need_out[l::4])
+            dl, gow[l], gob[l] = fpn_conv3x3_backward(merged[l], ow[l], g[l]) if w else (
+                _conv3x3_input_grad(ow[l], g[l]), None, None)
+            if dm is not None:
+                dl = fpn_upsample_add_backward(dm, tuple(dl.shape[2:]), base=dl)
+            dm = dl
+            gx[l], gd[l], gu[l] = fpn_lateral_adapters_backward(
+                x[l], lw[l], dm, down[l], up[l], index, hidden[l], ctx.scale, need_input_grad=need_x[l])
+            if any(need_lat[l::4]):
+                _, glw[l], glb[l] = fpn_lateral_conv_backward(x[l], lw[l], dm, need_input_grad=False)
+        out = [*glw, *glb, *gow, *gob, *gd, *gu]
+        out = [None if v is None else v.to(d).view(s) for v, (d, s) in zip(out, ctx.params)]
+        return (None, None, None, *gx, *out)
+
+
+def _conv3x3_input_grad(weight: torch.Tensor, grad_output: torch.Tensor) -> torch.Tensor:
+    """The input gradient of the pad-1 3x3 alone: the conv of the gradient with the weights transposed
+    in channels and flipped in space."""
+    zeros = torch.zeros(256, device=grad_output.device)
+    return fpn_conv3x3(grad_output, weight.flip(2, 3).transpose(0, 1), zeros)
+
+
 class FPNNeck(torch.nn.Module):
     """Trainable FPN neck: lateral 1x1 + top-down bilinear add + pad-1 3x3 per level, P6 =
     P5[::2, ::2], with fp32 master weights; the forward and backward run on this library's
     kernels in the features' dtype (bf16 / fp16, channels_last), and autograd sees the usual
-    parameters."""
+    parameters.
+
+    ``norm_groups``: a group norm over that many groups with its ``activation`` (None, "relu",
+    "leaky_relu" with slope ``alpha``, "swish") behind every 3x3, with weights ``norm_w`` / ``norm_b`` per
+    level; P6 comes from the normed P5.  ``adapters``: that many low-rank adapters of ``adapter_rank`` on
+    every lateral (``adapter_down`` [L, R, Cin], ``adapter_up`` [L, 256, R], zero at first), scaled by
+    ``adapter_scale``; ``forward`` then takes an adapter index per image.  To train adapters and norms
+    alone, switch the other parameters' requires_grad off: their gradients are then not computed."""
 
     def __init__(self, in_channels: Sequence[int] = (256, 512, 1024, 2048), out_channels: int = 256,
-                 return_p6: bool = True, seed: int = 0):
+                 return_p6: bool = True, seed: int = 0, norm_groups: int | None = None,
+                 activation: str | None = None, alpha: float = 0.01, eps: float = 1e-5, adapters: int = 0,
+                 adapter_rank: int = 16, adapter_scale: float = 1.0):
         super().__init__()
         if out_channels != 256:
             raise ValueError("the neck's kernels produce 256 channels")
+        if norm_groups is not None and (norm_groups < 1 or 256 % norm_groups):
+            raise ValueError("norm_groups must divide 256")
+        if activation not in _ACTIVATIONS or (norm_groups is None and _ACTIVATIONS[activation]):
+            raise ValueError("activation: a known one, and only behind a norm (norm_groups)")
+        if adapters < 0 or not 1 <= adapter_rank <= 64:
+            raise ValueError("adapters must not be negative, and their rank is 1 to 64")
         g = torch.Generator().manual_seed(seed)
         self.return_p6 = return_p6
         self.lateral_w = torch.nn.ParameterList(
@@ -216,15 +324,39 @@ class FPNNeck(torch.nn.Module):
             [torch.nn.Parameter(torch.randn(256, 256, 3, 3, generator=g) * (2.0 / 2304) ** 0.5)
              for _ in in_channels])
         self.output_b = torch.nn.ParameterList([torch.nn.Parameter(torch.zeros(256)) for _ in in_channels])
+        self.norm_groups, self.activation, self.alpha, self.eps = norm_groups, activation, alpha, eps
+        if norm_groups is not None:
+            self.norm_w = torch.nn.ParameterList([torch.nn.Parameter(torch.ones(256)) for _ in in_channels])
+            self.norm_b = torch.nn.ParameterList([torch.nn.Parameter(torch.zeros(256)) for _ in in_channels])
+        self.adapters, self.adapter_scale = adapters, adapter_scale
+        if adapters:
+            self.adapter_down = torch.nn.ParameterList(
+                [torch.nn.Parameter(torch.randn(adapters, adapter_rank, c, generator=g) * c ** -0.5)
+                 for c in in_channels])
+            self.adapter_up = torch.nn.ParameterList(
+                [torch.nn.Parameter(torch.zeros(adapters, 256, adapter_rank)) for _ in in_channels])
 
-    def forward(self, feats: Sequence[torch.Tensor]):
+    def forward(self, feats: Sequence[torch.Tensor], adapter_index: torch.Tensor | None = None):
+        """P2..P5 (and P6).  ``adapter_index``: one integer per image on the features' device, -1 for
+        none; without it no image has an adapter."""
         # (the lists' registered parameters in index order, without ParameterList's per-item
         # lookups)
         params = [*self.lateral_w._parameters.values(), *self.lateral_b._parameters.values(),
                   *self.output_w._parameters.values(), *self.output_b._parameters.values()]
-        return list(_NeckFunction.apply(self.return_p6, *feats, *params))
+        p6 = self.return_p6 and self.norm_groups is None
+        if adapter_index is None:
+            outs = _NeckFunction.apply(p6, *feats, *params)
+        else:
+            if not self.adapters:
+                raise ValueError("this neck has no adapters")
+            outs = _AdapterNeckFunction.apply(p6, self.adapter_scale, adapter_index, *feats, *params,
+                                              *self.adapter_down, *self.adapter_up)
+        if self.norm_groups is not None:
+            outs = _NormFunction.apply(self.norm_groups, self.eps, self.activation, self.alpha, self.return_p6,
+                                       *outs, *self.norm_w, *self.norm_b)
+        return list(outs)
 
-    def make_graphed(self, sample_feats: Sequence[torch.Tensor]):
+    def make_graphed(self, sample_feats: Sequence[torch.Tensor], adapter_index: torch.Tensor | None = None):
         """Captures this neck's forward and backward as CUDA graphs for the geometry, dtype and
         requires_grad pattern of ``sample_feats`` (C2..C5, channels_last CUDA tensors); returns
         a callable ``f(feats) -> [P2, .., P6]`` that replays them under autograd (weights are
@@ -233,8 +365,15 @@ class FPNNeck(torch.nn.Module):
         800x1216 batch-2 training step, with bitwise the same gradients.  The inputs of later
         calls must match the samples' shapes, dtypes and strides, and no output of an eager
         call may still hold its autograd graph while this captures (its gradient-accumulation
-        nodes would tie the capture to the default stream)."""
+        nodes would tie the capture to the default stream).  With ``adapter_index`` the callable is
+        ``f(feats, adapter_index)``, and later calls may pass other indices."""
         module = _Positional(self)
+        if adapter_index is not None:
+            graphed = torch.cuda.make_graphed_callables(module, (*sample_feats, adapter_index))
+
+            def run_adapters(feats: Sequence[torch.Tensor], adapter_index: torch.Tensor):
+                return list(graphed(*feats, adapter_index))
+            return run_adapters
         graphed = torch.cuda.make_graphed_callables(module, tuple(sample_feats))
 
         def run(feats: Sequence[torch.Tensor]):
@@ -243,11 +382,12 @@ class FPNNeck(torch.nn.Module):
 
 
 class _Positional(torch.nn.Module):
-    """FPNNeck with C2..C5 as four positional tensors (the form CUDA-graph capture takes)."""
+    """FPNNeck with C2..C5 (and the adapter index) as positional tensors (the form CUDA-graph capture
+    takes)."""
 
     def __init__(self, neck: FPNNeck):
         super().__init__()
         self.neck = neck
 
-    def forward(self, c2, c3, c4, c5):
-        return tuple(self.neck([c2, c3, c4, c5]))
+    def forward(self, c2, c3, c4, c5, adapter_index=None):
+        return tuple(self.neck([c2, c3, c4, c5], adapter_index))
