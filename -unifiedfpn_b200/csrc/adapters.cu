@@ -833,7 +833,8 @@ size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 bool adapter_sizes_ok(const AdapterProblem& p) {
   return (p.dtype == DType::BF16 || p.dtype == DType::F16) && p.N > 0 && p.H > 0 && p.W > 0 &&
          p.Cin > 0 && p.Cin % 8 == 0 && p.Cin <= 2048 && p.rank > 0 && p.rank <= kAdMaxRank &&
-         p.adapters > 0 && p.adapters <= 65535 && static_cast<long long>(p.H) * p.W < (1LL << 31) - 256;
+         p.adapters > 0 && p.adapters <= 65535 &&
+         static_cast<long long>(p.H) * p.W < ((1LL << 31) - 256) / p.N;
 }
 
 // Tiles of a map: with a coarse map the lateral's own 2-D tiles (their taps stay in a small box),

@@ -946,7 +946,7 @@ int adapter_problem(int dtype, int N, int Cin, int H, int W, int rank, int adapt
     return fail(UFPN_ERR_UNSUPPORTED, "Cin must be a multiple of 8, at most 2048");
   if (rank < 1 || rank > 64) return fail(UFPN_ERR_UNSUPPORTED, "adapters have rank 1 to 64");
   if (adapters > 65535) return fail(UFPN_ERR_UNSUPPORTED, "at most 65535 adapters");
-  if (static_cast<long long>(H) * W >= (1LL << 31) - 256)
+  if (static_cast<long long>(H) * W >= ((1LL << 31) - 256) / N)
     return fail(UFPN_ERR_UNSUPPORTED, "map too large");
   p->N = N;
   p->Cin = Cin;

@@ -1200,8 +1200,9 @@ bool gn_sizes_ok(int levels, int N, int C, const long long* pixels, int groups) 
   if (levels < 1 || levels > kGnMaxRuns || N < 1 || C < 8 || C % 8 != 0 || C > kGnMaxChannels ||
       groups < 1 || C % groups != 0)
     return false;
+  // (no map beyond 2^39 values: every product of the schedule stays inside its type)
   for (int l = 0; l < levels; ++l)
-    if (pixels[l] < 1) return false;
+    if (pixels[l] < 1 || pixels[l] > (1LL << 39) / N / C) return false;
   return true;
 }
 
