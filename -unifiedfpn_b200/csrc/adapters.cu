@@ -98,6 +98,7 @@ struct AdArgs {
   int h_accs;    // accumulators that h's k-blocks alternate over
   void* out;     // NHWC, out_c channels
   int out_c;
+  int map_h, map_w;  // fpn_adapter_split_kernel: the map behind the flattened one
 };
 constexpr int kAdMaxHAccs = 4;
 int ad_h_accs(int num_kb) { return std::min(kAdMaxHAccs, (num_kb + 7) / 8); }
@@ -557,6 +558,423 @@ __global__ void __launch_bounds__(kAdThreads, 1)
   }
 }
 
+// ------------------------------------------------------------------ few tiles
+// The same forward where a map has few tiles: a cluster of S CTAs shares a tile, each with 1 / S of the
+// k-blocks: one CTA needs 0.4 us for a k-block, most of it the tensor cores on 128 rows whatever the
+// map fills of them.  h up[a]^T is linear in h, so each CTA adds the share of its own partial h to its partial
+// product on the tensor cores; then all put their fp32 partial products into their own shared memory,
+// and after a cluster barrier CTA r reads rows r, r + S, .. of all S, adds them in order with the bias and
+// the top-down taps (fetched while the k-loop runs), and stores those rows.
+// Shared memory: the ring, up[a], barriers; after the k-loop the ring holds the parts of h, then the partial
+// product, and the partial h.
+struct AsSmem {
+  int stages, stage, up, h, bars, total;
+};
+__host__ __device__ constexpr AsSmem as_smem(int rp) {
+  AsSmem m{};
+  m.stages = rp <= 32 ? 4 : 3;
+  m.stage = kTcAStage + kTcBStage + rp * 128;
+  m.up = m.stages * m.stage;
+  m.h = kTcBlockM * kTcBlockN * 4;
+  m.bars = m.up + kTcBlockN * rp * 2;
+  m.total = m.bars + 256 + 1024;
+  return m;
+}
+constexpr bool as_smem_fits(int rp) {
+  return as_smem(rp).total <= 232448 && as_smem(rp).h + kTcBlockM * rp * 4 <= as_smem(rp).up;
+}
+static_assert(as_smem_fits(16) && as_smem_fits(32) && as_smem_fits(64), "adapter split smem");
+
+__device__ __forceinline__ void cluster_arrive() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() {
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr));
+  return v;
+}
+// (zeros without `on`; no branch, so that a thread's loads stay together)
+__device__ __forceinline__ float4 ld_cluster_f4_if(bool on, uint32_t addr) {
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %5, 0;\n\t"
+      "@p ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];\n\t}"
+      : "+f"(v.x), "+f"(v.y), "+f"(v.z), "+f"(v.w)
+      : "r"(addr), "r"(static_cast<int>(on)));
+  return v;
+}
+__device__ __forceinline__ void st_shared_f4(uint32_t addr, float a, float b, float c, float d) {
+  asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(a), "f"(b), "f"(c), "f"(d) : "memory");
+}
+
+template <typename T, int RP, int S>
+__global__ void __launch_bounds__(kAdThreads, 1)
+    fpn_adapter_split_kernel(const __grid_constant__ CUtensorMap map_a,
+                             const __grid_constant__ CUtensorMap map_b,
+                             const __grid_constant__ CUtensorMap map_u, const TcGemmArgs args,
+                             const AdArgs ad) {
+  constexpr int kParts = kAdParts<T>;
+  constexpr int kOwn = kTcBlockM / S;  // rows that this CTA finishes
+  constexpr int kRows = kOwn / 8;      // ... of a thread
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw_addr = smem_u32(smem_raw);
+  uint8_t* smem = smem_raw + ((1024u - (raw_addr & 1023u)) & 1023u);
+  constexpr AsSmem lay = as_smem(RP);
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + lay.bars);
+  uint64_t* empty_bar = full_bar + 4;
+  uint64_t* accf_bar = full_bar + 8;   // partial product final
+  uint64_t* hfull_bar = full_bar + 9;  // partial h final
+  uint64_t* tfull_bar = full_bar + 10;  // h and up in shared memory
+  uint64_t* done_bar = full_bar + 11;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(full_bar + 12);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const int rank = static_cast<int>(cluster_ctarank());
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < lay.stages; ++s) {
+      mbar_init(&full_bar[s], 1);
+      mbar_init(&empty_bar[s], 1);
+    }
+    mbar_init(accf_bar, 1);
+    mbar_init(hfull_bar, 1);
+    mbar_init(tfull_bar, 32 * kAdEpiWarps);
+    mbar_init(done_bar, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+    prefetch_tmap(&map_a);
+    prefetch_tmap(&map_b);
+    prefetch_tmap(&map_u);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, kTcTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  griddep_wait();
+
+  int n, x0, y0;  // (a map of one row: pixels x0 .. x0 + 127 of image n)
+  tc_tile_origin(args, static_cast<int>(blockIdx.x) / S, n, x0, y0);
+  const int adapter = ad_adapter(ad, n);
+  const bool has = adapter >= 0;
+  const int kb0 = rank * args.num_kb / S, kb1 = (rank + 1) * args.num_kb / S;  // non-empty (host)
+  const uint32_t base = smem_u32(smem);
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ TMA producer
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      int issued = 0;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (!mbar_wait(&empty_bar[stage], phase ^ 1u, abort_flag, args.status, kDevTimeoutAdapter)) break;
+        uint8_t* const sa = smem + stage * lay.stage;
+        mbar_arrive_expect_tx(&full_bar[stage], kTcAStage + kTcBStage + (has ? RP * 128 : 0));
+        tma_load_4d(sa, &map_a, &full_bar[stage], kb * 64, x0, 0, n, kPolicyEvictFirst);
+        tma_load_2d(sa + kTcAStage, &map_b, &full_bar[stage], kb * 64, 0, kPolicyEvictLast);
+        if (has)
+          tma_load_4d(sa + kTcAStage + kTcBStage, &map_u, &full_bar[stage], kb * 64, 0, 0, adapter,
+                      kPolicyEvictLast);
+        ++issued;
+        if (++stage == lay.stages) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+      for (int i = 0; i < lay.stages && i < issued; ++i) {  // (matters only when another role gave up)
+        if (--stage < 0) {
+          stage = lay.stages - 1;
+          phase ^= 1u;
+        }
+        mbar_wait_drain(&full_bar[stage], phase);
+      }
+    }
+    __syncwarp();
+    griddep_launch_dependents();
+    cluster_sync_all();
+    cluster_arrive();
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA issuer
+    if (lane == 0) {
+      constexpr uint32_t kFmt = TcElem<T>::kFmt;
+      constexpr uint32_t idesc = make_idesc(kTcBlockM, kTcBlockN, kFmt, kFmt);
+      constexpr uint32_t idesc_u = make_idesc(kTcBlockM, RP, kFmt, kFmt);
+      int stage = 0, hset = 0;
+      uint32_t phase = 0;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (!mbar_wait(&full_bar[stage], phase, abort_flag, args.status, kDevTimeoutAdapter)) break;
+        tc_fence_after();
+        const uint32_t sa = base + stage * lay.stage;
+        const uint64_t adesc = sdesc_kmajor_sw128(sa);
+        const uint64_t bdesc = sdesc_kmajor_sw128(sa + kTcAStage);
+        const uint64_t udesc = sdesc_kmajor_sw128(sa + kTcAStage + kTcBStage);
+        const uint32_t hacc = tmem_base + kTcBlockN + static_cast<uint32_t>(hset * RP);
+        const bool h_more = kb - kb0 >= ad.h_accs;
+        if (++hset == ad.h_accs) hset = 0;
+#pragma unroll
+        for (int k = 0; k < kMmaPerKb; ++k) {
+          tc_mma_f16(tmem_base, adesc + 2u * k, bdesc + 2u * k, idesc, (kb > kb0 || k > 0) ? 1u : 0u);
+          if (has) tc_mma_f16(hacc, adesc + 2u * k, udesc + 2u * k, idesc_u, (h_more || k > 0) ? 1u : 0u);
+        }
+        tc_commit(&empty_bar[stage]);
+        if (++stage == lay.stages) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+      if (has) {
+        tc_commit(hfull_bar);
+        if (mbar_wait(tfull_bar, 0, abort_flag, args.status, kDevTimeoutAdapter)) {
+          tc_fence_after();
+          const uint64_t vdesc = sdesc_kmajor_rows<RP * 2>(base + lay.up);
+#pragma unroll
+          for (int part = 0; part < kParts; ++part) {
+            const uint64_t tdesc = sdesc_kmajor_rows<RP * 2>(base + part * (kTcBlockM * RP * 2));
+#pragma unroll
+            for (int k = 0; k < RP / 16; ++k)
+              tc_mma_f16(tmem_base, tdesc + 2u * k, vdesc + 2u * k, idesc, 1u);
+          }
+        }
+      }
+      tc_commit(accf_bar);
+      tc_commit(done_bar);
+      mbar_wait_drain(done_bar, 0);
+    }
+    __syncwarp();
+    cluster_sync_all();
+    cluster_arrive();
+  } else {
+    // ------------------------------------------------------------ epilogue
+    const int ew = warp - 2;
+    const int t = ew * 32 + lane;
+    const int c4 = (t & 63) * 4;  // output channels c4 .. c4 + 3
+    const int r0 = (t >> 6) * S + rank;  // own rows r0, r0 + 8 S, ..
+    const int pixels = args.W;    // of an image
+    if (has && t < kTcBlockN) {  // up[a], a row a thread
+      const uint16_t* src = static_cast<const uint16_t*>(ad.v) + adapter * ad.va + t * ad.vc;
+#pragma unroll
+      for (int j = 0; j < RP / 8; ++j) {
+        uint4 q = make_uint4(0u, 0u, 0u, 0u);
+        if (j * 8 < ad.rank) {
+          if (ad.v_vec) {
+            q = __ldg(reinterpret_cast<const uint4*>(src) + j);
+          } else {
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int r = j * 8 + 2 * i;
+              const uint32_t lo = r < ad.rank ? __ldg(src + r) : 0;
+              const uint32_t hi = r + 1 < ad.rank ? __ldg(src + r + 1) : 0;
+              w[i] = lo | (hi << 16);
+            }
+            q = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        }
+        st_shared_v4(base + lay.up + row_chunk<RP * 2>(t, j), q);
+      }
+    }
+    // (rows past the map take its last pixel: their loads need no branch, and they are not stored)
+    float4 v[kRows];
+    {
+      float4 b = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (args.bias != nullptr) b = __ldg(reinterpret_cast<const float4*>(args.bias + c4));
+#pragma unroll
+      for (int i = 0; i < kRows; ++i) v[i] = b;
+    }
+    if (args.coarse != nullptr && x0 + r0 < pixels) {
+      const T* coarse = static_cast<const T*>(args.coarse) +
+                        static_cast<size_t>(n) * args.Hc * args.Wc * kTcBlockN + c4;
+      constexpr int kBatch = kRows < 4 ? kRows : 4;
+#pragma unroll
+      for (int i0 = 0; i0 < kRows; i0 += kBatch) {
+        uint2 q[kBatch][4];
+        float w[kBatch][4];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+          const int p = min(x0 + r0 + 8 * S * (i0 + i), pixels - 1);
+          const int py = p / ad.map_w, px = p - py * ad.map_w;
+          const TcTaps tp = tc_taps(py, px, ad.map_h, ad.map_w, args.Hc, args.Wc, args.scale_y, args.scale_x);
+          const T* top = coarse + static_cast<size_t>(tp.ya) * args.Wc * kTcBlockN;
+          const T* bottom = coarse + static_cast<size_t>(tp.yb) * args.Wc * kTcBlockN;
+          q[i][0] = __ldg(reinterpret_cast<const uint2*>(top + tp.xa * kTcBlockN));
+          q[i][1] = __ldg(reinterpret_cast<const uint2*>(top + tp.xb * kTcBlockN));
+          q[i][2] = __ldg(reinterpret_cast<const uint2*>(bottom + tp.xa * kTcBlockN));
+          q[i][3] = __ldg(reinterpret_cast<const uint2*>(bottom + tp.xb * kTcBlockN));
+          w[i][0] = tp.w00;
+          w[i][1] = tp.w01;
+          w[i][2] = tp.w10;
+          w[i][3] = tp.w11;
+        }
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float2 lo = Pack<T>::unpack(q[i][e].x), hi = Pack<T>::unpack(q[i][e].y);
+            float4& o = v[i0 + i];
+            o.x = fmaf(w[i][e], lo.x, o.x);
+            o.y = fmaf(w[i][e], lo.y, o.y);
+            o.z = fmaf(w[i][e], hi.x, o.z);
+            o.w = fmaf(w[i][e], hi.y, o.w);
+          }
+      }
+    }
+    const float hs = has ? ad.scale * (ad.scales != nullptr ? __ldg(ad.scales + adapter) : 1.f) : 0.f;
+
+    const int quarter = warp & 3, cq = ew >> 2;
+    const int row = quarter * 32 + lane;
+    const uint32_t lane_addr = static_cast<uint32_t>(quarter * 32) << 16;
+    bool ok = true;
+    if (has) {
+      ok = mbar_wait(hfull_bar, 0, abort_flag, args.status, kDevTimeoutAdapter);
+      if (__all_sync(0xffffffffu, ok)) {
+        // The ring is free: the MMAs, and so the loads, are through.
+        tc_fence_after();
+#pragma unroll 1
+        for (int j = cq; j < RP / 8; j += 4) {
+          float h[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) h[i] = 0.f;
+          for (int a = 0; a < ad.h_accs; ++a) {
+            uint32_t rr[8];
+            tmem_ld8(tmem_base + kTcBlockN + lane_addr + a * RP + j * 8, rr);
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 8; ++i) h[i] += __uint_as_float(rr[i]);
+          }
+#pragma unroll
+          for (int i = 0; i < 8; ++i) h[i] = j * 8 + i < ad.rank ? hs * h[i] : 0.f;
+          if (ad.hidden != nullptr) {
+            const uint32_t dst = base + lay.h + (row * RP + j * 8) * 4;
+            st_shared_f4(dst, h[0], h[1], h[2], h[3]);
+            st_shared_f4(dst + 16, h[4], h[5], h[6], h[7]);
+          }
+          uint16_t p[8][kParts];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) ad_split<T>(h[i], p[i]);
+#pragma unroll
+          for (int part = 0; part < kParts; ++part) {
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = p[2 * i][part] | (static_cast<uint32_t>(p[2 * i + 1][part]) << 16);
+            st_shared_v4(base + part * (kTcBlockM * RP * 2) + row_chunk<RP * 2>(row, j),
+                         make_uint4(w[0], w[1], w[2], w[3]));
+          }
+        }
+        fence_proxy_async_smem();
+        tc_fence_before();
+      }
+      mbar_arrive(tfull_bar);
+    }
+    ok = mbar_wait(accf_bar, 0, abort_flag, args.status, kDevTimeoutAdapter);
+    if (__all_sync(0xffffffffu, ok)) {
+      tc_fence_after();
+      if (x0 + quarter * 32 < pixels) {  // (rows past the map stay unwritten, and unread)
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          uint32_t rr[32];
+          tmem_ld32(tmem_base + lane_addr + cq * 64 + q * 32, rr);
+          tmem_wait_ld();
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {  // (16-byte chunk c of row r at c ^ (r % 8): no bank conflicts)
+            const int chunk = cq * 16 + q * 8 + j;
+            st_shared_v4(base + row * (kTcBlockN * 4) + ((chunk ^ (row & 7)) << 4),
+                         make_uint4(rr[4 * j], rr[4 * j + 1], rr[4 * j + 2], rr[4 * j + 3]));
+          }
+        }
+      }
+      tc_fence_before();
+    }
+    __syncwarp();
+    cluster_sync_all();
+
+    uint32_t part[S];
+#pragma unroll
+    for (int s = 0; s < S; ++s) part[s] = mapa_shared(base, s);
+    const bool rows = x0 + r0 < pixels;  // this warp has any
+    if (rows) {
+      float4 q[kRows][S];
+#pragma unroll
+      for (int i = 0; i < kRows; ++i) {
+        const int row = r0 + 8 * S * i;
+        const uint32_t off = row * (kTcBlockN * 4) + (((c4 >> 2) ^ (row & 7)) << 4);
+#pragma unroll
+        for (int s = 0; s < S; ++s) q[i][s] = ld_cluster_f4_if(x0 + row < pixels, part[s] + off);
+      }
+#pragma unroll
+      for (int i = 0; i < kRows; ++i) {
+#pragma unroll
+        for (int s = 1; s < S; ++s) {
+          q[i][0].x += q[i][s].x;
+          q[i][0].y += q[i][s].y;
+          q[i][0].z += q[i][s].z;
+          q[i][0].w += q[i][s].w;
+        }
+        v[i].x += q[i][0].x;
+        v[i].y += q[i][0].y;
+        v[i].z += q[i][0].z;
+        v[i].w += q[i][0].w;
+      }
+    }
+    if (ad.hidden != nullptr) {
+      // h of the own rows, four columns a thread, in its parts (zeros without an adapter)
+      const int q4 = ad.rank_pad >> 2;
+      for (int i = t; i < kOwn * q4; i += 32 * kAdEpiWarps) {
+        const int own = i / q4 * S + rank, c = (i % q4) * 4;
+        const int p = x0 + own;
+        if (p >= pixels) break;  // (rows grow with i)
+        float4 h = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (has) {
+#pragma unroll
+          for (int s = 0; s < S; ++s) {
+            const float4 q = ld_cluster_f4(part[s] + lay.h + (own * RP + c) * 4);
+            h.x += q.x;
+            h.y += q.y;
+            h.z += q.z;
+            h.w += q.w;
+          }
+        }
+        uint16_t a[kParts], b[kParts], e[kParts], f[kParts];
+        ad_split<T>(h.x, a);
+        ad_split<T>(h.y, b);
+        ad_split<T>(h.z, e);
+        ad_split<T>(h.w, f);
+        uint16_t* hid = static_cast<uint16_t*>(ad.hidden) +
+                        (static_cast<size_t>(n) * pixels + p) * ad.rank_pad * kParts + c;
+#pragma unroll
+        for (int k = 0; k < kParts; ++k)
+          *reinterpret_cast<uint2*>(hid + k * ad.rank_pad) =
+              make_uint2(a[k] | (static_cast<uint32_t>(b[k]) << 16), e[k] | (static_cast<uint32_t>(f[k]) << 16));
+      }
+    }
+    __syncwarp();
+    cluster_arrive();  // (the others' partials are read)
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+      const int p = x0 + r0 + 8 * S * i;
+      if (p >= pixels) break;
+      *reinterpret_cast<uint2*>(static_cast<T*>(ad.out) + (static_cast<size_t>(n) * pixels + p) * kTcBlockN + c4) =
+          make_uint2(Pack<T>::pack(v[i].x, v[i].y), Pack<T>::pack(v[i].z, v[i].w));
+    }
+  }
+
+  tc_fence_before();
+  __syncwarp();
+  cluster_wait();  // (no CTA ends while another reads its partials)
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, kTcTmemCols);
+  }
+}
+
 // ------------------------------------------------------------------ adapter gradients
 // part[unit][r][c] = sum over the unit's pixels of h[p][r] q[p][c]: for the channel blocks of x with
 // h = dh (ddown), and for dy with h (dup).  A tcgen05 GEMM over pixels (both operands MN-major
@@ -830,6 +1248,65 @@ int parts_of(DType dt) { return dt == DType::BF16 ? kAdParts<__nv_bfloat16> : kA
 int rank_tile(int rank) { return rank <= 16 ? 16 : rank <= 32 ? 32 : 64; }
 size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 
+// Runs fpn_adapter_split_kernel with S CTAs a tile if they are all resident at once and 4 k-blocks are
+// left for each (fewer cost more in the exchange than they save: 2 of rank 64 a CTA on 50 x 76 pixels,
+// 16.5 us, 4 of them 14.5 us, as long as unsplit); sets `done`.  Measured, split against not, 16 bits:
+// 64 maps of one pixel and K = 2048 14.4 / 22.6 us, 32 of 7 x 7 12.4 / 22.7, two of 50 x 76 with K = 1024
+// and a top-down add 14.5 / 16.7; K = 512 12.5 / 12.4.
+template <typename T, int RP, int S>
+cudaError_t try_adapter_split(const TcPlan& p, const TcGemmArgs& a, const CUtensorMap& map_u, const AdArgs& ad,
+                              cudaStream_t s, bool* done) {
+  if (a.num_kb < 4 * S || a.num_tiles > sm_count() / S) return cudaSuccess;
+  auto kern = fpn_adapter_split_kernel<T, RP, S>;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  // (clusters resident at once, the same at every rank: one CTA an SM)
+  static std::atomic<int> resident[64];
+  int fit = dev < 64 ? resident[dev].load(std::memory_order_acquire) : 0;
+  if (fit == 0) {
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, as_smem(RP).total);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(S);
+    cfg.blockDim = dim3(kAdThreads);
+    cfg.dynamicSmemBytes = as_smem(RP).total;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = S;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    e = cudaOccupancyMaxActiveClusters(&fit, kern, &cfg);
+    if (e != cudaSuccess) return e;
+    if (dev < 64) resident[dev].store(fit, std::memory_order_release);
+  }
+  if (a.num_tiles > fit) return cudaSuccess;
+  *done = true;
+  return launch_ex(kern, dim3(a.num_tiles * S), dim3(kAdThreads), as_smem(RP).total, s, LaunchOpts(), S, p.map_a,
+                   p.map_b, map_u, a, ad);
+}
+// The split into the most CTAs a tile that run at once; `done` stays false where none does.
+template <typename T, int RP>
+cudaError_t launch_adapter_split_rp(const TcPlan& p, const TcGemmArgs& a, const CUtensorMap& map_u, AdArgs ad,
+                                    cudaStream_t s, bool* done) {
+  ad.h_accs = ad_h_accs((a.num_kb + 7) / 8);
+  cudaError_t e = try_adapter_split<T, RP, 8>(p, a, map_u, ad, s, done);
+  ad.h_accs = ad_h_accs((a.num_kb + 3) / 4);
+  if (e == cudaSuccess && !*done) e = try_adapter_split<T, RP, 4>(p, a, map_u, ad, s, done);
+  ad.h_accs = ad_h_accs((a.num_kb + 1) / 2);
+  if (e == cudaSuccess && !*done) e = try_adapter_split<T, RP, 2>(p, a, map_u, ad, s, done);
+  return e;
+}
+template <typename T>
+cudaError_t launch_adapter_split(const TcPlan& p, const TcGemmArgs& a, const CUtensorMap& map_u, const AdArgs& ad,
+                                 cudaStream_t s, bool* done) {
+  return ad.rank <= 16   ? launch_adapter_split_rp<T, 16>(p, a, map_u, ad, s, done)
+         : ad.rank <= 32 ? launch_adapter_split_rp<T, 32>(p, a, map_u, ad, s, done)
+                         : launch_adapter_split_rp<T, 64>(p, a, map_u, ad, s, done);
+}
+
 bool adapter_sizes_ok(const AdapterProblem& p) {
   return (p.dtype == DType::BF16 || p.dtype == DType::F16) && p.N > 0 && p.H > 0 && p.W > 0 &&
          p.Cin > 0 && p.Cin % 8 == 0 && p.Cin <= 2048 && p.rank > 0 && p.rank <= kAdMaxRank &&
@@ -961,13 +1438,9 @@ cudaError_t launch_lateral_adapters(const AdapterProblem& p, const void* x, cons
                                     const void* coarse, int Hc, int Wc, void* out, void* hidden,
                                     int* status, cudaStream_t s) {
   if (!adapter_sizes_ok(p)) return cudaErrorInvalidValue;
-  const AdView v = adapter_view(p, coarse != nullptr);
-  TcPlan plan;
-  cudaError_t e = plan_tc_lateral(plan, p.dtype, x, w, bias, coarse, out, p.N, p.Cin, v.H, v.W, Hc, Wc,
-                                  v.tiling, status, 0);
-  if (e != cudaSuccess) return e;
   CUtensorMap map_u;
-  e = encode_nhwc_map(&map_u, p.dtype, down, p.adapters, 1, p.rank, p.Cin, p.Cin, rank_tile(p.rank), 1);
+  cudaError_t e =
+      encode_nhwc_map(&map_u, p.dtype, down, p.adapters, 1, p.rank, p.Cin, p.Cin, rank_tile(p.rank), 1);
   if (e != cudaSuccess) return e;
   AdArgs ad;
   std::memset(&ad, 0, sizeof(ad));
@@ -988,6 +1461,32 @@ cudaError_t launch_lateral_adapters(const AdapterProblem& p, const void* x, cons
   ad.h_accs = ad_h_accs((p.Cin + 63) / 64);
   ad.out = out;
   ad.out_c = 256;
+  ad.map_h = p.H;
+  ad.map_w = p.W;
+  TcPlan plan;
+  // Few tiles: split over k (at most half the SMs, so that two CTAs a tile fit).
+  if ((p.Cin + 63) / 64 >= 8 &&
+      (static_cast<long long>(p.H) * p.W + kTcBlockM - 1) / kTcBlockM * p.N <= sm_count() / 2) {
+    const AdView v = adapter_view(p, false);
+    e = plan_tc_lateral(plan, p.dtype, x, w, bias, nullptr, out, p.N, p.Cin, v.H, v.W, 0, 0, v.tiling, status, 0);
+    if (e != cudaSuccess) return e;
+    TcGemmArgs a;
+    std::memcpy(&a, plan.args, sizeof(a));
+    if (coarse) {
+      a.coarse = coarse;
+      a.Hc = Hc;
+      a.Wc = Wc;
+      a.scale_y = static_cast<float>(Hc) / static_cast<float>(p.H);
+      a.scale_x = static_cast<float>(Wc) / static_cast<float>(p.W);
+    }
+    bool done = false;
+    e = p.dtype == DType::BF16 ? launch_adapter_split<__nv_bfloat16>(plan, a, map_u, ad, s, &done)
+                               : launch_adapter_split<__half>(plan, a, map_u, ad, s, &done);
+    if (e != cudaSuccess || done) return e;
+  }
+  const AdView v = adapter_view(p, coarse != nullptr);
+  e = plan_tc_lateral(plan, p.dtype, x, w, bias, coarse, out, p.N, p.Cin, v.H, v.W, Hc, Wc, v.tiling, status, 0);
+  if (e != cudaSuccess) return e;
   return p.dtype == DType::BF16 ? launch_adapter_t<__nv_bfloat16>(plan, map_u, ad, s)
                                 : launch_adapter_t<__half>(plan, map_u, ad, s);
 }

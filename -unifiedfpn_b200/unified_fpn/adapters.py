@@ -14,7 +14,7 @@ from __future__ import annotations
 import torch
 
 from ._lib import check, lib
-from .groupnorm import _on_device
+from .groupnorm import _on_device, _stream
 from .ops import _DT
 
 _CL = torch.channels_last
@@ -108,19 +108,16 @@ def fpn_lateral_adapters(input: torch.Tensor, weight: torch.Tensor, bias: torch.
             raise ValueError("coarse must match the output's dtype, device, batch and channels")
         coarse = _cl(coarse)
         hc, wc = coarse.shape[2:]
-    rank = down.shape[1]
+    count, rank = down.shape[:2]
     out = torch.empty((n, 256, h, w), dtype=x.dtype, device=dev, memory_format=_CL)
     hidden = torch.empty((n, h, w, _PARTS[x.dtype], (rank + 7) // 8 * 8), dtype=x.dtype,
                          device=dev) if return_hidden else None
 
-    def call():
-        return lib.ufpn_lateral_adapters(
-            _DT[x.dtype], x.data_ptr(), wt.data_ptr(), b.data_ptr(), down.data_ptr(), up.data_ptr(),
-            index.data_ptr(), None if scales is None else scales.data_ptr(), scale,
-            None if coarse is None else coarse.data_ptr(), out.data_ptr(),
-            None if hidden is None else hidden.data_ptr(), n, cin, h, w, rank, down.shape[0], hc, wc,
-            torch.cuda.current_stream(dev).cuda_stream)
-    check(_on_device(dev, call), "ufpn_lateral_adapters")
+    check(_on_device(
+        dev, lib.ufpn_lateral_adapters, _DT[x.dtype], x.data_ptr(), wt.data_ptr(), b.data_ptr(), down.data_ptr(),
+        up.data_ptr(), index.data_ptr(), None if scales is None else scales.data_ptr(), scale,
+        None if coarse is None else coarse.data_ptr(), out.data_ptr(), None if hidden is None else hidden.data_ptr(),
+        n, cin, h, w, rank, count, hc, wc, _stream(dev)), "ufpn_lateral_adapters")
     return (out, hidden) if return_hidden else out
 
 
@@ -163,15 +160,13 @@ def fpn_lateral_adapters_backward(input: torch.Tensor, weight: torch.Tensor | No
     gup = grads[count * rank * cin:].view(count, 256, rank)
     code = _DT[x.dtype]
 
-    def call():
-        need = lib.ufpn_lateral_adapters_workspace(code, n, cin, h, w, rank, count, wtt is not None,
-                                                   need_input_grad)
-        work = torch.empty(need, device=dev, dtype=torch.uint8)
-        return lib.ufpn_lateral_adapters_backward(
-            code, x.data_ptr(), None if wt is None else wt.data_ptr(), None if wtt is None else wtt.data_ptr(),
-            g.data_ptr(), down.data_ptr(), up.data_ptr(), index.data_ptr(),
-            None if scales is None else scales.data_ptr(), scale, hidden.data_ptr(),
-            None if gx is None else gx.data_ptr(), gdown.data_ptr(), gup.data_ptr(), n, cin, h, w, rank, count,
-            work.data_ptr(), need, torch.cuda.current_stream(dev).cuda_stream)
-    check(_on_device(dev, call), "ufpn_lateral_adapters_backward")
+    need = _on_device(dev, lib.ufpn_lateral_adapters_workspace, code, n, cin, h, w, rank, count, wtt is not None,
+                      need_input_grad)
+    work = torch.empty(need, device=dev, dtype=torch.uint8)
+    check(_on_device(
+        dev, lib.ufpn_lateral_adapters_backward, code, x.data_ptr(), None if wt is None else wt.data_ptr(),
+        None if wtt is None else wtt.data_ptr(), g.data_ptr(), down.data_ptr(), up.data_ptr(), index.data_ptr(),
+        None if scales is None else scales.data_ptr(), scale, hidden.data_ptr(), None if gx is None else gx.data_ptr(),
+        gdown.data_ptr(), gup.data_ptr(), n, cin, h, w, rank, count, work.data_ptr(), need, _stream(dev)),
+        "ufpn_lateral_adapters_backward")
     return gx, gdown, gup

@@ -26,22 +26,28 @@ MAX_LEVELS = 8
 
 
 @functools.lru_cache(maxsize=256)
-def _workspace_bytes(device: int, code: int, n: int, c: int, pixels: tuple, groups: int, backward: int) -> int:
-    # (device in the key: the plan follows its SM count)
-    return lib.ufpn_group_norm_workspace(code, len(pixels), n, c, (ctypes.c_longlong * len(pixels))(*pixels),
-                                         groups, backward)
+def _workspace_bytes(dev: torch.device, code: int, n: int, c: int, pixels: tuple, groups: int, backward: int) -> int:
+    # (the plan follows the device's SM count)
+    return _on_device(dev, lib.ufpn_group_norm_workspace, code, len(pixels), n, c,
+                      (ctypes.c_longlong * len(pixels))(*pixels), groups, backward)
 
 
 def _ptrs(ts):
     return (ctypes.c_void_p * len(ts))(*[None if t is None else t.data_ptr() for t in ts])
 
 
-def _on_device(dev: torch.device, call):
-    """``call()`` with ``dev`` as the current CUDA device."""
-    if dev.index == torch.cuda.current_device():
-        return call()
+def _stream(dev: torch.device) -> int:
+    """Handle of torch's current stream on ``dev`` (the Stream object that
+    ``torch.cuda.current_stream`` makes costs 2 us a call)."""
+    return torch._C._cuda_getCurrentRawStream(dev.index)
+
+
+def _on_device(dev: torch.device, fn, *args) -> int:
+    """``fn(*args)`` with ``dev`` as the current CUDA device."""
+    if dev.index == torch._C._cuda_getDevice():
+        return fn(*args)
     with torch.cuda.device(dev):
-        return call()
+        return fn(*args)
 
 
 def _levels(input, what: str = "input"):
@@ -127,16 +133,14 @@ def fpn_group_norm(input: torch.Tensor | Sequence[torch.Tensor], weight=None, bi
         means, rstds = list(stats[0]), list(stats[1])
     code = _DT[xs[0].dtype]
     pixels = tuple([t.shape[2] * t.shape[3] for t in xs])
-    need = _workspace_bytes(dev.index, code, n, c, pixels, groups, 0)
+    need = _workspace_bytes(dev, code, n, c, pixels, groups, 0)
     work = torch.empty(need, device=dev, dtype=torch.uint8)
 
-    def call():
-        return lib.ufpn_group_norm(
-            code, len(xs), _ptrs(xs), _ptrs(ys), _ptrs(ws), _ptrs(bs), _ptrs(means) if means else None,
-            _ptrs(rstds) if rstds else None, n, c, (ctypes.c_longlong * len(xs))(*pixels), groups, eps,
-            _ACTIVATIONS[activation], alpha, work.data_ptr(), need,
-            torch.cuda.current_stream(dev).cuda_stream)
-    check(_on_device(dev, call), "ufpn_group_norm")
+    check(_on_device(
+        dev, lib.ufpn_group_norm, code, len(xs), _ptrs(xs), _ptrs(ys), None if weight is None else _ptrs(ws),
+        None if bias is None else _ptrs(bs), _ptrs(means) if means else None, _ptrs(rstds) if rstds else None, n, c,
+        (ctypes.c_longlong * len(xs))(*pixels), groups, eps, _ACTIVATIONS[activation], alpha, work.data_ptr(), need,
+        _stream(dev)), "ufpn_group_norm")
     if single:
         return (ys[0], means[0], rstds[0]) if return_stats else ys[0]
     return (ys, means, rstds) if return_stats else ys
@@ -179,16 +183,14 @@ def fpn_group_norm_backward(input, grad_output, mean, rstd, weight=None, bias=No
     pad = [None] * (len(xs) - rows)
     code = _DT[xs[0].dtype]
     pixels = tuple([t.shape[2] * t.shape[3] for t in xs])
-    need = _workspace_bytes(dev.index, code, n, c, pixels, groups, 1)
+    need = _workspace_bytes(dev, code, n, c, pixels, groups, 1)
     work = torch.empty(need, device=dev, dtype=torch.uint8)
 
-    def call():
-        return lib.ufpn_group_norm_backward(
-            code, len(xs), _ptrs(xs), _ptrs(gs), _ptrs(gxs) if gxs else None, _ptrs(ws), _ptrs(bs),
-            _ptrs(means), _ptrs(rstds), _ptrs(gw + pad), _ptrs(gb + pad), n, c,
-            (ctypes.c_longlong * len(xs))(*pixels), groups, _ACTIVATIONS[activation], alpha,
-            work.data_ptr(), need, torch.cuda.current_stream(dev).cuda_stream)
-    check(_on_device(dev, call), "ufpn_group_norm_backward")
+    check(_on_device(
+        dev, lib.ufpn_group_norm_backward, code, len(xs), _ptrs(xs), _ptrs(gs), _ptrs(gxs) if gxs else None, _ptrs(ws),
+        _ptrs(bs), _ptrs(means), _ptrs(rstds), _ptrs(gw + pad), _ptrs(gb + pad), n, c,
+        (ctypes.c_longlong * len(xs))(*pixels), groups, _ACTIVATIONS[activation], alpha, work.data_ptr(), need,
+        _stream(dev)), "ufpn_group_norm_backward")
     if single or shared:
         return (gxs[0] if single and gxs else gxs), gw[0], gb[0]
     # a parameter shared by the maps beside one that is not: its gradient is the sum over the maps

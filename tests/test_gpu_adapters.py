@@ -2,8 +2,8 @@
 
 Tolerances are counted.  With u = 2^-24: an fp32 sum of K products is within K u of the sum of
 their absolute values (any order); h keeps 2^-22 of itself (parts of 8 or 11 bits, the last one
-rounded to half a step; fp16 loses what is below 2^-24, 2^-25 absolute); a 16-bit result is rounded once, finfo.eps / 2 of its value.  The bounds use the absolute sums, element by
-element.
+rounded to half a step; fp16 loses what is below 2^-24, 2^-25 absolute); a 16-bit result is rounded
+once, finfo.eps / 2 of its value.  The bounds use the absolute sums, element by element.
 """
 import pytest
 import torch
@@ -282,3 +282,41 @@ def test_refusals(cuda_device):
         f(x, w, b, d, u, i, coarse=torch.zeros(2, 256, 5, 5, device=cuda_device, dtype=torch.bfloat16))
     torch.cuda.synchronize()
     assert U.device_status() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("shape,size", [
+    ((1, 1032, 17, 23, 64, 3), (9, 12)),   # four tiles, k in quarters: 17 k-blocks, the last one of 8 channels
+    ((2, 2040, 13, 29, 33, 2), (7, 15)),   # six tiles in eighths
+    ((2, 520, 40, 41, 9, 2), (20, 21)),    # 26 tiles in halves, ranks that are no whole vectors
+    ((37, 712, 3, 43, 40, 5), (2, 43)),    # 74 tiles in halves, one of a single pixel an image
+    ((37, 264, 3, 43, 40, 5), (2, 43)),    # too few k-blocks to split
+    ((3, 1024, 1, 1, 1, 2), (1, 1))])
+def test_few_tiles_split_over_k(cuda_device, dtype, shape, size):
+    import unified_fpn as U
+    n, cin, h, w, rank, count = shape
+    s = _make(n, cin, h, w, rank, count, dtype, cuda_device, sum(shape))
+    g = torch.Generator().manual_seed(h)
+    coarse = torch.randn(n, 256, *size, generator=g).to(dtype).to(cuda_device).contiguous(memory_format=CL)
+    out, hidden = U.fpn_lateral_adapters(s["x"], s["w"], s["b"], s["down"], s["up"], s["index"], scale=s["scales"],
+                                         coarse=coarse, return_hidden=True)
+    torch.cuda.synchronize()
+    assert U.device_status() == 0
+    r = _ref(s, coarse=coarse)
+    _check(out, r["out"], r["out_lim"], "out")
+    # the hidden values: their parts' sum
+    hid = hidden.double().sum(3).flatten(1, 2)
+    for i, a in enumerate(s["index"].tolist()):
+        if not 0 <= a < count:
+            assert not hid[i].any()
+            continue
+        x, d, sc = _px(s["x"])[i], s["down"][a].double(), s["scales"][a].double()
+        want = sc * (x @ d.t())
+        lim = sc * (cin + 4) * 2.0 ** -24 * (x.abs() @ d.abs().t()) + 2.0 ** -22 * want.abs() + 2.0 ** -25
+        assert ((hid[i, :, :rank] - want).abs() <= lim).all()
+        assert not hid[i, :, rank:].any()
+    # one image of the batch alone (another split): the same within the bounds; NaN stays in its image
+    x = s["x"].clone(memory_format=torch.preserve_format)
+    x[0] = float("nan")
+    other = U.fpn_lateral_adapters(x, s["w"], s["b"], s["down"], s["up"], s["index"], scale=s["scales"], coarse=coarse)
+    assert other[0].isnan().all() and torch.equal(other[1:], out[1:])
