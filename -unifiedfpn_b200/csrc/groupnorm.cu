@@ -40,6 +40,7 @@ namespace {
 constexpr int kGnWarps = 8;            // statistics warps, and as many apply warps
 constexpr int kGnThreads = 32 * kGnWarps;
 constexpr int kGnMergeThreads = 128;
+constexpr int kGnMergeRows = 1920;     // sums of an image that a merge has in shared memory at once
 constexpr int kGnMaxRuns = 8;         // runs (images of one level) per segment
 constexpr int kGnMaxChannels = 2048;  // 8 per thread of a half
 constexpr int kGnStage = 4096;         // one copy of a warp; backward: half of it x, half dy
@@ -159,18 +160,25 @@ struct GnArgs {
 };
 
 // 1 / (1 + exp(-z)) of a pair.  16-bit maps, whose results are rounded to 2^-9 or 2^-12, take the
-// fast exp and one fast reciprocal for both, 1 / a = b / (a b) (relative error about 2^-20; the
-// special-function unit sets their pace); exp(-z) is held below 2^60 for that, so z < -41 has a
-// sigmoid of 2^-60.  fp32 maps take the accurate exp and division.
+// approximate 2^v and 1 / v instructions (relative error about 2^-20 up to |z| = 40; beyond, exp(-z) = inf
+// gives 0), fp32 maps the accurate exp and division.
+__device__ __forceinline__ float gn_exp2(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float gn_inverse(float v) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
 template <typename T>
 __device__ __forceinline__ float2 gn_sigmoid(float2 z) {
   if constexpr (sizeof(T) == 2) {
-    const float a = 1.f + fminf(__expf(-z.x), 1.152921504606846976e18f);
-    const float b = 1.f + fminf(__expf(-z.y), 1.152921504606846976e18f);
-    // (fminf returns the bound for a NaN, which so stays out of the other channel; z itself
-    // carries it on)
-    const float r = __fdividef(1.f, a * b);
-    return make_float2(b * r, a * r);
+    constexpr float kLog2E = 1.44269504088896340736f;
+    const float2 v = mul2(z, both(-kLog2E));
+    const float2 d = add2(make_float2(gn_exp2(v.x), gn_exp2(v.y)), both(1.f));
+    return make_float2(gn_inverse(d.x), gn_inverse(d.y));
   } else {
     return make_float2(1.f / (1.f + expf(-z.x)), 1.f / (1.f + expf(-z.y)));
   }
@@ -205,6 +213,7 @@ struct GnSmem {
   float cnt[kGnThreads];  // [warp][pixel lane of the warp]
   // merge: per thread, then by group (mean, rstd; backward: the means of w dz and w dz xhat)
   float m1[kGnMergeThreads], m2[kGnMergeThreads], m3[kGnMergeThreads];
+  alignas(16) float2 rows[kGnMergeRows];
   float g1[kGnMaxChannels], g2[kGnMaxChannels];
   uint64_t stats_full[kGnWarps][kGnStatsStages], apply_full[kGnWarps][kGnApplyStages];
   uint64_t ready, taken;  // g1 and g2: written; in the apply warps' registers
@@ -472,7 +481,7 @@ __device__ __forceinline__ void gn_stats_sums(const GnArgs& a, const GnPlace& at
   float2 np[4], s1[4], s2[4];  // minus the thread's first pixel; sums relative to it
 #pragma unroll
   for (int i = 0; i < 4; ++i) np[i] = s1[i] = s2[i] = both(0.f);
-  ring.template pixels<kGnK>(
+  ring.template pixels<kGnK * 2 / sizeof(T)>(
       a, ln, s, static_cast<T*>(nullptr),
       [&](const Gn8<T>& x) {
         x.get(np);
@@ -591,12 +600,60 @@ __device__ __forceinline__ void gn_stats_reduce(const GnArgs& a, const GnPlace& 
   }
 }
 
+// The merge's rows [r0, r0 + n) of groups [g0, g0 + span) into shared memory.  (One asynchronous copy after
+// the other from a short loop: the same loads unrolled into registers took 13000 cycles at a launch's
+// first merge, most of them instruction fetches.)
+__device__ __forceinline__ void gn_merge_fetch(const GnArgs& a, const float2* rows, int g0, int span, int r0, int n,
+                                               GnSmem& s, int t) {
+  const float2* src = rows + static_cast<size_t>(r0) * a.groups + g0;
+  if ((a.groups & 1) == 0) {  // whole 16-byte vectors
+    const uint32_t dst = smem_u32(s.rows);
+    const int half = span >> 1;
+    if (span == a.groups) {
+#pragma unroll 1
+      for (int i = t; i < n * half; i += kGnMergeThreads)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + 16 * i), "l"(src + 2 * i) : "memory");
+    } else {  // (spans of 128)
+#pragma unroll 1
+      for (int i = t; i < n * half; i += kGnMergeThreads) {
+        const int r = i / (kGnMergeThreads / 2), c = 2 * (i % (kGnMergeThreads / 2));
+        if (g0 + c < a.groups)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + 16 * i),
+                       "l"(src + static_cast<size_t>(r) * a.groups + c)
+                       : "memory");
+      }
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+  } else {
+#pragma unroll 4
+    for (int i = t; i < n * span; i += kGnMergeThreads) {
+      const int r = i / span, c = i - r * span;
+      if (g0 + c < a.groups) s.rows[i] = __ldcg(src + static_cast<size_t>(r) * a.groups + c);
+    }
+  }
+  gn_merge_sync();
+}
+// f(row, its sums) for the rows of one thread: group g0 + lane, every per_g-th row from row j on.
+template <typename F>
+__device__ __forceinline__ void gn_merge_rows(const GnArgs& a, const float2* rows, int chunks, int g0, int span,
+                                              int j, int lane, int per_g, GnSmem& s, int t, F&& f) {
+  const int batch = kGnMergeRows / span / per_g * per_g;
+  for (int r0 = 0; r0 < chunks; r0 += batch) {
+    const int n = min(batch, chunks - r0);
+    if (r0 > 0) gn_merge_sync();
+    gn_merge_fetch(a, rows, g0, span, r0, n, s, t);
+    if (j < per_g && g0 + lane < a.groups) {
+#pragma unroll 2
+      for (int i = j; i < n; i += per_g) f(r0 + i, s.rows[i * span + lane]);
+    }
+  }
+}
+
 // The image's statistics from its chunks' rows, by group: g1 = mean, g2 = rstd.  A thread sums its
 // rows relative to its first one.
 __device__ __forceinline__ void gn_merge_stats(const GnArgs& a, const GnPlace& at, GnSmem& s, int t) {
   const size_t row0 = static_cast<size_t>(at.row_of_chunk0()) * a.groups;
   const GnRun& r = a.run[at.run];
-  const float2* rows = a.part + row0;
   const int chunks = r.chunks;
   const int span = min(a.groups, kGnMergeThreads);
   const int per_g = kGnMergeThreads / span;  // threads per group, each over every per_g-th row
@@ -604,32 +661,21 @@ __device__ __forceinline__ void gn_merge_stats(const GnArgs& a, const GnPlace& a
   const float cg = static_cast<float>(a.cg), px = static_cast<float>(r.pixels);
   const float per = static_cast<float>(r.per);
   const float tail = static_cast<float>(r.pixels - static_cast<long long>(chunks - 1) * r.per);
-  constexpr int K = 20;
   for (int g0 = 0; g0 < a.groups; g0 += span) {
     const int g = g0 + lane;
     const bool in = j < per_g && g < a.groups;
     const float pivot = in && j == 0 ? __ldcg(a.pivot + row0 + g) : 0.f;
+    float ref = 0.f, sd = 0.f, sq = 0.f, m2 = 0.f, cnt = 0.f;
+    gn_merge_rows(a, a.part + row0, chunks, g0, span, j, lane, per_g, s, t, [&](int i, float2 v) {
+      if (cnt == 0.f) ref = v.x;
+      const float n = i + 1 < chunks ? per : tail;
+      const float d = v.x - ref;
+      sd = fmaf(n, d, sd);
+      sq = fmaf(n * d, d, sq);
+      m2 += v.y;
+      cnt += n;
+    });
     if (in) {
-      float ref = 0.f, sd = 0.f, sq = 0.f, m2 = 0.f, cnt = 0.f;
-      for (int i0 = j; i0 < chunks; i0 += K * per_g) {
-        float2 v[K];
-#pragma unroll
-        for (int k = 0; k < K; ++k)
-          if (i0 + k * per_g < chunks) v[k] = __ldcg(rows + static_cast<size_t>(i0 + k * per_g) * a.groups + g);
-        if (i0 == j) ref = v[0].x;
-#pragma unroll
-        for (int k = 0; k < K; ++k) {
-          const int i = i0 + k * per_g;
-          if (i < chunks) {
-            const float n = i + 1 < chunks ? per : tail;
-            const float d = v[k].x - ref;
-            sd = fmaf(n, d, sd);
-            sq = fmaf(n * d, d, sq);
-            m2 += v[k].y;
-            cnt += n;
-          }
-        }
-      }
       const float m = cnt > 0.f ? sd / cnt : 0.f;
       s.m1[t] = ref + m;
       s.m2[t] = fmaf(cg, max_nan(fmaf(-m, sd, sq), 0.f), m2);
@@ -720,7 +766,7 @@ template <typename T, int kAct, bool kWhole, typename Ring>
 __device__ __forceinline__ void gn_apply_chunk(const GnArgs& a, const GnPlace& at, const GnLanes& ln, GnSmem& s,
                                                Ring& ring, const GnChannels<kWhole>& ch) {
   const float alpha = a.alpha;
-  ring.template pixels<kGnK / 2>(
+  ring.template pixels<kGnK / sizeof(T)>(
       a, ln, s, static_cast<T*>(a.run[at.run].y) + at.base + ln.v * 8, [](const Gn8<T>&) {},
       [&](const Gn8<T>& x, const Gn8<T>&, T* y) {
         float2 f[4];
@@ -748,7 +794,7 @@ __device__ __forceinline__ void gn_bwd_chunk_sums(const GnArgs& a, const GnPlace
                                                   GnSmem& s, Ring& ring, const GnChannels<kWhole>& ch,
                                                   float2 (&sz)[4], float2 (&sx)[4]) {
   const float alpha = a.alpha;
-  ring.template pixels<kGnK / 2>(
+  ring.template pixels<kGnK / sizeof(T)>(
       a, ln, s, static_cast<T*>(nullptr), [](const Gn8<T>&) {},
       [&](const Gn8<T>& x, const Gn8<T>& d, T*) {
         float2 f[4], h[4];
@@ -828,35 +874,25 @@ __device__ __forceinline__ void gn_bwd_reduce(const GnArgs& a, const GnPlace& at
 __device__ __forceinline__ void gn_bwd_merge(const GnArgs& a, const GnPlace& at, GnSmem& s, int t) {
   const GnRun& r = a.run[at.run];
   const float2* rows = a.part + static_cast<size_t>(at.row_of_chunk0()) * a.groups;
-  const int chunks = r.chunks;
   const int span = min(a.groups, kGnMergeThreads);
   const int per_g = kGnMergeThreads / span;
   const int j = t / span, lane = t - j * span;
   const float inv_m = 1.f / (static_cast<float>(r.pixels) * static_cast<float>(a.cg));
-  constexpr int K = 20;
   for (int g0 = 0; g0 < a.groups; g0 += span) {
     const int g = g0 + lane;
     const bool in = j < per_g && g < a.groups;
+    float z = 0.f, x = 0.f;
+    gn_merge_rows(a, rows, r.chunks, g0, span, j, lane, per_g, s, t, [&](int, float2 v) {
+      z += v.x;
+      x += v.y;
+    });
     if (in) {
-      float z = 0.f, x = 0.f;
-      for (int i0 = j; i0 < chunks; i0 += K * per_g) {
-        float2 v[K];
-#pragma unroll
-        for (int k = 0; k < K; ++k)
-          v[k] = i0 + k * per_g < chunks ? __ldcg(rows + static_cast<size_t>(i0 + k * per_g) * a.groups + g)
-                                         : both(0.f);
-#pragma unroll
-        for (int k = 0; k < K; ++k) {
-          z += v[k].x;
-          x += v[k].y;
-        }
-      }
       s.m1[t] = z;
       s.m2[t] = x;
     }
     gn_merge_sync();
     if (in && j == 0) {
-      float z = 0.f, x = 0.f;
+      z = x = 0.f;
       for (int i = 0; i < per_g; ++i) {
         z += s.m1[i * span + t];
         x += s.m2[i * span + t];
@@ -893,7 +929,7 @@ __device__ __forceinline__ void gn_bwd_apply_chunk(const GnArgs& a, const GnPlac
                                                    GnSmem& s, Ring& ring, const GnChannels<kWhole>& ch,
                                                    const GnGradient<kWhole>& gr) {
   const float alpha = a.alpha;
-  ring.template pixels<kGnK / 4>(
+  ring.template pixels<kGnK / 2 / sizeof(T)>(
       a, ln, s, static_cast<T*>(a.run[at.run].y) + at.base + ln.v * 8, [](const Gn8<T>&) {},
       [&](const Gn8<T>& x, const Gn8<T>& d, T* dx) {
         float2 f[4], h[4];
@@ -940,7 +976,6 @@ __device__ __forceinline__ bool gn_wait_segment(const GnArgs& a, GnSmem& s, int 
       return false;
     }
   }
-  __threadfence();
   return true;
 }
 // Whether the statistics of segment k may be read already: at most four segments ahead of the apply
@@ -1005,10 +1040,8 @@ __global__ void __launch_bounds__(2 * kGnThreads + kGnMergeThreads, 1)
       else
         gn_stats_reduce(a, at, ln, s);
       gn_stats_sync();
-      if (threadIdx.x == 0) {
-        __threadfence();
-        atomicAdd(a.done + cur.k, 1u);
-      }
+      if (threadIdx.x == 0)
+        asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(a.done + cur.k) : "memory");
       cur = nxt;
       at = then;
     }
