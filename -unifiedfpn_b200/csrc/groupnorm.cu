@@ -1,5 +1,6 @@
 // Group norm with an activation on channels-last maps, forward and backward, for one map or
-// the levels of a pyramid in one call.
+// the levels of a pyramid in one call.  (Two forms of the forward: below, for maps of any size, and
+// for small ones a cluster of blocks per map, further down.)
 //
 // Over the m = pixels * Cg values of group g of image n (Cg = C / groups adjacent channels):
 //   mean = sum x / m;  var = sum (x - mean)^2 / m;  rstd = 1 / sqrt(var + eps)
@@ -441,6 +442,10 @@ struct GnRing {
   }
 };
 
+__device__ __forceinline__ float to_float(float v) { return v; }
+__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+
 // Barriers of the statistics threads and of the merging threads.
 __device__ __forceinline__ void gn_stats_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kGnThreads) : "memory"); }
 __device__ __forceinline__ void gn_merge_sync() {
@@ -453,9 +458,9 @@ __device__ __forceinline__ float gn_lane_sum(float v, int width) {
   return v;
 }
 // Threads per group in a block's sums over channels: a power of two up to a warp.
-__device__ __forceinline__ int gn_group_width(const GnArgs& a) {
+__device__ __forceinline__ int gn_group_width(const GnArgs& a, int threads = kGnThreads) {
   int t = 32;
-  while (t > 1 && (t * a.groups > kGnThreads || t > a.cg)) t >>= 1;
+  while (t > 1 && (t * a.groups > threads || t > a.cg)) t >>= 1;
   return t;
 }
 
@@ -1112,6 +1117,230 @@ __global__ void __launch_bounds__(2 * kGnThreads + kGnMergeThreads, 1)
   }
 }
 
+// ------------------------------------------------------------------ small maps
+// The forward of maps that fit a cluster's shared memory: a cluster of blocks per image and level, each
+// block with a share of the pixels.  The share comes in by bulk copies and stays; the block takes its
+// mean and then its squares about that mean (both passes from shared memory), the blocks exchange (pivot,
+// mean, M2) through distributed shared memory, and the norm is applied from there.  x is read once, and
+// there are no device counters to clear and no wait across the grid.
+constexpr int kGsThreads = 512;
+constexpr int kGsPieces = 4;
+constexpr int kGsMaxCluster = 16;
+constexpr int kGsMaxLanes = 32;
+constexpr int kGsMaxGroups = 128;
+struct GnSmallSmem {
+  float red[8 * kGsThreads];  // a pixel lane's sums [lane][C]
+  float ch[kGnMaxChannels];
+  // by group: the block's pivot and its mean minus that; of every block of the cluster (pivot, mean, M2)
+  float pivot[kGsMaxGroups], mean[kGsMaxGroups];
+  float all[3][kGsMaxCluster][kGsMaxGroups + 1];  // (+ 1: 16 blocks' sums of a group in different banks)
+  float g1[kGsMaxGroups], g2[kGsMaxGroups];
+  uint64_t full[kGsPieces];
+  int abort_flag;
+};
+constexpr int kGsDataOffset = (sizeof(GnSmallSmem) + 127) / 128 * 128;
+constexpr long long kGsMaxShare = 96 << 10;
+static_assert(kGsDataOffset + kGsMaxShare <= 232448, "small group norm smem");
+
+__device__ __forceinline__ void st_cluster_f32(const float* p, uint32_t rank, float v) {
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(mapa_shared(smem_u32(p), rank)), "f"(v) : "memory");
+}
+
+// The pixels q = pl, pl + lanes, .. below cnt: f(its 8 channels, pixel).
+template <typename T, typename F>
+__device__ __forceinline__ void gn_small_pixels(uint32_t mine, int row, int pl, int lanes, int begin, int end, F&& f) {
+#pragma unroll 4
+  for (int q = begin + pl; q < end; q += lanes) {
+    Gn8<T> t;
+    t.load_shared(mine + static_cast<uint32_t>(q) * row);
+    f(t, q);
+  }
+}
+template <typename T, int kAct, bool kWhole>
+__device__ __forceinline__ void gn_small_apply(uint32_t mine, int row, int pl, int lanes, int cnt, T* y, int C,
+                                               float alpha, const GnChannels<kWhole>& ch) {
+  gn_small_pixels<T>(mine, row, pl, lanes, 0, cnt, [&](const Gn8<T>& x, int q) {
+    float2 f[4];
+    x.get(f);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = gn_act<T, kAct>(ch.z(ch.centred(f[i], i), i), alpha);
+    gn_put<T>(y + static_cast<size_t>(q) * C, f);
+  });
+}
+
+template <typename T, bool kWhole>
+__global__ void __launch_bounds__(kGsThreads, 1) gn_small_kernel(const __grid_constant__ GnArgs a, const int log_blocks) {
+  extern __shared__ __align__(128) uint8_t gs_smem[];
+  GnSmallSmem& s = *reinterpret_cast<GnSmallSmem*>(gs_smem);
+  const uint32_t data = smem_u32(gs_smem) + kGsDataOffset;
+  const T* const first_pixel = reinterpret_cast<const T*>(gs_smem + kGsDataOffset);
+  const int t = static_cast<int>(threadIdx.x);
+  const int blocks = 1 << log_blocks;
+  const int rank = static_cast<int>(blockIdx.x) & (blocks - 1), item = static_cast<int>(blockIdx.x) >> log_blocks;
+  const GnRun& r = a.run[item / a.N];
+  const int n = item % a.N;
+  const int row = a.C * static_cast<int>(sizeof(T));
+  const int pixels = static_cast<int>(r.pixels);
+  const int first = rank * r.per, cnt = max(min(r.per, pixels - first), 0);
+  const size_t base = (static_cast<size_t>(n) * pixels + first) * a.C;
+  const int piece = (cnt + kGsPieces - 1) / kGsPieces;  // pixels of a copy
+  if (t == 0) {
+    for (int i = 0; i < kGsPieces; ++i) mbar_init(&s.full[i], 1);
+    s.abort_flag = 0;
+    fence_barrier_init();
+    for (int i = 0; i * piece < cnt; ++i) {
+      const uint32_t bytes = static_cast<uint32_t>(min(piece, cnt - i * piece) * row);
+      mbar_arrive_expect_tx(&s.full[i], bytes);
+      bulk_load(gs_smem + kGsDataOffset + i * piece * row,
+                static_cast<const uint8_t*>(r.x) + (base * sizeof(T) + static_cast<size_t>(i) * piece * row), bytes,
+                &s.full[i]);
+    }
+  }
+  const int vc = a.C >> 3;
+  const int lanes = min(kGsThreads / vc, kGsMaxLanes);
+  const int pl = t / vc, v = t - pl * vc;
+  const bool active = pl < lanes;
+  const uint32_t mine = data + static_cast<uint32_t>(v * 8 * sizeof(T));
+  GnChannels<kWhole> ch;
+  if (active) ch.weights(r, v);
+  __syncthreads();
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // (this block has started)
+
+  // The block's mean by group, relative to the group's first value in the block (the pivot).
+  bool ok = true;
+  float2 acc[4], p[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) acc[i] = p[i] = both(0.f);
+  for (int i = 0; i * piece < cnt; ++i) {
+    ok = mbar_wait(&s.full[i], 0, &s.abort_flag, a.status, kDevTimeoutNorm) && ok;
+    if (i == 0) {
+      Gn8<T> f;
+      f.load_shared(mine);
+      f.get(p);
+    }
+    if (active)
+      gn_small_pixels<T>(mine, row, pl, lanes, i * piece, min(cnt, (i + 1) * piece), [&](const Gn8<T>& x, int) {
+        float2 f[4];
+        x.get(f);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) acc[k] = add2(acc[k], make_float2(f[k].x - p[k].x, f[k].y - p[k].y));
+      });
+  }
+  // (a timeout has set the status word; the block goes on to the cluster's barriers, with no copy in flight)
+  if (!ok && t == 0)
+    for (int i = 0; i * piece < cnt; ++i) mbar_wait_drain(&s.full[i], 0);
+  // The threads' sums over the pixel lanes, then store(group, f(channel, that) summed over its channels).
+  const bool pow2 = a.cg <= 32 && (a.cg & (a.cg - 1)) == 0;
+  const int width = min(gn_group_width(a, kGsThreads), 32), j = t % width;
+  auto sums = [&](auto&& f, auto&& store) {
+    if (active) gn_lane_store(&s.red[pl * a.C + v * 8], acc);
+    __syncthreads();
+    for (int c0 = 0; c0 < a.C; c0 += kGsThreads) {
+      const int c = c0 + t;
+      float z = 0.f;
+      if (c < a.C) {
+#pragma unroll 8
+        for (int l = 0; l < lanes; ++l) z += s.red[l * a.C + c];
+        z = f(c, z);
+      }
+      if (pow2) {  // adjacent threads have a group's channels
+        z = gn_lane_sum(z, a.cg);
+        if (c < a.C && (c & (a.cg - 1)) == 0) store(c / a.cg, z);
+      } else if (c < a.C) {
+        s.ch[c] = z;
+      }
+    }
+    __syncthreads();
+    if (pow2) return;
+    for (int g0 = 0; g0 < a.groups; g0 += kGsThreads / width) {
+      const int g = g0 + t / width, m = g < a.groups ? a.cg : 0;
+      float z = 0.f;
+      for (int c = j; c < m; c += width) z += s.ch[g * a.cg + c];
+      z = gn_lane_sum(z, width);
+      if (m > 0 && j == 0) store(g, z);
+    }
+    __syncthreads();
+  };
+  const float inv_cnt = cnt > 0 ? 1.f / static_cast<float>(cnt) : 0.f;
+  const float inv_cg = 1.f / static_cast<float>(a.cg);
+  sums(
+      [&](int c, float z) {
+        if (cnt == 0) return 0.f;
+        const int c0 = pow2 ? c & ~(a.cg - 1) : c - c % a.cg;
+        return (to_float(first_pixel[c]) - to_float(first_pixel[c0])) + z * inv_cnt;
+      },
+      [&](int g, float z) {
+        s.pivot[g] = cnt > 0 ? to_float(first_pixel[g * a.cg]) : 0.f;
+        s.mean[g] = z * inv_cg;
+      });
+  // Its squares about that mean.
+  {
+    GnByGroup<kWhole> np, nm;
+    if (active) {
+      np.set(a, v, [&](int g) { return -s.pivot[g]; });
+      nm.set(a, v, [&](int g) { return -s.mean[g]; });
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[i] = both(0.f);
+    if (active)
+      gn_small_pixels<T>(mine, row, pl, lanes, 0, cnt, [&](const Gn8<T>& x, int) {
+        float2 f[4];
+        x.get(f);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float2 d = add2(add2(f[k], np[k]), nm[k]);
+          acc[k] = fma2(d, d, acc[k]);
+        }
+      });
+  }
+  sums([](int, float z) { return z; }, [&](int g, float z) { s.all[2][rank][g] = z; });
+  __syncwarp();
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // (every block has started)
+  for (int i = t; i < blocks << 7; i += kGsThreads) {  // its sums to every block
+    const int to = i / kGsMaxGroups, g = i % kGsMaxGroups;
+    if (g < a.groups) {
+      st_cluster_f32(&s.all[0][rank][g], to, s.pivot[g]);
+      st_cluster_f32(&s.all[1][rank][g], to, s.mean[g]);
+      if (to != rank) st_cluster_f32(&s.all[2][rank][g], to, s.all[2][rank][g]);
+    }
+  }
+  __syncwarp();
+  cluster_sync_all();
+
+  // The image's statistics: a group's 16 threads have a block each.
+  for (int i = t; i < (a.groups + 1) / 2 * (2 * kGsMaxCluster); i += kGsThreads) {
+    const int g = min(i / kGsMaxCluster, a.groups - 1), b = i % kGsMaxCluster;
+    const float share = b < blocks ? static_cast<float>(max(min(r.per, pixels - b * r.per), 0)) : 0.f;
+    const float px = static_cast<float>(pixels), cg = static_cast<float>(a.cg);
+    const float pivot = s.all[0][0][g];
+    const float m = share > 0.f ? (s.all[0][b][g] - pivot) + s.all[1][b][g] : 0.f;
+    const float mean = gn_lane_sum(share * m, kGsMaxCluster) / px;
+    const float d = m - mean;
+    const float m2 = gn_lane_sum(share > 0.f ? fmaf(d * d, share * cg, s.all[2][b][g]) : 0.f, kGsMaxCluster);
+    if (b == 0) {
+      const float mu = mean + pivot;
+      const float rs = 1.f / sqrtf(m2 / (px * cg) + a.eps);
+      s.g1[g] = mu;
+      s.g2[g] = rs;
+      if (rank == 0 && r.mean != nullptr) {
+        r.mean[static_cast<size_t>(n) * a.groups + g] = mu;
+        r.rstd[static_cast<size_t>(n) * a.groups + g] = rs;
+      }
+    }
+  }
+  __syncthreads();
+  if (active) {
+    ch.statistics(a, v, s.g1, s.g2);
+    T* y = static_cast<T*>(r.y) + base + v * 8;
+    switch (a.act) {
+      case kGnRelu: gn_small_apply<T, kGnRelu>(mine, row, pl, lanes, cnt, y, a.C, a.alpha, ch); break;
+      case kGnLeaky: gn_small_apply<T, kGnLeaky>(mine, row, pl, lanes, cnt, y, a.C, a.alpha, ch); break;
+      case kGnSwish: gn_small_apply<T, kGnSwish>(mine, row, pl, lanes, cnt, y, a.C, a.alpha, ch); break;
+      default: gn_small_apply<T, kGnNone>(mine, row, pl, lanes, cnt, y, a.C, a.alpha, ch);
+    }
+  }
+}
+
 // dbias[c] and dweight[c] from every block's row: 32 channels per block, 32 row lanes.
 struct GnSumSpan {
   float* dw;  // null: not wanted
@@ -1310,11 +1539,55 @@ cudaError_t gn_run(const GnSchedule& sc, const GnArgs& a, const GroupNormLevel* 
   return e == cudaSuccess ? gn_sum_rows(sc, a, lv, levels, s) : e;
 }
 
+// The small kernel's cluster size for these maps, 0 where it does not apply: shares of about 16 KB (8 and
+// 32 KB measure the same), in one wave of clusters.  (A cluster's SMs lie in one GPC, so that not all 148
+// can be used: 16 clusters of 8 took two waves, 18.5 us against 10.4 us for 8 of them.)  Against the
+// cooperative kernel, bf16, C = 256, 32 groups: one pixel 6.3 / 10.4 us, 7 x 7 8.3 / 10.5, one to eight of
+// 25 x 38 10.4 / 12.4, four of 50 x 50 (80 KB a block) 12.4 / 14.1; two of 50 x 76 at 122 KB a block would
+// take 14.4 / 12.5.
+int gn_small_blocks(DType dt, int levels, int N, int C, const long long* pixels, int groups) {
+  if (groups > kGsMaxGroups || static_cast<long long>(N) * levels > 128) return 0;
+  const long long row = static_cast<long long>(C) * dtype_size(dt);
+  const int items = N * levels;
+  long long most = 0;
+  for (int l = 0; l < levels; ++l) most = std::max(most, pixels[l]);
+  if (most > kGsMaxCluster * kGsMaxShare / row) return 0;
+  int blocks = 1;
+  while (blocks < kGsMaxCluster && (most + blocks - 1) / blocks * row > (16 << 10)) blocks *= 2;
+  while (blocks > 1 && items * blocks > (blocks >= 8 ? 64 : 128)) blocks /= 2;
+  return (most + blocks - 1) / blocks * row <= kGsMaxShare ? blocks : 0;
+}
+template <typename T, bool kWhole>
+cudaError_t gn_small_launch(GnArgs& a, int levels, int blocks, cudaStream_t s) {
+  const auto kernel = gn_small_kernel<T, kWhole>;
+  static std::atomic<bool> configured[64];
+  const cudaError_t e = once_per_device(configured, [&] {
+    const cudaError_t f =
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             kGsDataOffset + static_cast<int>(kGsMaxShare));
+    return f != cudaSuccess ? f : cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  });
+  if (e != cudaSuccess) return e;
+  int share = 0, log_blocks = 0;
+  while ((1 << log_blocks) < blocks) ++log_blocks;
+  for (int l = 0; l < levels; ++l) {
+    a.run[l].per = static_cast<int>((a.run[l].pixels + blocks - 1) / blocks);
+    share = std::max(share, a.run[l].per);
+  }
+  return launch_ex(kernel, dim3(static_cast<unsigned>(levels * a.N * blocks)), dim3(kGsThreads),
+                   kGsDataOffset + static_cast<size_t>(share) * a.C * sizeof(T), s, LaunchOpts(), blocks, a, log_blocks);
+}
+template <typename T>
+cudaError_t gn_small_run(GnArgs& a, int levels, int blocks, cudaStream_t s) {
+  return a.cg % 8 == 0 ? gn_small_launch<T, true>(a, levels, blocks, s) : gn_small_launch<T, false>(a, levels, blocks, s);
+}
+
 }  // namespace
 
 size_t group_norm_workspace_bytes(DType dt, int levels, int N, int C, const long long* pixels,
                                   int groups, bool backward) {
   if (!gn_sizes_ok(levels, N, C, pixels, groups)) return 0;
+  if (!backward && gn_small_blocks(dt, levels, N, C, pixels, groups) > 0) return 256;  // (unused)
   const GnSchedule sc = gn_schedule_for(dt, levels, N, C, pixels, backward);
   return sc.rows < (1LL << 31) ? gn_workspace(sc, C, groups, backward).total : 0;
 }
@@ -1324,25 +1597,8 @@ cudaError_t launch_group_norm(DType dt, const GroupNormLevel* lv, int levels, in
                               bool backward, void* ws, size_t ws_bytes, int* status,
                               cudaStream_t s) {
   if (!gn_sizes_ok(levels, N, C, pixels, groups)) return cudaErrorInvalidValue;
-  const GnSchedule sc = gn_schedule_for(dt, levels, N, C, pixels, backward);
-  if (sc.rows >= (1LL << 31)) return cudaErrorInvalidValue;
-  const GnWorkspace w = gn_workspace(sc, C, groups, backward);
-  if (w.total > ws_bytes) return cudaErrorInvalidValue;
   GnArgs a;
   std::memset(&a, 0, sizeof(a));
-  for (int l = 0; l < levels; ++l) {
-    a.run[l] = sc.run[l];
-    a.run[l].x = lv[l].x;
-    a.run[l].g = lv[l].grad;
-    a.run[l].y = lv[l].y;
-    a.run[l].w = lv[l].weight;
-    a.run[l].b = lv[l].bias;
-    a.run[l].mean = lv[l].mean;
-    a.run[l].rstd = lv[l].rstd;
-    a.apply |= lv[l].y != nullptr;
-  }
-  std::memcpy(a.phase, sc.phase, sizeof(a.phase));
-  a.phases = sc.phases;
   a.N = N;
   a.C = C;
   a.groups = groups;
@@ -1351,6 +1607,41 @@ cudaError_t launch_group_norm(DType dt, const GroupNormLevel* lv, int levels, in
   a.alpha = alpha;
   a.eps = eps;
   a.status = status;
+  auto maps = [&] {
+    for (int l = 0; l < levels; ++l) {
+      a.run[l].x = lv[l].x;
+      a.run[l].g = lv[l].grad;
+      a.run[l].y = lv[l].y;
+      a.run[l].w = lv[l].weight;
+      a.run[l].b = lv[l].bias;
+      a.run[l].mean = lv[l].mean;
+      a.run[l].rstd = lv[l].rstd;
+      a.run[l].pixels = pixels[l];
+      a.apply |= lv[l].y != nullptr;
+    }
+  };
+  const int small = backward ? 0 : gn_small_blocks(dt, levels, N, C, pixels, groups);
+  if (small > 0) {
+    maps();
+    switch (dt) {
+      case DType::BF16:
+        return gn_small_run<__nv_bfloat16>(a, levels, small, s);
+      case DType::F16:
+        return gn_small_run<__half>(a, levels, small, s);
+      case DType::F32:
+        return gn_small_run<float>(a, levels, small, s);
+      default:
+        return cudaErrorInvalidValue;
+    }
+  }
+  const GnSchedule sc = gn_schedule_for(dt, levels, N, C, pixels, backward);
+  if (sc.rows >= (1LL << 31)) return cudaErrorInvalidValue;
+  const GnWorkspace w = gn_workspace(sc, C, groups, backward);
+  if (w.total > ws_bytes) return cudaErrorInvalidValue;
+  std::memcpy(a.run, sc.run, sizeof(a.run));
+  maps();
+  std::memcpy(a.phase, sc.phase, sizeof(a.phase));
+  a.phases = sc.phases;
   uint8_t* base = static_cast<uint8_t*>(ws);
   a.done = reinterpret_cast<unsigned*>(base);
   a.part = reinterpret_cast<float2*>(base + w.part);
