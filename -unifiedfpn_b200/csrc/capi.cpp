@@ -543,8 +543,8 @@ int group_norm_levels(int dtype, int levels, const void* const* x, const void* c
       return fail(UFPN_ERR_ALIGNMENT, "tensors must be 16-byte aligned");
   }
   const size_t need = ufpn::group_norm_workspace_bytes(*dt, levels, N, C, pixels, groups, backward);
-  if (need == 0) return fail(UFPN_ERR_INVALID_ARG, "sizes out of range");
-  if (!workspace || workspace_bytes < need)
+  if (need == ufpn::kGroupNormNoSizes) return fail(UFPN_ERR_INVALID_ARG, "sizes out of range");
+  if (need > 0 && (!workspace || workspace_bytes < need))
     return fail(UFPN_ERR_INVALID_ARG, "workspace smaller than ufpn_group_norm_workspace");
   if (!ufpn::aligned16(workspace)) return fail(UFPN_ERR_ALIGNMENT, "workspace must be 16-byte aligned");
   return UFPN_OK;
@@ -556,7 +556,8 @@ size_t ufpn_group_norm_workspace(int dtype, int levels, int N, int C, const long
   DType dt;
   if (!parse_dtype(dtype, &dt) || !pixels) return 0;
   try {
-    return ufpn::group_norm_workspace_bytes(dt, levels, N, C, pixels, groups, backward != 0);
+    const size_t need = ufpn::group_norm_workspace_bytes(dt, levels, N, C, pixels, groups, backward != 0);
+    return need == ufpn::kGroupNormNoSizes ? 0 : need;
   } catch (...) {
     return 0;
   }

@@ -1586,10 +1586,10 @@ cudaError_t gn_small_run(GnArgs& a, int levels, int blocks, cudaStream_t s) {
 
 size_t group_norm_workspace_bytes(DType dt, int levels, int N, int C, const long long* pixels,
                                   int groups, bool backward) {
-  if (!gn_sizes_ok(levels, N, C, pixels, groups)) return 0;
-  if (!backward && gn_small_blocks(dt, levels, N, C, pixels, groups) > 0) return 256;  // (unused)
+  if (!gn_sizes_ok(levels, N, C, pixels, groups)) return kGroupNormNoSizes;
+  if (!backward && gn_small_blocks(dt, levels, N, C, pixels, groups) > 0) return 0;
   const GnSchedule sc = gn_schedule_for(dt, levels, N, C, pixels, backward);
-  return sc.rows < (1LL << 31) ? gn_workspace(sc, C, groups, backward).total : 0;
+  return sc.rows < (1LL << 31) ? gn_workspace(sc, C, groups, backward).total : kGroupNormNoSizes;
 }
 
 cudaError_t launch_group_norm(DType dt, const GroupNormLevel* lv, int levels, int N, int C,

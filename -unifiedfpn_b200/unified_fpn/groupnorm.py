@@ -13,6 +13,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+from array import array
 from typing import Sequence
 
 import torch
@@ -32,8 +33,16 @@ def _workspace_bytes(dev: torch.device, code: int, n: int, c: int, pixels: tuple
                       (ctypes.c_longlong * len(pixels))(*pixels), groups, backward)
 
 
-def _ptrs(ts):
-    return (ctypes.c_void_p * len(ts))(*[None if t is None else t.data_ptr() for t in ts])
+def _table(*lists):
+    """The lists' entries (tensors as addresses, None as 0, integers) as one array of 64-bit words, and the
+    address of each list (None for a list that is None).  The array must outlive the call."""
+    words, at = array("Q"), []
+    for entries in lists:
+        at.append(None if entries is None else len(words))
+        if entries is not None:
+            words.extend([t if type(t) is int else 0 if t is None else t.data_ptr() for t in entries])
+    base = words.buffer_info()[0]
+    return words, [None if k is None else base + 8 * k for k in at]
 
 
 def _stream(dev: torch.device) -> int:
@@ -74,7 +83,7 @@ def _levels(input, what: str = "input"):
 def _params(p, what: str, n: int, c: int, dev: torch.device):
     """Per-level fp32 vectors of a weight or bias argument (None, one vector or one per level)."""
     if p is None:
-        return [None] * n, True
+        return None, True
     shared = isinstance(p, torch.Tensor)
     ps = [p] * n if shared else list(p)
     if len(ps) != n:
@@ -134,13 +143,11 @@ def fpn_group_norm(input: torch.Tensor | Sequence[torch.Tensor], weight=None, bi
     code = _DT[xs[0].dtype]
     pixels = tuple([t.shape[2] * t.shape[3] for t in xs])
     need = _workspace_bytes(dev, code, n, c, pixels, groups, 0)
-    work = torch.empty(need, device=dev, dtype=torch.uint8)
-
+    work = torch.empty(need, device=dev, dtype=torch.uint8) if need else None
+    words, (px, xp, yp, wp, bp, mp, rp) = _table(pixels, xs, ys, ws, bs, means, rstds)
     check(_on_device(
-        dev, lib.ufpn_group_norm, code, len(xs), _ptrs(xs), _ptrs(ys), None if weight is None else _ptrs(ws),
-        None if bias is None else _ptrs(bs), _ptrs(means) if means else None, _ptrs(rstds) if rstds else None, n, c,
-        (ctypes.c_longlong * len(xs))(*pixels), groups, eps, _ACTIVATIONS[activation], alpha, work.data_ptr(), need,
-        _stream(dev)), "ufpn_group_norm")
+        dev, lib.ufpn_group_norm, code, len(xs), xp, yp, wp, bp, mp, rp, n, c, px, groups, eps,
+        _ACTIVATIONS[activation], alpha, work.data_ptr() if need else None, need, _stream(dev)), "ufpn_group_norm")
     if single:
         return (ys[0], means[0], rstds[0]) if return_stats else ys[0]
     return (ys, means, rstds) if return_stats else ys
@@ -185,12 +192,11 @@ def fpn_group_norm_backward(input, grad_output, mean, rstd, weight=None, bias=No
     pixels = tuple([t.shape[2] * t.shape[3] for t in xs])
     need = _workspace_bytes(dev, code, n, c, pixels, groups, 1)
     work = torch.empty(need, device=dev, dtype=torch.uint8)
-
+    words, (px, xp, gp, gxp, wp, bp, mp, rp, gwp, gbp) = _table(pixels, xs, gs, gxs, ws, bs, means, rstds, gw + pad,
+                                                                gb + pad)
     check(_on_device(
-        dev, lib.ufpn_group_norm_backward, code, len(xs), _ptrs(xs), _ptrs(gs), _ptrs(gxs) if gxs else None, _ptrs(ws),
-        _ptrs(bs), _ptrs(means), _ptrs(rstds), _ptrs(gw + pad), _ptrs(gb + pad), n, c,
-        (ctypes.c_longlong * len(xs))(*pixels), groups, _ACTIVATIONS[activation], alpha, work.data_ptr(), need,
-        _stream(dev)), "ufpn_group_norm_backward")
+        dev, lib.ufpn_group_norm_backward, code, len(xs), xp, gp, gxp, wp, bp, mp, rp, gwp, gbp, n, c, px, groups,
+        _ACTIVATIONS[activation], alpha, work.data_ptr(), need, _stream(dev)), "ufpn_group_norm_backward")
     if single or shared:
         return (gxs[0] if single and gxs else gxs), gw[0], gb[0]
     # a parameter shared by the maps beside one that is not: its gradient is the sum over the maps

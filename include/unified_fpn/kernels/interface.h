@@ -117,7 +117,8 @@ struct GroupNormLevel {
   float* dweight;  // backward, [C], null: not wanted; a level after the first with neither adds
   float* dbias;    // its sums to the level before it (weights shared by several levels)
 };
-// Scratch of one call (0: sizes out of range).  pixels[l] = H * W of level l.
+// Scratch of one call (kGroupNormNoSizes: sizes out of range; 0: none).  pixels[l] = H * W of level l.
+constexpr size_t kGroupNormNoSizes = ~static_cast<size_t>(0);
 size_t group_norm_workspace_bytes(DType dt, int levels, int N, int C, const long long* pixels,
                                   int groups, bool backward);
 cudaError_t launch_group_norm(DType dt, const GroupNormLevel* lv, int levels, int N, int C,

@@ -319,7 +319,7 @@ size_t ufpn_lateral_adapters_workspace(int dtype, int N, int Cin, int H, int W, 
  *   mean, rstd: [levels] fp32 [N][groups] outputs for the backward; the arrays may be NULL.
  *   pixels: [levels] H * W.
  *   workspace: ufpn_group_norm_workspace(...) bytes of device memory, 16-byte aligned, used by
- *   this call alone until it has run. */
+ *   this call alone until it has run; may be NULL where that is 0. */
 int ufpn_group_norm(int dtype, int levels, const void* const* x, void* const* y,
                     const float* const* weight, const float* const* bias, float* const* mean,
                     float* const* rstd, int N, int C, const long long* pixels, int groups, float eps,
@@ -336,7 +336,8 @@ int ufpn_group_norm_backward(int dtype, int levels, const void* const* x, const 
                              float* const* grad_bias, int N, int C, const long long* pixels,
                              int groups, int activation, float alpha, void* workspace,
                              size_t workspace_bytes, void* stream);
-/* Workspace bytes of either (0 for sizes that they refuse). */
+/* Workspace bytes of either on the current device (0: small maps, which need none, and sizes that
+ * the calls refuse). */
 size_t ufpn_group_norm_workspace(int dtype, int levels, int N, int C, const long long* pixels,
                                  int groups, int backward);
 

@@ -23,9 +23,9 @@ def _px(*v):
 
 
 def _norm(L, **kw):
-    """ufpn_group_norm of one map 1 x 64 x 100 with arguments replaced by name."""
+    """ufpn_group_norm of one map 1 x 64 x 100000 with arguments replaced by name."""
     a = dict(dtype=2, levels=1, x=_arr(OK), y=_arr(OK), weight=None, bias=None, mean=None, rstd=None, N=1, C=64,
-             pixels=_px(100), groups=8, eps=1e-5, act=0, alpha=0.0, ws=OK, ws_bytes=1 << 40)
+             pixels=_px(100000), groups=8, eps=1e-5, act=0, alpha=0.0, ws=OK, ws_bytes=1 << 40)
     a.update(kw)
     return L.lib.ufpn_group_norm(*a.values(), None)
 
@@ -66,8 +66,8 @@ def test_group_norm_refusals_of_one_direction(L):
 
 def test_group_norm_workspace(L):
     size = lambda c=64, g=8, bwd=0, *px: L.lib.ufpn_group_norm_workspace(2, len(px), 2, c, _px(*px), g, bwd)  # noqa: E731
-    assert size(64, 8, 0, 100) > 0
-    assert size(64, 8, 1, 100) > size(64, 8, 0, 100)
+    assert size(64, 8, 0, 100) == 0 and size(64, 8, 0, 100000) > 0  # (small maps need none)
+    assert size(64, 8, 1, 100) > 0 and size(64, 8, 1, 100000) > size(64, 8, 0, 100000)
     assert size(64, 8, 0, 1 << 22) < 64 << 20  # (partials, not a copy of the map)
     for bad in ((12, 4, 0, 100), (64, 7, 0, 100), (64, 8, 0, 0), (64, 8, 0), (64, 8, 0, *[4] * 9)):
         assert size(*bad) == 0
