@@ -1013,7 +1013,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   const int split = u % a.splits;
   const int n = a.n0 + u / a.splits;
   const int adapter = __ldg(a.index + n);
-  if (adapter < 0 || adapter >= a.adapters) return;  // (before any barrier or TMEM)
+  if (adapter < 0 || adapter >= a.adapters) {  // (before any barrier or TMEM)
+    griddep_wait();
+    return;
+  }
 
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_addr = smem_u32(smem_raw);
@@ -1206,17 +1209,47 @@ __global__ void __launch_bounds__(256) adapter_reduce_kernel(const ArArgs a) {
   *out = a.more ? *out + acc : acc;
 }
 
-// up [L][256][R] -> [L][R][256]
-__global__ void __launch_bounds__(256) adapter_transpose_kernel(const uint16_t* __restrict__ up,
-                                                                uint16_t* __restrict__ out, int rank) {
-  const size_t a = blockIdx.x;
-  for (int r = 0; r < rank; ++r)
-    out[(a * rank + r) * 256 + threadIdx.x] = up[(a * 256 + threadIdx.x) * rank + r];
+// The backward's operands: up [L][256][R] -> [L][R][256] (block l), and W [256][K] -> [K rounded up to
+// 256][256], 32 input channels a block, zeros past K.
+__global__ void __launch_bounds__(256)
+    adapter_transpose_kernel(const uint16_t* __restrict__ up, uint16_t* __restrict__ up_t, int rank, int adapters,
+                             const uint16_t* __restrict__ w, uint16_t* __restrict__ w_t, int K) {
+  griddep_launch_dependents();
+  const int t = static_cast<int>(threadIdx.x);
+  if (static_cast<int>(blockIdx.x) < adapters) {
+    const size_t a = blockIdx.x;
+#pragma unroll 4
+    for (int r = 0; r < rank; ++r) up_t[(a * rank + r) * 256 + t] = __ldg(up + (a * 256 + t) * rank + r);
+    return;
+  }
+  __shared__ __align__(16) uint16_t tile[32][256 + 8];
+  const int k0 = (static_cast<int>(blockIdx.x) - adapters) * 32;
+  uint4 q[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = i * 64 + (t >> 2), k = k0 + (t & 3) * 8;
+    q[i] = k < K ? __ldg(reinterpret_cast<const uint4*>(w + static_cast<size_t>(row) * K + k)) : make_uint4(0u, 0u, 0u, 0u);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t u[4] = {q[i].x, q[i].y, q[i].z, q[i].w};
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      tile[(t & 3) * 8 + e][i * 64 + (t >> 2)] = static_cast<uint16_t>(u[e >> 1] >> (16 * (e & 1)));
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = i * 8 + (t >> 5);
+    *reinterpret_cast<uint4*>(w_t + static_cast<size_t>(k0 + row) * 256 + (t & 31) * 8) =
+        *reinterpret_cast<const uint4*>(&tile[row][(t & 31) * 8]);
+  }
 }
 
 // ------------------------------------------------------------------ host side
 template <typename T, int RP, bool kTaps>
-cudaError_t launch_adapter_rp(const TcPlan& p, const CUtensorMap& map_u, const AdArgs& ad, cudaStream_t s) {
+cudaError_t launch_adapter_rp(const TcPlan& p, const CUtensorMap& map_u, const AdArgs& ad, const LaunchOpts& opts,
+                              cudaStream_t s) {
   using Cfg = AdCfg<RP, kAdParts<T>>;
   auto kern = fpn_adapter_kernel<T, RP, kTaps>;
   static std::atomic<bool> configured[64];
@@ -1226,21 +1259,23 @@ cudaError_t launch_adapter_rp(const TcPlan& p, const CUtensorMap& map_u, const A
   if (e != cudaSuccess) return e;
   TcGemmArgs a;
   std::memcpy(&a, p.args, sizeof(a));
-  return launch_ex(kern, dim3(p.grid), dim3(kAdThreads), Cfg::kSmemBytes, s, LaunchOpts(), 1, p.map_a,
+  return launch_ex(kern, dim3(p.grid), dim3(kAdThreads), Cfg::kSmemBytes, s, opts, 1, p.map_a,
                    p.map_b, p.map_coarse, map_u, a, ad);
 }
 template <typename T, bool kTaps>
-cudaError_t launch_adapter_rank(const TcPlan& p, const CUtensorMap& map_u, const AdArgs& ad, cudaStream_t s) {
-  return ad.rank <= 16   ? launch_adapter_rp<T, 16, kTaps>(p, map_u, ad, s)
-         : ad.rank <= 32 ? launch_adapter_rp<T, 32, kTaps>(p, map_u, ad, s)
-                         : launch_adapter_rp<T, 64, kTaps>(p, map_u, ad, s);
+cudaError_t launch_adapter_rank(const TcPlan& p, const CUtensorMap& map_u, const AdArgs& ad, const LaunchOpts& opts,
+                                cudaStream_t s) {
+  return ad.rank <= 16   ? launch_adapter_rp<T, 16, kTaps>(p, map_u, ad, opts, s)
+         : ad.rank <= 32 ? launch_adapter_rp<T, 32, kTaps>(p, map_u, ad, opts, s)
+                         : launch_adapter_rp<T, 64, kTaps>(p, map_u, ad, opts, s);
 }
 template <typename T>
-cudaError_t launch_adapter_t(const TcPlan& p, const CUtensorMap& map_u, const AdArgs& ad, cudaStream_t s) {
+cudaError_t launch_adapter_t(const TcPlan& p, const CUtensorMap& map_u, const AdArgs& ad, const LaunchOpts& opts,
+                             cudaStream_t s) {
   TcGemmArgs a;
   std::memcpy(&a, p.args, sizeof(a));
-  return a.coarse != nullptr && a.cbox_w <= 0 ? launch_adapter_rank<T, true>(p, map_u, ad, s)
-                                              : launch_adapter_rank<T, false>(p, map_u, ad, s);
+  return a.coarse != nullptr && a.cbox_w <= 0 ? launch_adapter_rank<T, true>(p, map_u, ad, opts, s)
+                                              : launch_adapter_rank<T, false>(p, map_u, ad, opts, s);
 }
 
 int pad8(int v) { return (v + 7) / 8 * 8; }
@@ -1407,7 +1442,7 @@ cudaError_t adapter_grads_t(const AdapterProblem& p, const void* x, const void* 
     a.part = part;
     a.status = status;
     e = launch_ex(kern, dim3(static_cast<unsigned>(images) * g.splits * g.blocks), dim3(kTcThreads),
-                  kAgSmemBytes, s, LaunchOpts(), 1, mx, my, mdh, mh, a);
+                  kAgSmemBytes, s, pdl, 1, mx, my, mdh, mh, a);
     if (e != cudaSuccess) return e;
     ArArgs r;
     std::memset(&r, 0, sizeof(r));
@@ -1424,8 +1459,7 @@ cudaError_t adapter_grads_t(const AdapterProblem& p, const void* x, const void* 
     r.ddown = ddown;
     r.dup = dup;
     r.more = n0 > 0;
-    e = launch_ex(adapter_reduce_kernel, dim3(g.blocks * p.rank, p.adapters), dim3(256), 0, s,
-                  LaunchOpts(), 1, r);
+    e = launch_ex(adapter_reduce_kernel, dim3(g.blocks * p.rank, p.adapters), dim3(256), 0, s, pdl, 1, r);
     if (e != cudaSuccess) return e;
   }
   return cudaSuccess;
@@ -1487,8 +1521,8 @@ cudaError_t launch_lateral_adapters(const AdapterProblem& p, const void* x, cons
   const AdView v = adapter_view(p, coarse != nullptr);
   e = plan_tc_lateral(plan, p.dtype, x, w, bias, coarse, out, p.N, p.Cin, v.H, v.W, Hc, Wc, v.tiling, status, 0);
   if (e != cudaSuccess) return e;
-  return p.dtype == DType::BF16 ? launch_adapter_t<__nv_bfloat16>(plan, map_u, ad, s)
-                                : launch_adapter_t<__half>(plan, map_u, ad, s);
+  return p.dtype == DType::BF16 ? launch_adapter_t<__nv_bfloat16>(plan, map_u, ad, LaunchOpts(), s)
+                                : launch_adapter_t<__half>(plan, map_u, ad, LaunchOpts(), s);
 }
 
 size_t lateral_adapters_workspace_bytes(const AdapterProblem& p, bool has_w_t, bool need_dx) {
@@ -1506,15 +1540,14 @@ cudaError_t launch_lateral_adapters_backward(const AdapterProblem& p, const void
   uint8_t* base = static_cast<uint8_t*>(ws);
   void* up_t = base + wl.up_t;
   void* dh = base + wl.dh;
-  cudaError_t e = launch_ex(adapter_transpose_kernel, dim3(p.adapters), dim3(256), 0, s, LaunchOpts(), 1,
-                            static_cast<const uint16_t*>(up), static_cast<uint16_t*>(up_t), p.rank);
-  if (e != cudaSuccess) return e;
   const int slices = (p.Cin + 255) / 256;
-  if (dx && !w_t) {
-    if ((e = launch_transpose_weights(p.dtype, w, base + wl.w_t, 256, p.Cin, slices * 256, s)) != cudaSuccess)
-      return e;
-    w_t = base + wl.w_t;
-  }
+  const bool own_w_t = dx && !w_t;
+  cudaError_t e = launch_ex(adapter_transpose_kernel, dim3(p.adapters + (own_w_t ? slices * 8 : 0)), dim3(256), 0, s,
+                            LaunchOpts(), 1, static_cast<const uint16_t*>(up), static_cast<uint16_t*>(up_t), p.rank,
+                            p.adapters, static_cast<const uint16_t*>(w), reinterpret_cast<uint16_t*>(base + wl.w_t),
+                            p.Cin);
+  if (e != cudaSuccess) return e;
+  if (own_w_t) w_t = base + wl.w_t;
   const AdView v = adapter_view(p, false);
   TcPlan plan;
   // (without dx the output and weight maps are unused: any valid tensors)
@@ -1543,8 +1576,11 @@ cudaError_t launch_lateral_adapters_backward(const AdapterProblem& p, const void
   ad.h_accs = ad_h_accs(4);
   ad.out = dx;
   ad.out_c = p.Cin;
-  e = p.dtype == DType::BF16 ? launch_adapter_t<__nv_bfloat16>(plan, map_u, ad, s)
-                             : launch_adapter_t<__half>(plan, map_u, ad, s);
+  // The call's kernels after the first launch ahead and wait on the device for the one before.
+  LaunchOpts ahead;
+  ahead.pdl = true;
+  e = p.dtype == DType::BF16 ? launch_adapter_t<__nv_bfloat16>(plan, map_u, ad, ahead, s)
+                             : launch_adapter_t<__half>(plan, map_u, ad, ahead, s);
   if (e != cudaSuccess) return e;
   float* part = reinterpret_cast<float*>(base + wl.part);
   return p.dtype == DType::BF16

@@ -155,9 +155,8 @@ def fpn_lateral_adapters_backward(input: torch.Tensor, weight: torch.Tensor | No
         else:
             wt = _weight(weight, x)
     gx = torch.empty_like(x, memory_format=_CL) if need_input_grad else None
-    grads = torch.empty(count * rank * (cin + 256), device=dev, dtype=torch.float32)
-    gdown = grads[:count * rank * cin].view(count, rank, cin)
-    gup = grads[count * rank * cin:].view(count, 256, rank)
+    gdown = torch.empty((count, rank, cin), device=dev, dtype=torch.float32)
+    gup = torch.empty((count, 256, rank), device=dev, dtype=torch.float32)
     code = _DT[x.dtype]
 
     need = _on_device(dev, lib.ufpn_lateral_adapters_workspace, code, n, cin, h, w, rank, count, wtt is not None,

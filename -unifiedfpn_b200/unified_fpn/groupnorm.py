@@ -138,8 +138,8 @@ def fpn_group_norm(input: torch.Tensor | Sequence[torch.Tensor], weight=None, bi
             raise ValueError("out must be channels_last maps like the inputs")
     means = rstds = None
     if return_stats:
-        stats = torch.empty((2, len(xs), n, groups), device=dev, dtype=torch.float32)
-        means, rstds = list(stats[0]), list(stats[1])
+        stats = torch.empty((2 * len(xs), n, groups), device=dev, dtype=torch.float32).unbind()
+        means, rstds = list(stats[:len(xs)]), list(stats[len(xs):])
     code = _DT[xs[0].dtype]
     pixels = tuple([t.shape[2] * t.shape[3] for t in xs])
     need = _workspace_bytes(dev, code, n, c, pixels, groups, 0)
@@ -165,9 +165,11 @@ def fpn_group_norm_backward(input, grad_output, mean, rstd, weight=None, bias=No
         raise ValueError(f"unknown activation {activation!r}")
     xs, single = _levels(input)
     gs, _ = _levels(grad_output, "grad_output")
-    if len(gs) != len(xs) or any(g.shape != x.shape or g.dtype is not x.dtype or g.device != x.device
-                                 for g, x in zip(gs, xs)):
+    if len(gs) != len(xs):
         raise ValueError("grad_output must have the input's shapes, dtype and device")
+    for g, x in zip(gs, xs):
+        if g.shape != x.shape or g.dtype is not x.dtype or g.device != x.device:
+            raise ValueError("grad_output must have the input's shapes, dtype and device")
     n, c = xs[0].shape[:2]
     dev = xs[0].device
     means = [mean] if isinstance(mean, torch.Tensor) else list(mean)
@@ -175,18 +177,20 @@ def fpn_group_norm_backward(input, grad_output, mean, rstd, weight=None, bias=No
     groups = means[0].shape[-1] if means and means[0].dim() == 2 else 0
     _check_groups(c, groups)
     for ts, what in ((means, "mean"), (rstds, "rstd")):
-        if len(ts) != len(xs) or any(tuple(t.shape) != (n, groups) or t.dtype is not torch.float32
-                                     or t.device != dev for t in ts):
+        ok = len(ts) == len(xs)
+        for k, t in enumerate(ts):
+            ok = ok and t.shape == (n, groups) and t.dtype is torch.float32 and t.device == dev
+            if ok and not t.is_contiguous():
+                ts[k] = t.contiguous()
+        if not ok:
             raise ValueError(f"{what} must be fp32 [N, groups] per map on the maps' device")
-    means = [t.contiguous() for t in means]
-    rstds = [t.contiguous() for t in rstds]
     ws, shared_w = _params(weight, "weight", len(xs), c, dev)
     bs, shared_b = _params(bias, "bias", len(xs), c, dev)
     shared = shared_w and shared_b
     gxs = [torch.empty_like(t, memory_format=_CL) for t in xs] if need_input_grad else None
     rows = 1 if shared else len(xs)
-    gwb = torch.empty((2, rows, c), device=dev, dtype=torch.float32)
-    gw, gb = list(gwb[0]), list(gwb[1])
+    gwb = torch.empty((2 * rows, c), device=dev, dtype=torch.float32).unbind()
+    gw, gb = list(gwb[:rows]), list(gwb[rows:])
     pad = [None] * (len(xs) - rows)
     code = _DT[xs[0].dtype]
     pixels = tuple([t.shape[2] * t.shape[3] for t in xs])
