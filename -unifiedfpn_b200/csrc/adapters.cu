@@ -108,13 +108,15 @@ __device__ __forceinline__ int ad_adapter(const AdArgs& a, int n) {
   return i >= 0 && i < a.adapters ? i : -1;
 }
 
-// v ~ the sum of its parts.  (fp16: a value beyond its range keeps the rest in the second.)
+// v ~ the sum of its parts.  (A value beyond the type's range keeps the rest in the next part; infinity, and
+// what exceeds the parts' ranges together, ends in the last one.)
 template <typename T>
 __device__ __forceinline__ void ad_split(float v, uint16_t (&part)[kAdParts<T>]) {
+  constexpr float kMax = TcElem<T>::kFmt == 0 ? 65504.f : 3.3895313892515355e38f;
 #pragma unroll
   for (int i = 0; i < kAdParts<T>; ++i) {
     float c = v;
-    if constexpr (TcElem<T>::kFmt == 0) c = v > 65504.f ? 65504.f : (v < -65504.f ? -65504.f : v);
+    if (i + 1 < kAdParts<T>) c = v > kMax ? kMax : (v < -kMax ? -kMax : v);
     part[i] = Pack<T>::bits(c);
     v -= Pack<T>::unpack(static_cast<uint32_t>(part[i])).x;
   }

@@ -205,3 +205,36 @@ def test_graphed_steps_with_changing_indices(cuda_device):
             assert torch.equal(a, b), (seed, k)
     torch.cuda.synchronize()
     assert U.device_status() == 0
+
+
+def test_calls_at_once_on_two_streams(cuda_device):
+    """Norms of maps of both forms and adapters of both, running on two streams together: the results of the
+    same calls one after the other, bit for bit."""
+    import unified_fpn as U
+    g = torch.Generator().manual_seed(5)
+
+    def t(*shape):
+        return torch.randn(*shape, generator=g).to(torch.bfloat16).to(cuda_device)
+    maps = [t(2, 256, 120, 160).contiguous(memory_format=CL), t(1, 256, 9, 11).contiguous(memory_format=CL)]
+    x = [t(2, 256, 120, 160).contiguous(memory_format=CL), t(2, 1024, 12, 13).contiguous(memory_format=CL)]
+    w, down, up = [t(256, v.shape[1]) for v in x], [t(2, 8, v.shape[1]) for v in x], t(2, 256, 8)
+    b, index = torch.zeros(256, device=cuda_device), torch.tensor([1, 0], device=cuda_device)
+
+    def calls(k):
+        out = list(U.fpn_group_norm(maps[k], groups=32, activation="swish", return_stats=True))
+        out.append(U.fpn_group_norm_backward(maps[k], maps[k], out[1], out[2], activation="swish")[0])
+        o, h = U.fpn_lateral_adapters(x[k], w[k], b, down[k], up, index, return_hidden=True)
+        return out + [o, *U.fpn_lateral_adapters_backward(x[k], w[k], o, down[k], up, index, h)]
+    want = [calls(0), calls(1)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(cuda_device), torch.cuda.Stream(cuda_device)]
+    got = [[], []]
+    for _ in range(6):
+        for k, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[k].append(calls(k))
+    torch.cuda.synchronize()
+    assert U.device_status() == 0
+    for k in range(2):
+        for run in got[k]:
+            assert all(torch.equal(a, v) for a, v in zip(run, want[k]))

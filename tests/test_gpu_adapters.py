@@ -320,3 +320,29 @@ def test_few_tiles_split_over_k(cuda_device, dtype, shape, size):
     x[0] = float("nan")
     other = U.fpn_lateral_adapters(x, s["w"], s["b"], s["down"], s["up"], s["index"], scale=s["scales"], coarse=coarse)
     assert other[0].isnan().all() and torch.equal(other[1:], out[1:])
+
+
+@pytest.mark.parametrize("h,w", [(3, 5), (130, 120)])  # (split over k, and not)
+def test_hidden_values_beyond_the_16_bit_range(cuda_device, h, w):
+    """fp16: h = 102 400 (above 65 504) still counts in full; beyond both parts' range the result is not finite
+    rather than a wrong number.  bf16: infinities stay infinities."""
+    import unified_fpn as U
+    dev, cin = cuda_device, 512
+    x = torch.ones(2, cin, h, w, device=dev, dtype=torch.float16).contiguous(memory_format=CL)
+    wt, b = torch.zeros(256, cin, device=dev, dtype=torch.float16), torch.zeros(256, device=dev)
+    down = torch.full((2, 1, cin), 200.0, device=dev, dtype=torch.float16)
+    down[1] = 800.0
+    up = torch.full((2, 256, 1), 2.0 ** -10, device=dev, dtype=torch.float16)
+    index = torch.tensor([0, 1], device=dev)
+    out, hid = U.fpn_lateral_adapters(x, wt, b, down, up, index, return_hidden=True)
+    assert (out[0] == 100.0).all() and (hid[0].float().sum(2)[..., 0] == 102400.0).all()
+    assert not hid[1].float().sum(2)[..., 0].isfinite().any()
+    gd, gu = U.fpn_lateral_adapters_backward(x, None, torch.ones_like(out), down, up, index, hid,
+                                             need_input_grad=False)[1:]
+    assert (gu[0] == 102400.0 * h * w).all() and not gu[1].isfinite().any()
+    assert gd[0].isfinite().all()
+    xb = x.bfloat16().contiguous(memory_format=CL)
+    xb[1, 0, 0, 0] = float("inf")
+    out, hid = U.fpn_lateral_adapters(xb, wt.bfloat16(), b, down.bfloat16(), up.bfloat16(), index, return_hidden=True)
+    assert (hid[1, 0, 0].float().sum(0)[0] == float("inf")) and hid[0].isfinite().all()
+    assert out[0].isfinite().all() and out[1, :, 1:].isfinite().all()
