@@ -121,7 +121,7 @@ __device__ __forceinline__ void gn_put(T* p, const float2 (&f)[4]) {
       h[2 * e] = f[i * (V / 2) + e].x;
       h[2 * e + 1] = f[i * (V / 2) + e].y;
     }
-    *(reinterpret_cast<uint4*>(p) + i) = Vec16<T>::pack(h);
+    __stcs(reinterpret_cast<uint4*>(p) + i, Vec16<T>::pack(h));  // (not read again here: x keeps the L2 cache)
   }
 }
 
@@ -321,7 +321,10 @@ struct GnCursor {
 };
 
 // A warp's ring of kStages copies and the batches of its chunks through it.
-template <typename T, bool kBackward, int kStages>
+// kLast: the last reading of its maps, which may leave the L2 cache.  (The forward's first reading asks to
+// stay, 42 against 49 us for an R50 pyramid; the backward's, of twice the bytes, does better not to: 146
+// against 154 us for the training pyramid.)
+template <typename T, bool kBackward, int kStages, bool kLast>
 struct GnRing {
   static constexpr int kEsz = static_cast<int>(sizeof(T));
   uint8_t* buf;
@@ -348,6 +351,9 @@ struct GnRing {
     dy = static_cast<const uint8_t*>(r.g) + off;
     ahead = 0;
   }
+  __device__ __forceinline__ void load(uint8_t* dst, const uint8_t* src, uint32_t bytes, int slot) {
+    bulk_load_hint(dst, src, bytes, &full[slot], kLast || kBackward ? kPolicyEvictFirst : kPolicyEvictLast);
+  }
   // Starts batch i into a stage.
   __device__ __forceinline__ void issue(const GnArgs& a, const GnLanes& ln, int i, int slot) {
     const int lane = static_cast<int>(threadIdx.x) & 31;
@@ -360,15 +366,14 @@ struct GnRing {
     const uint32_t bytes = static_cast<uint32_t>(n * row);
     if (lane == 0) mbar_arrive_expect_tx(&full[slot], kBackward ? 2 * bytes : bytes);
     if (ln.cbs == 1) {  // whole pixels: contiguous
-      bulk_load(dst, x + off, bytes, &full[slot]);
-      if constexpr (kBackward) bulk_load(dst + kGnStage / 2, dy + off, bytes, &full[slot]);
+      load(dst, x + off, bytes, slot);
+      if constexpr (kBackward) load(dst + kGnStage / 2, dy + off, bytes, slot);
     } else {
       __syncwarp();
       for (int k = lane; k < n; k += 32) {
         const size_t o = off + static_cast<size_t>(k) * (a.C * kEsz);
-        bulk_load(dst + k * row, x + o, static_cast<uint32_t>(row), &full[slot]);
-        if constexpr (kBackward)
-          bulk_load(dst + kGnStage / 2 + k * row, dy + o, static_cast<uint32_t>(row), &full[slot]);
+        load(dst + k * row, x + o, static_cast<uint32_t>(row), slot);
+        if constexpr (kBackward) load(dst + kGnStage / 2 + k * row, dy + o, static_cast<uint32_t>(row), slot);
       }
     }
   }
@@ -1012,7 +1017,7 @@ __global__ void __launch_bounds__(2 * kGnThreads + kGnMergeThreads, 1)
   __syncthreads();
   if (warp < kGnWarps) {
     const GnLanes ln(a.C, static_cast<int>(sizeof(T)), warp, lane, kCapacity);
-    GnRing<T, kBackward, kGnStatsStages> ring;
+    GnRing<T, kBackward, kGnStatsStages, false> ring;
     ring.buf = s.stats_ring[warp];
     ring.full = s.stats_full[warp];
     GnCursor cur(a);
@@ -1055,7 +1060,7 @@ __global__ void __launch_bounds__(2 * kGnThreads + kGnMergeThreads, 1)
     return;
   } else if (warp < 2 * kGnWarps) {
     const GnLanes ln(a.C, static_cast<int>(sizeof(T)), warp - kGnWarps, lane, kCapacity);
-    GnRing<T, kBackward, kGnApplyStages> ring;
+    GnRing<T, kBackward, kGnApplyStages, true> ring;
     ring.buf = s.apply_ring[warp - kGnWarps];
     ring.full = s.apply_full[warp - kGnWarps];
     uint32_t phase = 0;
