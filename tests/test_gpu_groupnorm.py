@@ -4,8 +4,8 @@ Tolerances are counted, not fitted.  A result is an fp32 computation rounded onc
 type: half a step of that type (finfo.eps / 2, relative) plus the fp32 part.  With u = 2^-24, S =
 1 + max |x| rstd |w| + |b| bounds every intermediate: x - mean carries u |x| for the stored mean
 and u for itself, the mean and rstd a few u each (their sums are trees of at most some dozens of
-sequential fp32 additions), the activation's sigmoid 2^-21 relative for 16-bit maps: 16 u S = 2^-20
-S covers their sum for values, and each gradient factor below says what it multiplies.
+sequential fp32 additions), the swish of 16-bit maps 2^-21 (1 + |z|) for its approximate exponential and
+reciprocal: 16 u S = 2^-20 S covers their sum for values, and each gradient factor below says what it multiplies.
 """
 import pytest
 import torch
