@@ -1292,6 +1292,14 @@ int parts_of(DType dt) { return dt == DType::BF16 ? kAdParts<__nv_bfloat16> : kA
 int rank_tile(int rank) { return rank <= 16 ? 16 : rank <= 32 ? 32 : 64; }
 size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 
+// Launched ahead of the end of the kernel before on the stream, which the kernel waits for on the device
+// before it reads or writes anything (1 to 3 us a call: 143.7 -> 141.6 for P2 of eight images).
+LaunchOpts adapter_ahead() {
+  LaunchOpts o;
+  o.pdl = true;
+  return o;
+}
+
 // Runs fpn_adapter_split_kernel with S CTAs a tile if they are all resident at once and 4 k-blocks are
 // left for each (fewer cost more in the exchange than they save: 2 of rank 64 a CTA on 50 x 76 pixels,
 // 16.5 us, 4 of them 14.5 us, as long as unsplit); sets `done`.  Measured, split against not, 16 bits:
@@ -1328,7 +1336,7 @@ cudaError_t try_adapter_split(const TcPlan& p, const TcGemmArgs& a, const CUtens
   }
   if (a.num_tiles > fit) return cudaSuccess;
   *done = true;
-  return launch_ex(kern, dim3(a.num_tiles * S), dim3(kAdThreads), as_smem(RP).total, s, LaunchOpts(), S, p.map_a,
+  return launch_ex(kern, dim3(a.num_tiles * S), dim3(kAdThreads), as_smem(RP).total, s, adapter_ahead(), S, p.map_a,
                    p.map_b, map_u, a, ad);
 }
 // The split into the most CTAs a tile that run at once; `done` stays false where none does.
@@ -1433,8 +1441,7 @@ cudaError_t adapter_grads_t(const AdapterProblem& p, const void* x, const void* 
     return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kAgSmemBytes);
   });
   if (e != cudaSuccess) return e;
-  LaunchOpts pdl;
-  pdl.pdl = true;
+  const LaunchOpts pdl = adapter_ahead();
   for (int n0 = 0; n0 < p.N; n0 += g.images) {
     const int images = std::min(g.images, p.N - n0);
     AgArgs a;
@@ -1530,8 +1537,8 @@ cudaError_t launch_lateral_adapters(const AdapterProblem& p, const void* x, cons
   const AdView v = adapter_view(p, coarse != nullptr);
   e = plan_tc_lateral(plan, p.dtype, x, w, bias, coarse, out, p.N, p.Cin, v.H, v.W, Hc, Wc, v.tiling, status, 0);
   if (e != cudaSuccess) return e;
-  return p.dtype == DType::BF16 ? launch_adapter_t<__nv_bfloat16>(plan, map_u, ad, LaunchOpts(), s)
-                                : launch_adapter_t<__half>(plan, map_u, ad, LaunchOpts(), s);
+  return p.dtype == DType::BF16 ? launch_adapter_t<__nv_bfloat16>(plan, map_u, ad, adapter_ahead(), s)
+                                : launch_adapter_t<__half>(plan, map_u, ad, adapter_ahead(), s);
 }
 
 size_t lateral_adapters_workspace_bytes(const AdapterProblem& p, bool has_w_t, bool need_dx) {
@@ -1585,11 +1592,8 @@ cudaError_t launch_lateral_adapters_backward(const AdapterProblem& p, const void
   ad.h_accs = ad_h_accs(4);
   ad.out = dx;
   ad.out_c = p.Cin;
-  // The call's kernels after the first launch ahead and wait on the device for the one before.
-  LaunchOpts ahead;
-  ahead.pdl = true;
-  e = p.dtype == DType::BF16 ? launch_adapter_t<__nv_bfloat16>(plan, map_u, ad, ahead, s)
-                             : launch_adapter_t<__half>(plan, map_u, ad, ahead, s);
+  e = p.dtype == DType::BF16 ? launch_adapter_t<__nv_bfloat16>(plan, map_u, ad, adapter_ahead(), s)
+                             : launch_adapter_t<__half>(plan, map_u, ad, adapter_ahead(), s);
   if (e != cudaSuccess) return e;
   float* part = reinterpret_cast<float*>(base + wl.part);
   return p.dtype == DType::BF16
