@@ -201,6 +201,17 @@ class _NeckFunction(torch.autograd.Function):
                 *gl, *gbl, *gw3, *gb3)
 
 
+def _output_grads(grads, maps) -> list:
+    """Gradients of P2..P5 like ``maps`` (zeros for one that is None), P6's added to P5's."""
+    g = [torch.zeros_like(m, memory_format=_CL) if d is None else _layout(d, m.dtype, m.device)
+         for d, m in zip(grads, maps)]
+    if len(grads) > 4 and grads[4] is not None:
+        if grads[3] is not None and g[3].data_ptr() == grads[3].data_ptr():  # (the caller's stays as it is)
+            g[3] = g[3].clone(memory_format=_CL)
+        fpn_p6_backward(_layout(grads[4], maps[3].dtype, maps[3].device), g[3])
+    return g
+
+
 class _NormFunction(torch.autograd.Function):
     """Group norm and activation of P2..P5, and P6 from the normed P5."""
 
@@ -216,13 +227,7 @@ class _NormFunction(torch.autograd.Function):
     def backward(ctx, *grads):
         t = ctx.saved_tensors
         maps, mean, rstd, w, b = (list(t[i:i + 4]) for i in range(0, 20, 4))
-        dt = maps[0].dtype
-        g = [torch.zeros_like(m, memory_format=_CL) if d is None else _layout(d, dt, m.device)
-             for d, m in zip(grads, maps)]
-        if len(grads) > 4 and grads[4] is not None:
-            if g[3] is grads[3]:  # (the caller's tensor stays as it is)
-                g[3] = g[3].clone(memory_format=_CL)
-            fpn_p6_backward(grads[4], g[3])
+        g = _output_grads(grads, maps)
         gx, gw, gb = fpn_group_norm_backward(maps, g, mean, rstd, w, b, *ctx.act,
                                              need_input_grad=any(ctx.needs_input_grad[5:9]))
         return (None,) * 5 + (*(gx or [None] * 4), *[v.to(p.dtype).view_as(p) for v, p in zip(gw, w)],
@@ -237,7 +242,6 @@ class _AdapterNeckFunction(torch.autograd.Function):
     def forward(ctx, return_p6, scale, index, c2, c3, c4, c5, *params):
         feats = [c2, c3, c4, c5]
         lw, lb, ow, ob, down, up = (list(params[i:i + 4]) for i in range(0, 24, 4))
-        dt = c2.dtype
         x = [f.contiguous(memory_format=_CL) for f in feats]
         merged, hidden = [None] * 4, [None] * 4
         for l in (3, 2, 1, 0):
@@ -248,7 +252,6 @@ class _AdapterNeckFunction(torch.autograd.Function):
         ctx.save_for_backward(index, *x, *merged, *hidden, *lw, *ow, *down, *up)
         ctx.scale = scale
         ctx.params = [(p.dtype, p.shape) for p in params]
-        ctx.dtype = dt
         return (*outs, fpn_p6(outs[3])) if return_p6 else tuple(outs)
 
     @staticmethod
@@ -258,12 +261,7 @@ class _AdapterNeckFunction(torch.autograd.Function):
         x, merged, hidden, lw, ow, down, up = (list(t[i:i + 4]) for i in range(1, 29, 4))
         need = ctx.needs_input_grad
         need_x, need_lat, need_out = need[3:7], need[7:15], need[15:23]
-        g = [torch.zeros_like(m, memory_format=_CL) if d is None else _layout(d, ctx.dtype, m.device)
-             for d, m in zip(grads, merged)]
-        if len(grads) > 4 and grads[4] is not None:
-            if g[3] is grads[3]:
-                g[3] = g[3].clone(memory_format=_CL)
-            fpn_p6_backward(grads[4], g[3])
+        g = _output_grads(grads, merged)
         gx, glw, glb, gow, gob, gd, gu = ([None] * 4 for _ in range(7))
         dm = None
         for l in range(4):  # finest first: the top-down adjoint

@@ -238,3 +238,27 @@ def test_calls_at_once_on_two_streams(cuda_device):
     for k in range(2):
         for run in got[k]:
             assert all(torch.equal(a, v) for a, v in zip(run, want[k]))
+
+
+@pytest.mark.parametrize("adapters", [True, False])
+def test_losses_of_some_outputs(cuda_device, adapters):
+    """A loss of P3 and P6 alone whose gradients are broadcast scalars (stride 0); the others' are missing."""
+    import unified_fpn as U
+    neck = _neck(U, cuda_device, norm_groups=16 if not adapters else None,
+                 activation="swish" if not adapters else None, adapters=2, adapter_rank=4)
+    feats, _ = _data(cuda_device)
+    index = torch.tensor(INDEX, device=cuda_device) if adapters else None
+    x = [f.to(cuda_device).contiguous(memory_format=CL).requires_grad_() for f in feats]
+    outs = neck(x, index)
+    (outs[1].sum() + 2.0 * outs[4].sum()).backward()
+    ref, xr, leaves = _oracle(neck, feats, INDEX if adapters else None)
+    (ref[1].sum() + 2.0 * ref[4].sum()).backward()
+    for l in range(1, 4):
+        O.check_close(x[l].grad.float().cpu(), xr[l].grad.float(), "grad16", tol=2e-2)
+    assert not x[0].grad.any()
+    for name, p in neck.named_parameters():
+        want = leaves[name].grad
+        if want is None or name.endswith(".0"):
+            assert p.grad is None or not p.grad.any(), name
+        else:
+            O.check_close(p.grad.cpu(), want.float(), "grad16", tol=2e-2)
