@@ -20,8 +20,8 @@
 // The kernel moves bytes.  The batch is cut into segments whose maps stay in the 126 MB L2 cache;
 // in one cooperative launch of a block per SM, eight warps of a block take the statistics of the
 // segments one after the other from HBM while eight others apply the norm to the segment before,
-// which they read again from L2: HBM reads and writes overlap, and the second reading costs no
-// HBM traffic.  A segment's blocks count themselves into a device counter when their sums are
+// which they read again, from L2 as far as it still holds them (all of 70 MB, half of 250 MB): HBM reads
+// and writes overlap.  A segment's blocks count themselves into a device counter when their sums are
 // written; four more warps wait for the count and merge the sums for the apply warps, while these
 // still work on the segment before.  Every warp keeps bulk copies in flight into a ring of its own
 // in shared memory and waits for no other warp (a ring shared by eight warps cost about 800 cycles
@@ -43,7 +43,7 @@ constexpr int kGnThreads = 32 * kGnWarps;
 constexpr int kGnMergeThreads = 128;
 constexpr int kGnMergeRows = 1920;     // sums of an image that a merge has in shared memory at once
 constexpr int kGnMaxRuns = 8;         // runs (images of one level) per segment
-constexpr int kGnMaxChannels = 2048;  // 8 per thread of a half
+constexpr int kGnMaxChannels = 2048;  // 8 per statistics thread
 constexpr int kGnStage = 4096;         // one copy of a warp; backward: half of it x, half dy
 constexpr int kGnK = 8;                // pixels read before their arithmetic
 constexpr int kGnStatsStages = 3, kGnApplyStages = 2;  // per warp
@@ -611,8 +611,8 @@ __device__ __forceinline__ void gn_stats_reduce(const GnArgs& a, const GnPlace& 
 }
 
 // The merge's rows [r0, r0 + n) of groups [g0, g0 + span) into shared memory.  (One asynchronous copy after
-// the other from a short loop: the same loads unrolled into registers took 13000 cycles at a launch's
-// first merge, most of them instruction fetches.)
+// the other from a short loop, all in flight at once; under the streaming of the other warps a copy takes
+// 2000 to 13000 cycles.)
 __device__ __forceinline__ void gn_merge_fetch(const GnArgs& a, const float2* rows, int g0, int span, int r0, int n,
                                                GnSmem& s, int t) {
   const float2* src = rows + static_cast<size_t>(r0) * a.groups + g0;
@@ -989,8 +989,8 @@ __device__ __forceinline__ bool gn_wait_segment(const GnArgs& a, GnSmem& s, int 
   return true;
 }
 // Whether the statistics of segment k may be read already: at most four segments ahead of the apply
-// warps, so that these find theirs in L2 (two ahead left them waiting: 134 us instead of 119 us for 8 x
-// 200 x 304 x 256 bf16).
+// warps, so that these find theirs in L2 (two ahead left them waiting: 129 us instead of 125 us for 8 x
+// 200 x 304 x 256 bf16 with swish).
 __device__ __forceinline__ bool gn_may_read(const GnArgs& a, GnSmem& s, int k) {
   return !a.apply || *static_cast<volatile int*>(&s.applied) >= k - 3;
 }
@@ -1452,8 +1452,8 @@ GnSchedule gn_schedule(DType dt, int levels, int N, int C, const long long* pixe
 }
 
 // Segment size: bytes of x (the backward's come with dy).  A segment is read again from L2 while the
-// next ones stream in, so a few of them have to fit its 126 MB; half the size costs more waits than it
-// saves (R50 pyramid 47 -> 50 us).
+// next ones stream in, so a few of them ought to fit its 126 MB; half the size reads less from HBM, but
+// waits more often (the training pyramid 148 -> 152 us, the others within 1 %), twice the size costs 7 %.
 constexpr long long kGnForwardBudget = 64LL << 20;
 constexpr long long kGnBackwardBudget = 32LL << 20;
 
