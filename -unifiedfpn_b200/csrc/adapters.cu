@@ -14,10 +14,17 @@
 // back into shared memory as the A operand of a last MMA against up[a], on the accumulator that
 // already holds x W^T.  So an adapter costs R / 256 more tensor work and no further pass.
 //
-// h is kept in 16-bit parts, hi = round(h), the next = round(h - hi) and so on: three of bf16 or two
-// of fp16 carry 22 bits and more.  One rounding to bf16 would be the largest error of the fp32 weight
-// gradients, and of an adapter's share of out; the further parts cost one k-step of the last MMA each,
-// and columns of the gradients' GEMM.  The tensor cores' fp32 accumulation rounds every step
+// h is kept in 16-bit parts, hi = round(h), the next = round(h - hi) and so on: three of bf16 carry 22
+// bits and more, two of fp16 as many down to |h| = 2^-3 and whatever lies above 2^-25 below that (there
+// the second part is subnormal).  For out and dx that is enough: fp16 results have steps of 2^-24
+// themselves.  The weight gradients are fp32, and dh is as small as up and dy make it, so their GEMM, which
+// can weigh each part's columns when it adds them, takes other parts of fp16: dh / 2, then
+// what is left times 2^10 and times 2^22 (all bits down to 2^-47), and for h the bits that the second part
+// lost times 2^11 (down to 2^-36) as a third part.  (With two plain parts ddown was 1e-3 off at dy and up
+// of 1e-3, 0.37 at 3e-5 and 1e-4.)
+// One rounding to bf16 would be the largest error of the fp32 weight gradients, and of an adapter's share
+// of out; the further parts cost one k-step of the last MMA each, and columns of the gradients'
+// GEMM.  The tensor cores' fp32 accumulation rounds every step
 // downwards, an error that grows with the number of steps: the products behind h are split over up to
 // four accumulators (32 steps each at K = 2048: dup 3.1e-6 -> 0.8e-6 off at fp16).
 #include "kernels.h"
@@ -25,6 +32,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 #include <cstring>
 
 namespace ufpn {
@@ -44,7 +52,8 @@ constexpr int kAdWarpCols = kTcBlockN / (kAdEpiWarps / 4);  // output channels o
 constexpr int kDevTimeoutAdapter = 0x107;
 
 template <typename T>
-constexpr int kAdParts = TcElem<T>::kFmt == 1 ? 3 : 2;  // of h: bf16, fp16
+constexpr int kAdParts = TcElem<T>::kFmt == 1 ? 3 : 2;  // of h in the last MMA: bf16, fp16
+constexpr int kAdStored = 3;                            // of h and dh as stored for the gradients, at most
 
 // K-major operand rows of RB = 32, 64 or 128 bytes under the swizzle of that width (16-byte chunk c of
 // row r at c ^ (r * RB / 128 % (RB / 16))), 8-row atoms of 8 RB bytes.
@@ -97,6 +106,7 @@ struct AdArgs {
   int v_rows;    // output channels
   int v_vec;     // vr == 1 and every row is whole 16-byte vectors
   void* hidden;  // [pixels][parts][rank_pad], or null
+  int store;     // its parts (kAdPlain and so on)
   int rank_pad;  // rank rounded up to 8
   int want_out;  // 0: only hidden
   int h_accs;    // accumulators that h's k-blocks alternate over
@@ -115,14 +125,79 @@ __device__ __forceinline__ int ad_adapter(const AdArgs& a, int n) {
 // v ~ the sum of its parts.  (A value beyond the type's range keeps the rest in the next part; infinity, and
 // what exceeds the parts' ranges together, ends in the last one.)
 template <typename T>
-__device__ __forceinline__ void ad_split(float v, uint16_t (&part)[kAdParts<T>]) {
+__device__ __forceinline__ float ad_clamp(float v) {
   constexpr float kMax = TcElem<T>::kFmt == 0 ? 65504.f : 3.3895313892515355e38f;
+  return v > kMax ? kMax : (v < -kMax ? -kMax : v);
+}
+template <typename T>
+__device__ __forceinline__ void ad_split(float v, uint16_t (&part)[kAdParts<T>]) {
 #pragma unroll
   for (int i = 0; i < kAdParts<T>; ++i) {
     float c = v;
-    if (i + 1 < kAdParts<T>) c = v > kMax ? kMax : (v < -kMax ? -kMax : v);
+    if (i + 1 < kAdParts<T>) c = ad_clamp<T>(v);
     part[i] = Pack<T>::bits(c);
     v -= Pack<T>::unpack(static_cast<uint32_t>(part[i])).x;
+  }
+}
+
+// What `hidden` holds.  fp16: two plain parts; h in three, the third for the bits below the second's steps
+// (0 where that is normal, so that h stays the sum of the parts elsewhere); or dh in three.
+enum : int { kAdPlain = 0, kAdFineH = 1, kAdFineDh = 2 };
+template <typename T>
+__host__ __device__ constexpr int ad_stored(int store) {
+  return kAdParts<T> == kAdStored || store != kAdPlain ? kAdStored : 2;
+}
+// What a part of the fp16 forms is multiplied by.  dh is halved: values up to 131 008, as two plain parts
+// take them.
+__host__ __device__ constexpr float ad_factor(int store, int part) {
+  if (store == kAdFineDh) return part == 0 ? 0x1p-1f : part == 1 ? 0x1p10f : 0x1p22f;
+  return store == kAdFineH && part == 2 ? 0x1p11f : 1.f;
+}
+__host__ __device__ constexpr float ad_weight(int store, int part) { return 1.f / ad_factor(store, part); }
+
+// Part i of v in `hidden`, taken off v.  (fp16: infinity and what exceeds the first two parts' ranges end
+// in the second.)
+template <typename T>
+__device__ __forceinline__ uint32_t ad_take(float& v, int store, int i) {
+  float c = v;
+  if constexpr (kAdParts<T> == kAdStored) {
+    if (i + 1 < kAdStored) c = ad_clamp<T>(v);
+  } else {
+    c = v * ad_factor(store, i);
+    if (i == 0) {
+      c = ad_clamp<T>(c);
+      // (No subnormal first part of dh: the tensor cores align a step's products to the largest exponent
+      // and count a subnormal's as 2^-14, which cost ddown 3e-6 at dh = 1.5e-7 where the second part alone
+      // carries it to 5e-7.)
+      if (store == kAdFineDh && fabsf(c) < 0x1p-14f) c = 0.f;
+    }
+  }
+  const uint32_t bits = Pack<T>::bits(c);
+  const float taken = Pack<T>::unpack(bits).x;
+  if constexpr (kAdParts<T> == kAdStored) {
+    v -= taken;
+  } else {
+    v = fmaf(-taken, ad_weight(store, i), v);  // (exact)
+    if (i == 1 && !(fabsf(taken) < (store == kAdFineDh ? HUGE_VALF : 0x1p-14f))) v = 0.f;
+  }
+  return bits;
+}
+
+// The parts of eight values.  (A call: inlined, its registers were spilled in calls without `hidden` too, which
+// cost these up to 5 %.)
+template <typename T>
+__device__ __noinline__ void ad_take8(uint4* dst, int stride, int store, float v0, float v1, float v2, float v3, float v4,
+                                      float v5, float v6, float v7) {
+  float v[8] = {v0, v1, v2, v3, v4, v5, v6, v7};
+#pragma unroll
+  for (int part = 0; part < kAdStored; ++part) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      w[i] = ad_take<T>(v[2 * i], store, part);
+      w[i] |= ad_take<T>(v[2 * i + 1], store, part) << 16;
+    }
+    if (part < ad_stored<T>(store)) dst[part * stride] = make_uint4(w[0], w[1], w[2], w[3]);
   }
 }
 
@@ -385,11 +460,11 @@ __global__ void __launch_bounds__(kAdThreads, 1)
         fence_proxy_async_smem();
         mbar_arrive(wfull_bar);
       }
-      uint4* hid = nullptr;  // this thread's pixel of `hidden`: kParts * rank_pad elements
+      uint4* hid = nullptr;  // this thread's pixel of `hidden`
       if (ad.hidden != nullptr && slice == 0 && valid)
         hid = reinterpret_cast<uint4*>(
             static_cast<uint8_t*>(ad.hidden) +
-            ((static_cast<size_t>(n) * args.H + py) * args.W + px) * ad.rank_pad * (2 * kParts));
+            ((static_cast<size_t>(n) * args.H + py) * args.W + px) * ad.rank_pad * (2 * ad_stored<T>(ad.store)));
       if (has) {
         if (ad.want_out && cq >= 2 && (adapter != v_adapter || slice != v_slice)) {
           // up[a] (this slice's 256 rows): one row a thread of the upper two quarters
@@ -441,23 +516,29 @@ __global__ void __launch_bounds__(kAdThreads, 1)
 #pragma unroll
             for (int i = 0; i < 8; ++i) h[i] += __uint_as_float(r[i]);
           }
-          uint32_t w[kParts][4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            uint16_t p0[kParts], p1[kParts];
-            const int c = j * 8 + 2 * i;
-            ad_split<T>(c < ad.rank ? s * h[2 * i] : 0.f, p0);
-            ad_split<T>(c + 1 < ad.rank ? s * h[2 * i + 1] : 0.f, p1);
+          for (int i = 0; i < 8; ++i) h[i] = j * 8 + i < ad.rank ? s * h[i] : 0.f;
+          if (kParts == kAdStored || ad.want_out) {
+            uint32_t w[kParts][4];
 #pragma unroll
-            for (int part = 0; part < kParts; ++part)
-              w[part][i] = p0[part] | (static_cast<uint32_t>(p1[part]) << 16);
+            for (int i = 0; i < 4; ++i) {
+              uint16_t p0[kParts], p1[kParts];
+              ad_split<T>(h[2 * i], p0);
+              ad_split<T>(h[2 * i + 1], p1);
+#pragma unroll
+              for (int part = 0; part < kParts; ++part)
+                w[part][i] = p0[part] | (static_cast<uint32_t>(p1[part]) << 16);
+            }
+#pragma unroll
+            for (int part = 0; part < kParts; ++part) {
+              const uint4 q = make_uint4(w[part][0], w[part][1], w[part][2], w[part][3]);
+              if (ad.want_out) st_shared_v4(t_addr + part * Cfg::kPart + row_chunk<Cfg::kRow>(row, j), q);
+              if (kParts == kAdStored && hid != nullptr && j * 8 < ad.rank_pad)
+                hid[(part * ad.rank_pad >> 3) + j] = q;
+            }
           }
-#pragma unroll
-          for (int part = 0; part < kParts; ++part) {
-            const uint4 q = make_uint4(w[part][0], w[part][1], w[part][2], w[part][3]);
-            if (ad.want_out) st_shared_v4(t_addr + part * Cfg::kPart + row_chunk<Cfg::kRow>(row, j), q);
-            if (hid != nullptr && j * 8 < ad.rank_pad) hid[(part * ad.rank_pad >> 3) + j] = q;
-          }
+          if (kParts != kAdStored && hid != nullptr && j * 8 < ad.rank_pad)
+            ad_take8<T>(hid + j, ad.rank_pad >> 3, ad.store, h[0], h[1], h[2], h[3], h[4], h[5], h[6], h[7]);
         }
         fence_proxy_async_smem();
         tc_fence_before();
@@ -465,7 +546,7 @@ __global__ void __launch_bounds__(kAdThreads, 1)
         h_phase ^= 1u;
         if (!ad.want_out) mbar_arrive(acce_bar);
       } else if (hid != nullptr && cq == 0) {
-        for (int j = 0; j < ad.rank_pad * kParts / 8; ++j) hid[j] = make_uint4(0u, 0u, 0u, 0u);
+        for (int j = 0; j < ad.rank_pad * ad_stored<T>(ad.store) / 8; ++j) hid[j] = make_uint4(0u, 0u, 0u, 0u);
       }
       if (!ad.want_out) continue;
 
@@ -951,17 +1032,17 @@ __global__ void __launch_bounds__(kAdThreads, 1)
             h.w += q.w;
           }
         }
-        uint16_t a[kParts], b[kParts], e[kParts], f[kParts];
-        ad_split<T>(h.x, a);
-        ad_split<T>(h.y, b);
-        ad_split<T>(h.z, e);
-        ad_split<T>(h.w, f);
         uint16_t* hid = static_cast<uint16_t*>(ad.hidden) +
-                        (static_cast<size_t>(n) * pixels + p) * ad.rank_pad * kParts + c;
+                        (static_cast<size_t>(n) * pixels + p) * ad.rank_pad * ad_stored<T>(ad.store) + c;
 #pragma unroll
-        for (int k = 0; k < kParts; ++k)
-          *reinterpret_cast<uint2*>(hid + k * ad.rank_pad) =
-              make_uint2(a[k] | (static_cast<uint32_t>(b[k]) << 16), e[k] | (static_cast<uint32_t>(f[k]) << 16));
+        for (int k = 0; k < kAdStored; ++k) {
+          uint2 q;
+          q.x = ad_take<T>(h.x, ad.store, k);
+          q.x |= ad_take<T>(h.y, ad.store, k) << 16;
+          q.y = ad_take<T>(h.z, ad.store, k);
+          q.y |= ad_take<T>(h.w, ad.store, k) << 16;
+          if (k < ad_stored<T>(ad.store)) *reinterpret_cast<uint2*>(hid + k * ad.rank_pad) = q;
+        }
       }
     }
     __syncwarp();
@@ -988,7 +1069,7 @@ __global__ void __launch_bounds__(kAdThreads, 1)
 // part[unit][r][c] = sum over the unit's pixels of h[p][r] q[p][c]: for the channel blocks of x with
 // h = dh (ddown), and for dy with h (dup).  A tcgen05 GEMM over pixels (both operands MN-major
 // 64-pixel boxes): M = 256 channels in two accumulators, N = parts x rank_pad columns, the parts of
-// h side by side, added when the accumulators are read.  Where TMEM has room (N <= 128), the k-blocks
+// h side by side, weighed and added when the accumulators are read.  Where TMEM has room (N <= 128), the k-blocks
 // alternate over two pairs of accumulators: at most 64 steps on one (see the rounding above).
 constexpr int kAgChunk = 64 * 128;
 constexpr int kAgStages = 4;
@@ -1005,6 +1086,7 @@ struct AgArgs {
   int splits, per, num_kb;  // 64-pixel k-blocks of an image: num_kb, `per` of them a split
   int blocks, x_blocks;     // 256-channel blocks: x_blocks of x, then one of dy
   int rank_pad;
+  int store;  // of h (dh: kAdFineDh)
   float* part;  // [image - n0][split][block][rank_pad][256]
   int* status;
 };
@@ -1043,8 +1125,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   const CUtensorMap* mh = is_x ? &map_dh : &map_h;
   const int c0 = is_x ? block * 256 : 0;
   const int kb0 = split * a.per, kb1 = min(a.num_kb, kb0 + a.per);  // non-empty (host)
-  constexpr int kParts = kAdParts<T>;
-  const int cols = (kParts * a.rank_pad + 15) / 16 * 16;  // (columns past the parts are zeros)
+  constexpr bool kPlain = kAdParts<T> == kAdStored;  // all parts count once
+  const int store = is_x ? kAdFineDh : a.store;
+  const int parts = ad_stored<T>(store);
+  const int cols = (parts * a.rank_pad + 15) / 16 * 16;  // (columns past the parts are zeros)
   const int hchunks = (cols + 63) / 64;
   const int sets = cols <= 128 ? 2 : 1;  // accumulators at columns 256 * half + 128 * set
 
@@ -1144,15 +1228,18 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       for (int r = 0; r < a.rank_pad; r += 8) {
         float sum[8] = {};
 #pragma unroll
-        for (int part = kParts - 1; part >= 0; --part)  // the smallest first
+        for (int part = kAdStored - 1; part >= 0; --part) {  // the smallest first
+          if (part >= parts) continue;
+          const float weight = kPlain ? 1.f : ad_weight(store, part);
           for (int set = 0; set < used; ++set) {
             uint32_t v[8];
             __syncwarp();
             tmem_ld8(acc + 128 * set + part * a.rank_pad + r, v);
             tmem_wait_ld();
 #pragma unroll
-            for (int i = 0; i < 8; ++i) sum[i] += __uint_as_float(v[i]);
+            for (int i = 0; i < 8; ++i) sum[i] = fmaf(weight, __uint_as_float(v[i]), sum[i]);
           }
+        }
 #pragma unroll
         for (int i = 0; i < 8; ++i) dst[(r + i) * 256] = sum[i];
       }
@@ -1288,7 +1375,10 @@ cudaError_t launch_adapter_t(const TcPlan& p, const CUtensorMap& map_u, const Ad
 }
 
 int pad8(int v) { return (v + 7) / 8 * 8; }
-int parts_of(DType dt) { return dt == DType::BF16 ? kAdParts<__nv_bfloat16> : kAdParts<__half>; }
+int store_h(const AdapterProblem& p) { return p.hidden_parts == kAdStored ? kAdFineH : kAdPlain; }
+int stored(DType dt, int store) {
+  return dt == DType::BF16 ? ad_stored<__nv_bfloat16>(store) : ad_stored<__half>(store);
+}
 int rank_tile(int rank) { return rank <= 16 ? 16 : rank <= 32 ? 32 : 64; }
 size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 
@@ -1363,6 +1453,7 @@ bool adapter_sizes_ok(const AdapterProblem& p) {
   return (p.dtype == DType::BF16 || p.dtype == DType::F16) && p.N > 0 && p.H > 0 && p.W > 0 &&
          p.Cin > 0 && p.Cin % 8 == 0 && p.Cin <= 2048 && p.rank > 0 && p.rank <= kAdMaxRank &&
          p.adapters > 0 && p.adapters <= 65535 &&
+         (p.hidden_parts == kAdStored || (p.hidden_parts == 2 && p.dtype == DType::F16)) &&
          static_cast<long long>(p.H) * p.W < ((1LL << 31) - 256) / p.N;
 }
 
@@ -1401,7 +1492,7 @@ AgPlan adapter_grad_plan(const AdapterProblem& p) {
   const long long units = static_cast<long long>(p.N) * g.blocks;
   int k = static_cast<int>(std::max<long long>(1, sm_count() / units));
   k = std::min(k, std::max(1, g.num_kb / 4));
-  const int most = (parts_of(p.dtype) * pad8(p.rank) + 15) / 16 * 16 <= 128 ? 32 : 16;  // k-blocks
+  const int most = (kAdStored * pad8(p.rank) + 15) / 16 * 16 <= 128 ? 32 : 16;  // k-blocks
   g.per = std::min(most, (g.num_kb + k - 1) / k);
   g.splits = (g.num_kb + g.per - 1) / g.per;
   g.image_bytes = static_cast<size_t>(g.splits) * g.blocks * pad8(p.rank) * 256 * sizeof(float);
@@ -1417,7 +1508,7 @@ AdWorkspace adapter_workspace(const AdapterProblem& p, bool own_w_t) {
   w.up_t = 0;
   w.w_t = w.up_t + align256(static_cast<size_t>(p.adapters) * p.rank * 256 * 2);
   w.dh = w.w_t + (own_w_t ? static_cast<size_t>((p.Cin + 255) / 256) * 256 * 256 * 2 : 0);
-  w.part = w.dh + align256(static_cast<size_t>(p.N) * p.H * p.W * parts_of(p.dtype) * pad8(p.rank) * 2);
+  w.part = w.dh + align256(static_cast<size_t>(p.N) * p.H * p.W * kAdStored * pad8(p.rank) * 2);
   const AgPlan g = adapter_grad_plan(p);
   w.total = w.part + g.images * g.image_bytes;
   return w;
@@ -1428,11 +1519,12 @@ cudaError_t adapter_grads_t(const AdapterProblem& p, const void* x, const void* 
                             const void* h, float* part, float* ddown, float* dup, int* status,
                             cudaStream_t s) {
   const AgPlan g = adapter_grad_plan(p);
-  const int hw = p.H * p.W, hc = parts_of(p.dtype) * pad8(p.rank);
+  const int hw = p.H * p.W;
+  const int dhc = kAdStored * pad8(p.rank), hc = stored(p.dtype, store_h(p)) * pad8(p.rank);
   CUtensorMap mx, my, mdh, mh;
   cudaError_t e = encode_nhwc_map(&mx, p.dtype, x, p.N, 1, hw, p.Cin, p.Cin, 64, 1);
   if (e == cudaSuccess) e = encode_nhwc_map(&my, p.dtype, dy, p.N, 1, hw, 256, 256, 64, 1);
-  if (e == cudaSuccess) e = encode_nhwc_map(&mdh, p.dtype, dh, p.N, 1, hw, hc, hc, 64, 1);
+  if (e == cudaSuccess) e = encode_nhwc_map(&mdh, p.dtype, dh, p.N, 1, hw, dhc, dhc, 64, 1);
   if (e == cudaSuccess) e = encode_nhwc_map(&mh, p.dtype, h, p.N, 1, hw, hc, hc, 64, 1);
   if (e != cudaSuccess) return e;
   auto kern = fpn_adapter_grad_kernel<T>;
@@ -1455,6 +1547,7 @@ cudaError_t adapter_grads_t(const AdapterProblem& p, const void* x, const void* 
     a.blocks = g.blocks;
     a.x_blocks = g.x_blocks;
     a.rank_pad = pad8(p.rank);
+    a.store = store_h(p);
     a.part = part;
     a.status = status;
     e = launch_ex(kern, dim3(static_cast<unsigned>(images) * g.splits * g.blocks), dim3(kTcThreads),
@@ -1506,6 +1599,7 @@ cudaError_t launch_lateral_adapters(const AdapterProblem& p, const void* x, cons
   ad.v_rows = 256;
   ad.v_vec = p.rank % 8 == 0 && aligned16(up);
   ad.hidden = hidden;
+  ad.store = store_h(p);
   ad.rank_pad = pad8(p.rank);
   ad.want_out = 1;
   ad.h_accs = ad_h_accs((p.Cin + 63) / 64);
@@ -1587,6 +1681,7 @@ cudaError_t launch_lateral_adapters_backward(const AdapterProblem& p, const void
   ad.vr = p.Cin;
   ad.v_rows = p.Cin;
   ad.hidden = dh;
+  ad.store = kAdFineDh;
   ad.rank_pad = pad8(p.rank);
   ad.want_out = dx != nullptr;
   ad.h_accs = ad_h_accs(4);

@@ -939,7 +939,7 @@ int conv3x3_backward(int dtype, const void* x, const void* w, const void* w_f,
 namespace {
 // The checks of the adapter calls on sizes; fills `p`.
 int adapter_problem(int dtype, int N, int Cin, int H, int W, int rank, int adapters, const int* index,
-                    const float* scales, float scale, ufpn::AdapterProblem* p) {
+                    const float* scales, float scale, int hidden_parts, ufpn::AdapterProblem* p) {
   if (!parse_16bit(dtype, &p->dtype)) return fail(UFPN_ERR_UNSUPPORTED, "adapters take bf16 or fp16");
   if (N <= 0 || Cin <= 0 || H <= 0 || W <= 0 || adapters <= 0)
     return fail(UFPN_ERR_INVALID_ARG, "sizes must be positive");
@@ -949,6 +949,8 @@ int adapter_problem(int dtype, int N, int Cin, int H, int W, int rank, int adapt
   if (adapters > 65535) return fail(UFPN_ERR_UNSUPPORTED, "at most 65535 adapters");
   if (static_cast<long long>(H) * W >= ((1LL << 31) - 256) / N)
     return fail(UFPN_ERR_UNSUPPORTED, "map too large");
+  if (hidden_parts != 3 && !(hidden_parts == 2 && p->dtype == DType::F16))
+    return fail(UFPN_ERR_INVALID_ARG, "hidden has 3 parts, or 2 of fp16");
   p->N = N;
   p->Cin = Cin;
   p->H = H;
@@ -958,17 +960,29 @@ int adapter_problem(int dtype, int N, int Cin, int H, int W, int rank, int adapt
   p->index = index;
   p->scales = scales;
   p->scale = scale;
+  p->hidden_parts = hidden_parts;
   return UFPN_OK;
 }
+// hidden of the entries without `hidden_parts`
+int plain_hidden_parts(int dtype) { return dtype == UFPN_DTYPE_F16 ? 2 : 3; }
 }  // namespace
 
 int ufpn_lateral_adapters(int dtype, const void* x, const void* w, const float* bias,
                           const void* down, const void* up, const int* index, const float* scales,
                           float scale, const void* coarse, void* out, void* hidden, int N, int Cin,
                           int H, int W, int rank, int adapters, int Hc, int Wc, void* stream) {
+  return ufpn_lateral_adapters_parts(dtype, x, w, bias, down, up, index, scales, scale, coarse, out, hidden,
+                                     plain_hidden_parts(dtype), N, Cin, H, W, rank, adapters, Hc, Wc, stream);
+}
+
+int ufpn_lateral_adapters_parts(int dtype, const void* x, const void* w, const float* bias,
+                                const void* down, const void* up, const int* index,
+                                const float* scales, float scale, const void* coarse, void* out,
+                                void* hidden, int hidden_parts, int N, int Cin, int H, int W, int rank,
+                                int adapters, int Hc, int Wc, void* stream) {
   return guarded([&] {
     ufpn::AdapterProblem p;
-    const int rc = adapter_problem(dtype, N, Cin, H, W, rank, adapters, index, scales, scale, &p);
+    const int rc = adapter_problem(dtype, N, Cin, H, W, rank, adapters, index, scales, scale, hidden_parts, &p);
     if (rc != UFPN_OK) return rc;
     if (!x || !w || !bias || !down || !up || !index || !out)
       return fail(UFPN_ERR_INVALID_ARG, "NULL tensor pointer");
@@ -988,7 +1002,7 @@ int ufpn_lateral_adapters(int dtype, const void* x, const void* w, const float* 
 size_t ufpn_lateral_adapters_workspace(int dtype, int N, int Cin, int H, int W, int rank,
                                        int adapters, int has_w_t, int need_grad_x) {
   ufpn::AdapterProblem p;
-  if (adapter_problem(dtype, N, Cin, H, W, rank, adapters, nullptr, nullptr, 1.f, &p) != UFPN_OK) return 0;
+  if (adapter_problem(dtype, N, Cin, H, W, rank, adapters, nullptr, nullptr, 1.f, 3, &p) != UFPN_OK) return 0;
   return ufpn::lateral_adapters_workspace_bytes(p, has_w_t != 0, need_grad_x != 0);
 }
 
@@ -999,9 +1013,21 @@ int ufpn_lateral_adapters_backward(int dtype, const void* x, const void* w, cons
                                    float* grad_up, int N, int Cin, int H, int W, int rank,
                                    int adapters, void* workspace, size_t workspace_bytes,
                                    void* stream) {
+  return ufpn_lateral_adapters_backward_parts(dtype, x, w, w_t, grad_out, down, up, index, scales, scale, hidden,
+                                              plain_hidden_parts(dtype), grad_x, grad_down, grad_up, N, Cin, H, W,
+                                              rank, adapters, workspace, workspace_bytes, stream);
+}
+
+int ufpn_lateral_adapters_backward_parts(int dtype, const void* x, const void* w, const void* w_t,
+                                         const void* grad_out, const void* down, const void* up,
+                                         const int* index, const float* scales, float scale,
+                                         const void* hidden, int hidden_parts, void* grad_x,
+                                         float* grad_down, float* grad_up, int N, int Cin, int H, int W,
+                                         int rank, int adapters, void* workspace,
+                                         size_t workspace_bytes, void* stream) {
   return guarded([&] {
     ufpn::AdapterProblem p;
-    const int rc = adapter_problem(dtype, N, Cin, H, W, rank, adapters, index, scales, scale, &p);
+    const int rc = adapter_problem(dtype, N, Cin, H, W, rank, adapters, index, scales, scale, hidden_parts, &p);
     if (rc != UFPN_OK) return rc;
     if (!x || !grad_out || !down || !up || !index || !hidden || !grad_down || !grad_up ||
         (grad_x && !w && !w_t))

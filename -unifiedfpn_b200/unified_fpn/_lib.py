@@ -104,6 +104,11 @@ SIGNATURES = {
     "ufpn_group_norm_workspace": (c_size_t, [c_int, c_int, c_int, c_int, c_void_p, c_int, c_int]),
     "ufpn_lateral_adapters": (
         c_int, [c_int] + [c_void_p] * 7 + [c_float] + [c_void_p] * 3 + [c_int] * 8 + [c_void_p]),
+    "ufpn_lateral_adapters_parts": (
+        c_int, [c_int] + [c_void_p] * 7 + [c_float] + [c_void_p] * 3 + [c_int] * 9 + [c_void_p]),
+    "ufpn_lateral_adapters_backward_parts": (
+        c_int, [c_int] + [c_void_p] * 8 + [c_float, c_void_p, c_int] + [c_void_p] * 3 + [c_int] * 6 + [
+            c_void_p, c_size_t, c_void_p]),
     "ufpn_lateral_adapters_backward": (
         c_int, [c_int] + [c_void_p] * 8 + [c_float] + [c_void_p] * 4 + [c_int] * 6 + [c_void_p, c_size_t,
                                                                                       c_void_p]),

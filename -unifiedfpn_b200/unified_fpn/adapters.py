@@ -19,7 +19,7 @@ from .ops import _DT
 
 _CL = torch.channels_last
 MAX_RANK = 64
-_PARTS = {torch.bfloat16: 3, torch.float16: 2}  # 16-bit values that make up one of h
+_PARTS = 3  # 16-bit values that make up one of h
 
 
 def _cl(t: torch.Tensor) -> torch.Tensor:
@@ -91,8 +91,10 @@ def fpn_lateral_adapters(input: torch.Tensor, weight: torch.Tensor, bias: torch.
     ``index``: one integer per image on the device, values outside 0 .. L - 1 (-1 by convention) run
     without an adapter; ``scale``: a number, or [L] on the device.  ``weight`` [256, Cin] or [256,
     Cin, 1, 1], ``bias`` [256], Cin a multiple of 8, at most 2048.  Sums are fp32 and rounded once;
-    h is carried in 16-bit parts, 3 of bf16 or 2 of fp16.  With ``return_hidden`` also returns h in that
-    form (opaque, [N, H, W, parts, R rounded up to 8]) for :func:`fpn_lateral_adapters_backward`."""
+    h is carried in 16-bit parts of 22 bits and more together, of which fp16 loses what is below 2^-25 (up
+    to 2^-25 * sum_r |up| in the output, whose own steps end at 2^-24).  With ``return_hidden`` also returns
+    h in parts (opaque, [N, H, W, 3, R rounded up to 8]; fp16: what is below 2^-36 is lost) for
+    :func:`fpn_lateral_adapters_backward`."""
     down, up, index, scales, scale = _check(input, down, up, index, scale)
     x = _cl(input)
     n, cin, h, w = x.shape
@@ -111,14 +113,14 @@ def fpn_lateral_adapters(input: torch.Tensor, weight: torch.Tensor, bias: torch.
     count, rank = down.shape[:2]
     # (channels_last; torch.empty with the memory format takes a microsecond more)
     out = torch.empty_strided((n, 256, h, w), (h * w * 256, 1, w * 256, 256), dtype=x.dtype, device=dev)
-    hidden = torch.empty((n, h, w, _PARTS[x.dtype], (rank + 7) // 8 * 8), dtype=x.dtype,
+    hidden = torch.empty((n, h, w, _PARTS, (rank + 7) // 8 * 8), dtype=x.dtype,
                          device=dev) if return_hidden else None
 
     check(_on_device(
-        dev, lib.ufpn_lateral_adapters, _DT[x.dtype], x.data_ptr(), wt.data_ptr(), b.data_ptr(), down.data_ptr(),
+        dev, lib.ufpn_lateral_adapters_parts, _DT[x.dtype], x.data_ptr(), wt.data_ptr(), b.data_ptr(), down.data_ptr(),
         up.data_ptr(), index.data_ptr(), None if scales is None else scales.data_ptr(), scale,
         None if coarse is None else coarse.data_ptr(), out.data_ptr(), None if hidden is None else hidden.data_ptr(),
-        n, cin, h, w, rank, count, hc, wc, _stream(dev)), "ufpn_lateral_adapters")
+        _PARTS, n, cin, h, w, rank, count, hc, wc, _stream(dev)), "ufpn_lateral_adapters")
     return (out, hidden) if return_hidden else out
 
 
@@ -132,7 +134,9 @@ def fpn_lateral_adapters_backward(input: torch.Tensor, weight: torch.Tensor | No
     ``weight_t``: the weights transposed for the input gradient, as
     :func:`fpn_lateral_conv_backward` takes them (``weight`` is then not read).  The shared weight's
     and bias's gradients are :func:`fpn_lateral_conv_backward`'s, the coarse map's
-    :func:`fpn_upsample_add_backward`'s.  Deterministic (every sum in a fixed order)."""
+    :func:`fpn_upsample_add_backward`'s.  Deterministic (every sum in a fixed order).  fp16: dh = scale *
+    grad_output up[a] enters grad_down to 22 bits and more, of which what is below 2^-47 is lost, and
+    grad_input (steps of 2^-24) without what is below 2^-25 of it."""
     down, up, index, scales, scale = _check(input, down, up, index, scale)
     x = _cl(input)
     n, cin, h, w = x.shape
@@ -141,7 +145,7 @@ def fpn_lateral_adapters_backward(input: torch.Tensor, weight: torch.Tensor | No
         raise ValueError("grad_output must be [N, 256, H, W] in the input's dtype")
     g = _cl(grad_output)
     count, rank = down.shape[:2]
-    if hidden.dtype is not x.dtype or tuple(hidden.shape) != (n, h, w, _PARTS[x.dtype], (rank + 7) // 8 * 8) \
+    if hidden.dtype is not x.dtype or tuple(hidden.shape) != (n, h, w, _PARTS, (rank + 7) // 8 * 8) \
             or hidden.device != dev or not hidden.is_contiguous():
         raise ValueError("hidden must be what the forward returned")
     wt = wtt = None
@@ -164,9 +168,10 @@ def fpn_lateral_adapters_backward(input: torch.Tensor, weight: torch.Tensor | No
                       need_input_grad)
     work = torch.empty(need, device=dev, dtype=torch.uint8)
     check(_on_device(
-        dev, lib.ufpn_lateral_adapters_backward, code, x.data_ptr(), None if wt is None else wt.data_ptr(),
+        dev, lib.ufpn_lateral_adapters_backward_parts, code, x.data_ptr(), None if wt is None else wt.data_ptr(),
         None if wtt is None else wtt.data_ptr(), g.data_ptr(), down.data_ptr(), up.data_ptr(), index.data_ptr(),
-        None if scales is None else scales.data_ptr(), scale, hidden.data_ptr(), None if gx is None else gx.data_ptr(),
+        None if scales is None else scales.data_ptr(), scale, hidden.data_ptr(), _PARTS,
+        None if gx is None else gx.data_ptr(),
         gdown.data_ptr(), gup.data_ptr(), n, cin, h, w, rank, count, work.data_ptr(), need, _stream(dev)),
         "ufpn_lateral_adapters_backward")
     return gx, gdown, gup

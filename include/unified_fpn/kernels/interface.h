@@ -433,9 +433,11 @@ struct AdapterProblem {
   const int* index;     // [N] device: the image's adapter, outside 0 .. adapters - 1: none
   const float* scales;  // [adapters] device, or null (1)
   float scale;          // times scales[a]
+  int hidden_parts;     // 3; fp16 also 2
 };
 // out = x w^T + bias + h up[a]^T [+ bilinear(coarse)], h = scale x down[a]^T; hidden (optional):
-// [pixels][parts][rank padded to 8], h as the sum of 3 (bf16) or 2 (fp16) parts.
+// [pixels][hidden_parts][rank padded to 8], h in parts: their sum, but for a third part of fp16, which
+// counts 2^-11 times.
 cudaError_t launch_lateral_adapters(const AdapterProblem& p, const void* x, const void* w,
                                     const float* bias, const void* down, const void* up,
                                     const void* coarse, int Hc, int Wc, void* out, void* hidden,

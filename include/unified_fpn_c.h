@@ -286,11 +286,21 @@ int ufpn_conv3x3_act(int dtype, const void* x, const void* w, const float* bias,
  *   [adapters] on the device or NULL (1); coarse as ufpn_lateral_conv, or NULL.
  *   hidden: NULL, or [N * H * W][parts][rank rounded up to 8] elements that receive h for the
  *   backward, in 3 parts (BF16) or 2 (F16): the 16-bit value nearest to h, then the nearest to what
- *   is left; zeros without an adapter. */
+ *   is left; zeros without an adapter.
+ * h has 22 bits and more; F16 loses what is below 2^-25 of it (up to 2^-25 sum_r |up| in out, beside its
+ * own steps of 2^-24; grad_up through two parts of hidden, see below). */
 int ufpn_lateral_adapters(int dtype, const void* x, const void* w, const float* bias,
                           const void* down, const void* up, const int* index, const float* scales,
                           float scale, const void* coarse, void* out, void* hidden, int N, int Cin,
                           int H, int W, int rank, int adapters, int Hc, int Wc, void* stream);
+/* The same with hidden in hidden_parts parts: 3, or 2 with F16 as above.  Three of F16 are the two and
+ * 2^11 times the bits of h from 2^-36 to 2^-25 that the second one could not hold (0 where it could):
+ * grad_up then keeps 22 bits of every h down to 2^-14. */
+int ufpn_lateral_adapters_parts(int dtype, const void* x, const void* w, const float* bias,
+                                const void* down, const void* up, const int* index,
+                                const float* scales, float scale, const void* coarse, void* out,
+                                void* hidden, int hidden_parts, int N, int Cin, int H, int W, int rank,
+                                int adapters, int Hc, int Wc, void* stream);
 /* Its gradients but for w, bias (ufpn_lateral_conv_backward) and coarse (ufpn_upsample_add_backward):
  * grad_x (NULL: none), grad_down [adapters][rank][Cin] and grad_up [adapters][256][rank] in fp32 (zeros
  * for an adapter without images).  hidden: from the forward.  For grad_x the weights as w
@@ -304,7 +314,15 @@ int ufpn_lateral_adapters_backward(int dtype, const void* x, const void* w, cons
                                    float* grad_up, int N, int Cin, int H, int W, int rank,
                                    int adapters, void* workspace, size_t workspace_bytes,
                                    void* stream);
-/* (0 for sizes that the call refuses) */
+/* The same for a hidden of hidden_parts parts (ufpn_lateral_adapters_parts). */
+int ufpn_lateral_adapters_backward_parts(int dtype, const void* x, const void* w, const void* w_t,
+                                         const void* grad_out, const void* down, const void* up,
+                                         const int* index, const float* scales, float scale,
+                                         const void* hidden, int hidden_parts, void* grad_x,
+                                         float* grad_down, float* grad_up, int N, int Cin, int H, int W,
+                                         int rank, int adapters, void* workspace,
+                                         size_t workspace_bytes, void* stream);
+/* (0 for sizes that the calls refuse) */
 size_t ufpn_lateral_adapters_workspace(int dtype, int N, int Cin, int H, int W, int rank,
                                        int adapters, int has_w_t, int need_grad_x);
 
