@@ -58,6 +58,7 @@ class UnifiedFPN:
         self._config = None
         self._scale_buf = None      # e4m3 input scales, a stable device address per engine
         self._norm = None           # group norm of the outputs: (weights, biases, groups, eps, act, alpha)
+        self._norm_params = None    # its vectors [weights, biases][P2..P5][256], a stable address per engine
 
     def __del__(self):
         h = getattr(self, "_h", None)
@@ -128,8 +129,9 @@ class UnifiedFPN:
                        alpha: float = 0.01) -> None:
         """A group norm with an activation behind every level's 3x3 (:func:`fpn_group_norm` over P2..P5
         in one call, in place); P6 then comes from the normed P5.  ``weights`` / ``biases``: four [256]
-        vectors, for P2..P5 (``biases`` None = 0); ``weights=None`` takes the norm away again.  An
-        activation set by :meth:`set_activation` acts before the norm."""
+        vectors, for P2..P5 (``biases`` None = 0), copied here; ``weights=None`` takes the norm away again.
+        An activation set by :meth:`set_activation` acts before the norm.  Waits for the device: forwards
+        already enqueued, on any stream, run with what was set before, later ones with the new vectors."""
         if weights is None:
             self._norm = None
             return
@@ -139,12 +141,21 @@ class UnifiedFPN:
             raise ValueError("groups must divide 256")
         if not eps >= 0:
             raise ValueError("eps must not be negative")
-        params = []
         for name, seq in (("weights", weights), ("biases", biases)):
             if seq is not None and (len(seq) != 4 or any(t.numel() != 256 for t in seq)):
                 raise ValueError(f"{name} must be four vectors of 256 (P2-P5)")
-            params.append(None if seq is None else
-                          [t.detach().reshape(-1).to(self.device, torch.float32).clone() for t in seq])
+        values = [None if seq is None else
+                  torch.stack([t.detach().reshape(-1).to(self.device, torch.float32) for t in seq])
+                  for seq in (weights, biases)]
+        # (forwards may be reading the old vectors on other streams than this one, and the next may run there)
+        torch.cuda.synchronize(self.device)
+        if self._norm_params is None:
+            self._norm_params = torch.empty((2, 4, 256), device=self.device)
+        for buf, v in zip(self._norm_params, values):
+            if v is not None:
+                buf.copy_(v)
+        torch.cuda.synchronize(self.device)
+        params = [None if v is None else list(buf.unbind()) for buf, v in zip(self._norm_params, values)]
         self._norm = (*params, groups, eps, activation, alpha)
 
     def _apply_norm(self, outs, p6):
