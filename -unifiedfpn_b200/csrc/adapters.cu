@@ -75,7 +75,7 @@ __device__ __forceinline__ uint32_t row_chunk(int row, int chunk) {
 
 // Shared memory of fpn_adapter_kernel for ranks up to RP.  (Keeping 256 x 256 weights resident instead
 // of streaming them with every tile changed nothing: 148 against 146 us on P2 of eight images.)
-template <int RP, int kParts>
+template <int RP, int kParts, bool kTaps>
 struct AdCfg {
   static constexpr int kRow = RP * 2;   // bytes of a row of h or up
   static constexpr int kU = RP * 128;   // one k-block of down[a]
@@ -83,8 +83,9 @@ struct AdCfg {
   static constexpr int kStage = kOffU + kU;
   static constexpr int kStages = RP <= 32 ? 3 : 2;  // (three of 56 KB would not fit)
   static constexpr int kPart = kTcBlockM * kRow;
-  // h's parts; before them, in the same place, the top-down weights (their MMA is over when h is)
-  static constexpr int kT = kParts * kPart > kTcAStage ? kParts * kPart : kTcAStage;
+  // h's parts; before them, in the same place, the top-down weights in up to two parts (their MMA is over when
+  // h is)
+  static constexpr int kT = kTaps || kParts * kPart > 2 * kTcAStage ? kParts * kPart : 2 * kTcAStage;
   static constexpr int kStaging = 1024;  // per epilogue warp: 8 pixels x 64 channels
   static constexpr int kOffV = kStages * kStage;  // up[a]: 256 rows
   static constexpr int kOffT = kOffV + kTcBlockN * kRow;
@@ -113,6 +114,7 @@ struct AdArgs {
   void* out;     // NHWC, out_c channels
   int out_c;
   int map_h, map_w;  // fpn_adapter_split_kernel: the map behind the flattened one
+  int bil_parts;     // 16-bit parts of the top-down weights on the tensor cores
 };
 constexpr int kAdMaxHAccs = 4;
 int ad_h_accs(int num_kb) { return std::min(kAdMaxHAccs, (num_kb + 7) / 8); }
@@ -201,7 +203,20 @@ __device__ __noinline__ void ad_take8(uint4* dst, int stride, int store, float v
   }
 }
 
-// kTaps: the top-down taps are added from global memory in the epilogue (their box exceeds 64 pixels).
+// The taps of a pixel; one of weight 0 is another of the same pixel, so that what it holds stays out.
+__device__ __forceinline__ TcTaps ad_taps(int py, int px, int H, int W, int Hc, int Wc, float scale_y, float scale_x) {
+  TcTaps t = tc_taps(py, px, H, W, Hc, Wc, scale_y, scale_x);
+  if (t.w01 == 0.f) t.xb = t.xa;
+  if (t.w10 == 0.f) t.yb = t.ya;
+  return t;
+}
+
+// kTaps: the top-down taps are added from global memory in the epilogue (their box exceeds 64 pixels).  Else
+// an MMA adds them, which multiplies every pixel of the tile's coarse box by a weight, 0 for most: an
+// infinity or a NaN reaches all 128 pixels of the tile.  So a block that has stored any such value (each warp
+// looks at four of its pixels) computes its tiles once more with the taps that each pixel uses, from global
+// memory.  (Taking them out of the box before the MMA, by the epilogue's idle warps, kept it waiting: 149
+// instead of 144 us on P2 of eight images, which it takes without any of this.)
 template <typename T, int RP, bool kTaps>
 __global__ void __launch_bounds__(kAdThreads, 1)
     fpn_adapter_kernel(const __grid_constant__ CUtensorMap map_a,
@@ -210,7 +225,7 @@ __global__ void __launch_bounds__(kAdThreads, 1)
                        const __grid_constant__ CUtensorMap map_u, const TcGemmArgs args,
                        const AdArgs ad) {
   constexpr int kParts = kAdParts<T>;
-  using Cfg = AdCfg<RP, kParts>;
+  using Cfg = AdCfg<RP, kParts, kTaps>;
   constexpr int S = Cfg::kStages;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_addr = smem_u32(smem_raw);
@@ -224,13 +239,19 @@ __global__ void __launch_bounds__(kAdThreads, 1)
   uint64_t* tfull_bar = accf_bar + 3;  // h and up in shared memory
   uint64_t* wfull_bar = accf_bar + 4;  // the top-down weights in shared memory
   uint64_t* done_bar = accf_bar + 5;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(accf_bar + 6);
+  uint64_t* once_bar = accf_bar + 6;  // every tile stored once
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(accf_bar + 7);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  volatile int* nonfinite = abort_flag + 1;  // ... with an infinity or a NaN among them
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   const bool bil_mma = !kTaps && args.coarse != nullptr;
-  const int nkb = args.num_kb + (bil_mma ? 1 : 0);  // k-blocks of a tile: the products', the top-down add's
+  // Whether the block's tiles are computed again; a false after a timeout.
+  auto again = [&]() {
+    mbar_arrive(once_bar);
+    return mbar_wait(once_bar, 0, abort_flag, args.status, kDevTimeoutAdapter) && *nonfinite != 0;
+  };
   constexpr uint32_t kHCol = kTcBlockN;  // h accumulators: TMEM columns from 256, RP each
 
   if (threadIdx.x == 0) {
@@ -242,9 +263,11 @@ __global__ void __launch_bounds__(kAdThreads, 1)
     mbar_init(acce_bar, 32 * kAdEpiWarps);
     mbar_init(hfull_bar, 1);
     mbar_init(tfull_bar, kAdEpiWarps * 32);
-    mbar_init(wfull_bar, kTcBlockM);
+    mbar_init(wfull_bar, kTcBlockM * ad.bil_parts);
     mbar_init(done_bar, 1);
+    mbar_init(once_bar, 32 + 1 + 32 * kAdEpiWarps);  // TMA warp, MMA issuer, epilogue
     *abort_flag = 0;
+    *nonfinite = 0;
     fence_barrier_init();
     prefetch_tmap(&map_a);
     prefetch_tmap(&map_b);
@@ -267,51 +290,57 @@ __global__ void __launch_bounds__(kAdThreads, 1)
     uint32_t phase = 0;
     bool ok = true;
     const uint32_t box_bytes = static_cast<uint32_t>(args.cbox_w * args.cbox_h * 128);  // 64 channels
-    for (int tile = blockIdx.x; ok && tile < args.num_tiles; tile += gridDim.x) {
-      int n, x0, y0, slice;
-      tc_tile_origin(args, tile, n, x0, y0, slice);
-      const int adapter = ad_adapter(ad, n);
-      if (!ad.want_out && adapter < 0) continue;
-      for (int kb = 0; kb < nkb; ++kb) {
-        ok = mbar_wait(&empty_bar[stage], phase ^ 1u, abort_flag, args.status, kDevTimeoutAdapter);
-        if (!__all_sync(0xffffffffu, ok)) {
-          ok = false;
-          break;
-        }
-        uint8_t* const sa = smem + stage * Cfg::kStage;
-        uint8_t* const su = sa + Cfg::kOffU;
-        if (kb < args.num_kb) {
-          if (lane == 0) {
-            mbar_arrive_expect_tx(&full_bar[stage], kTcAStage + (ad.want_out ? kTcBStage : 0) +
-                                                        (adapter >= 0 ? Cfg::kU : 0));
-            tma_load_4d(sa, &map_a, &full_bar[stage], kb * 64, x0, y0, n, kPolicyEvictFirst);
-            if (ad.want_out)
-              tma_load_2d(sa + kTcAStage, &map_b, &full_bar[stage], kb * 64, slice * kTcBlockN,
-                          kPolicyEvictLast);
-            if (adapter >= 0)
-              tma_load_4d(su, &map_u, &full_bar[stage], kb * 64, 0, 0, adapter, kPolicyEvictLast);
+    for (bool bil = bil_mma;; bil = false) {
+      const int nkb = args.num_kb + (bil ? 1 : 0);  // k-blocks of a tile: the products', the top-down add's
+      for (int tile = blockIdx.x; ok && tile < args.num_tiles; tile += gridDim.x) {
+        int n, x0, y0, slice;
+        tc_tile_origin(args, tile, n, x0, y0, slice);
+        const int adapter = ad_adapter(ad, n);
+        if (!ad.want_out && adapter < 0) continue;
+        for (int kb = 0; kb < nkb; ++kb) {
+          ok = mbar_wait(&empty_bar[stage], phase ^ 1u, abort_flag, args.status, kDevTimeoutAdapter);
+          if (!__all_sync(0xffffffffu, ok)) {
+            ok = false;
+            break;
           }
-        } else {
-          // top-down k-block: the tile's coarse box as the B operand (the weights: the epilogue)
-          uint8_t* const sb = sa + kTcAStage;
-          tc_zero_btail(sb, lane, args.cbox_w * args.cbox_h, 4);
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) {
-            const int cy = static_cast<int>(tc_src(y0, args.scale_y, args.Hc));
-            const int cx = static_cast<int>(tc_src(x0, args.scale_x, args.Wc));
-            mbar_arrive_expect_tx(&full_bar[stage], box_bytes * 4);
-            for (int b = 0; b < 4; ++b)
-              tma_load_4d(sb + b * (kTcCoarseMaxPix * 128), &map_coarse, &full_bar[stage], b * 64, cx,
-                          cy, n, kPolicyEvictLast);
+          uint8_t* const sa = smem + stage * Cfg::kStage;
+          uint8_t* const su = sa + Cfg::kOffU;
+          if (kb < args.num_kb) {
+            if (lane == 0) {
+              mbar_arrive_expect_tx(&full_bar[stage], kTcAStage + (ad.want_out ? kTcBStage : 0) +
+                                                          (adapter >= 0 ? Cfg::kU : 0));
+              tma_load_4d(sa, &map_a, &full_bar[stage], kb * 64, x0, y0, n, kPolicyEvictFirst);
+              if (ad.want_out)
+                tma_load_2d(sa + kTcAStage, &map_b, &full_bar[stage], kb * 64, slice * kTcBlockN,
+                            kPolicyEvictLast);
+              if (adapter >= 0)
+                tma_load_4d(su, &map_u, &full_bar[stage], kb * 64, 0, 0, adapter, kPolicyEvictLast);
+            }
+          } else {
+            // top-down k-block: the tile's coarse box as the B operand (the weights: the epilogue)
+            uint8_t* const sb = sa + kTcAStage;
+            tc_zero_btail(sb, lane, args.cbox_w * args.cbox_h, 4);
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              const int cy = static_cast<int>(tc_src(y0, args.scale_y, args.Hc));
+              const int cx = static_cast<int>(tc_src(x0, args.scale_x, args.Wc));
+              mbar_arrive_expect_tx(&full_bar[stage], box_bytes * 4);
+              for (int b = 0; b < 4; ++b)
+                tma_load_4d(sb + b * (kTcCoarseMaxPix * 128), &map_coarse, &full_bar[stage], b * 64, cx,
+                            cy, n, kPolicyEvictLast);
+            }
           }
-        }
-        ++issued;
-        if (++stage == S) {
-          stage = 0;
-          phase ^= 1u;
+          ++issued;
+          if (++stage == S) {
+            stage = 0;
+            phase ^= 1u;
+          }
         }
       }
+      if (!bil) break;
+      griddep_launch_dependents();
+      if (!ok || !__all_sync(0xffffffffu, again())) break;
     }
     griddep_launch_dependents();
     if (lane == 0) {  // (matters only when another role gave up early)
@@ -334,73 +363,79 @@ __global__ void __launch_bounds__(kAdThreads, 1)
       uint32_t phase = 0, tile_phase = 0, h_phase = 0;
       const uint32_t t_addr = smem_u32(smem + Cfg::kOffT);
       bool ok = true;
-      for (int tile = blockIdx.x; ok && tile < args.num_tiles; tile += gridDim.x) {
-        int n, x0, y0, slice;
-        tc_tile_origin(args, tile, n, x0, y0, slice);
-        const bool has = ad_adapter(ad, n) >= 0;
-        if (!ad.want_out && !has) continue;
-        if (!mbar_wait(acce_bar, tile_phase ^ 1u, abort_flag, args.status, kDevTimeoutAdapter)) break;
-        tc_fence_after();
-        int hset = 0;  // kb modulo h_accs
-        for (int kb = 0; kb < nkb; ++kb) {
-          if (!mbar_wait(&full_bar[stage], phase, abort_flag, args.status, kDevTimeoutAdapter)) {
-            ok = false;
-            break;
-          }
+      for (bool bil = bil_mma;; bil = false) {
+        const int nkb = args.num_kb + (bil ? 1 : 0);
+        for (int tile = blockIdx.x; ok && tile < args.num_tiles; tile += gridDim.x) {
+          int n, x0, y0, slice;
+          tc_tile_origin(args, tile, n, x0, y0, slice);
+          const bool has = ad_adapter(ad, n) >= 0;
+          if (!ad.want_out && !has) continue;
+          if (!(ok = mbar_wait(acce_bar, tile_phase ^ 1u, abort_flag, args.status, kDevTimeoutAdapter))) break;
           tc_fence_after();
-          const uint32_t sa = smem_u32(smem + stage * Cfg::kStage);
-          const uint64_t adesc = sdesc_kmajor_sw128(sa);
-          if (kb < args.num_kb) {
-            const uint64_t bdesc = sdesc_kmajor_sw128(sa + kTcAStage);
-            const uint64_t udesc = sdesc_kmajor_sw128(sa + Cfg::kOffU);
-            // (the two products' steps alternate: the small ones, each waiting for the one before on its
-            // accumulator, run behind the large ones)
-            const uint32_t hacc = tmem_base + kHCol + static_cast<uint32_t>(hset * RP);
-            const bool h_more = kb >= ad.h_accs;
-            if (++hset == ad.h_accs) hset = 0;
-#pragma unroll
-            for (int k = 0; k < kMmaPerKb; ++k) {
-              if (ad.want_out)
-                tc_mma_f16(tmem_base, adesc + 2u * k, bdesc + 2u * k, idesc, (kb > 0 || k > 0) ? 1u : 0u);
-              if (has) tc_mma_f16(hacc, adesc + 2u * k, udesc + 2u * k, idesc_u, (h_more || k > 0) ? 1u : 0u);
-            }
-          } else {
-            if (!mbar_wait(wfull_bar, tile_phase, abort_flag, args.status, kDevTimeoutAdapter)) {
+          int hset = 0;  // kb modulo h_accs
+          for (int kb = 0; kb < nkb; ++kb) {
+            if (!mbar_wait(&full_bar[stage], phase, abort_flag, args.status, kDevTimeoutAdapter)) {
               ok = false;
               break;
             }
             tc_fence_after();
-            const uint64_t wdesc = sdesc_kmajor_sw128(t_addr);
-            const uint64_t bdesc = sdesc_mnmajor_sw128(sa + kTcAStage, kTcCoarseMaxPix * 128);
+            const uint32_t sa = smem_u32(smem + stage * Cfg::kStage);
+            const uint64_t adesc = sdesc_kmajor_sw128(sa);
+            if (kb < args.num_kb) {
+              const uint64_t bdesc = sdesc_kmajor_sw128(sa + kTcAStage);
+              const uint64_t udesc = sdesc_kmajor_sw128(sa + Cfg::kOffU);
+              // (the two products' steps alternate: the small ones, each waiting for the one before on its
+              // accumulator, run behind the large ones)
+              const uint32_t hacc = tmem_base + kHCol + static_cast<uint32_t>(hset * RP);
+              const bool h_more = kb >= ad.h_accs;
+              if (++hset == ad.h_accs) hset = 0;
 #pragma unroll
-            for (int k = 0; k < kMmaPerKb; ++k)
-              tc_mma_f16(tmem_base, wdesc + 2u * k, bdesc + 128u * k, idesc_bmn, 1u);
-          }
-          tc_commit(&empty_bar[stage]);
-          if (++stage == S) {
-            stage = 0;
-            phase ^= 1u;
-          }
-        }
-        if (!ok) break;
-        if (has) {
-          tc_commit(hfull_bar);
-          if (ad.want_out) {
-            if (!mbar_wait(tfull_bar, h_phase, abort_flag, args.status, kDevTimeoutAdapter)) break;
-            tc_fence_after();
-            const uint64_t vdesc = sdesc_kmajor_rows<Cfg::kRow>(smem_u32(smem + Cfg::kOffV));
+              for (int k = 0; k < kMmaPerKb; ++k) {
+                if (ad.want_out)
+                  tc_mma_f16(tmem_base, adesc + 2u * k, bdesc + 2u * k, idesc, (kb > 0 || k > 0) ? 1u : 0u);
+                if (has) tc_mma_f16(hacc, adesc + 2u * k, udesc + 2u * k, idesc_u, (h_more || k > 0) ? 1u : 0u);
+              }
+            } else {
+              if (!mbar_wait(wfull_bar, tile_phase, abort_flag, args.status, kDevTimeoutAdapter)) {
+                ok = false;
+                break;
+              }
+              tc_fence_after();
+              const uint64_t bdesc = sdesc_mnmajor_sw128(sa + kTcAStage, kTcCoarseMaxPix * 128);
+              for (int part = 0; part < ad.bil_parts; ++part) {
+                const uint64_t wdesc = sdesc_kmajor_sw128(t_addr + part * kTcAStage);
 #pragma unroll
-            for (int part = 0; part < kParts; ++part) {
-              const uint64_t tdesc = sdesc_kmajor_rows<Cfg::kRow>(t_addr + part * Cfg::kPart);
-#pragma unroll
-              for (int k = 0; k < RP / 16; ++k)
-                tc_mma_f16(tmem_base, tdesc + 2u * k, vdesc + 2u * k, idesc, 1u);
+                for (int k = 0; k < kMmaPerKb; ++k)
+                  tc_mma_f16(tmem_base, wdesc + 2u * k, bdesc + 128u * k, idesc_bmn, 1u);
+              }
+            }
+            tc_commit(&empty_bar[stage]);
+            if (++stage == S) {
+              stage = 0;
+              phase ^= 1u;
             }
           }
-          h_phase ^= 1u;
+          if (!ok) break;
+          if (has) {
+            tc_commit(hfull_bar);
+            if (ad.want_out) {
+              if (!(ok = mbar_wait(tfull_bar, h_phase, abort_flag, args.status, kDevTimeoutAdapter))) break;
+              tc_fence_after();
+              const uint64_t vdesc = sdesc_kmajor_rows<Cfg::kRow>(smem_u32(smem + Cfg::kOffV));
+#pragma unroll
+              for (int part = 0; part < kParts; ++part) {
+                const uint64_t tdesc = sdesc_kmajor_rows<Cfg::kRow>(t_addr + part * Cfg::kPart);
+#pragma unroll
+                for (int k = 0; k < RP / 16; ++k)
+                  tc_mma_f16(tmem_base, tdesc + 2u * k, vdesc + 2u * k, idesc, 1u);
+              }
+            }
+            h_phase ^= 1u;
+          }
+          if (ad.want_out) tc_commit(accf_bar);
+          tile_phase ^= 1u;
         }
-        if (ad.want_out) tc_commit(accf_bar);
-        tile_phase ^= 1u;
+        if (!bil || !ok || !again()) break;
       }
       tc_commit(done_bar);
       mbar_wait_drain(done_bar, 0);
@@ -422,220 +457,266 @@ __global__ void __launch_bounds__(kAdThreads, 1)
     for (int i = lane; i < kAdWarpCols; i += 32)
       bias_s[i] = args.bias != nullptr ? __ldg(args.bias + cq * kAdWarpCols + i) : 0.f;
     __syncwarp();
-    for (int tile = blockIdx.x; tile < args.num_tiles; tile += gridDim.x) {
-      int n, x0, y0, slice;
-      tc_tile_origin(args, tile, n, x0, y0, slice);
-      const int adapter = ad_adapter(ad, n);
-      const bool has = adapter >= 0;
-      const int py = y0 + (row >> tw_shift), px = x0 + (row & tw_mask);
-      const bool valid = py < args.H && px < args.W;
-      // Here the tile before is through: its MMAs have read h, up and the top-down weights.
-      if (bil_mma && cq == 0) {
-        // this pixel's row of the top-down weights: four of 64 coarse pixels
-        const uint4 z = make_uint4(0u, 0u, 0u, 0u);
+    for (bool bil = bil_mma;; bil = false) {
+      for (int tile = blockIdx.x; tile < args.num_tiles; tile += gridDim.x) {
+        int n, x0, y0, slice;
+        tc_tile_origin(args, tile, n, x0, y0, slice);
+        const int adapter = ad_adapter(ad, n);
+        const bool has = adapter >= 0;
+        const int py = y0 + (row >> tw_shift), px = x0 + (row & tw_mask);
+        const bool valid = py < args.H && px < args.W;
+        // Here the tile before is through: its MMAs have read h, up and the top-down weights.
+        if (bil && cq < ad.bil_parts) {
+          // this pixel's row of the top-down weights, part cq: four of 64 coarse pixels
+          const uint32_t wrow = t_addr + cq * kTcAStage + row * 128;
+          const uint4 z = make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) st_shared_v4(t_addr + row * 128 + ((j ^ (row & 7)) << 4), z);
-        const TcTaps tp = tc_taps(py, px, args.H, args.W, args.Hc, args.Wc, args.scale_y, args.scale_x);
-        const int cy0 = static_cast<int>(tc_src(y0, args.scale_y, args.Hc));
-        const int cx0 = static_cast<int>(tc_src(x0, args.scale_x, args.Wc));
-        int k[4] = {(tp.ya - cy0) * args.cbox_w + tp.xa - cx0, (tp.ya - cy0) * args.cbox_w + tp.xb - cx0,
-                    (tp.yb - cy0) * args.cbox_w + tp.xa - cx0, (tp.yb - cy0) * args.cbox_w + tp.xb - cx0};
-        float w[4] = {tp.w00, tp.w01, tp.w10, tp.w11};
-        // (corners that coincide at the map's border add their weights)
+          for (int j = 0; j < 8; ++j) st_shared_v4(wrow + ((j ^ (row & 7)) << 4), z);
+          const TcTaps tp = tc_taps(py, px, args.H, args.W, args.Hc, args.Wc, args.scale_y, args.scale_x);
+          const int cy0 = static_cast<int>(tc_src(y0, args.scale_y, args.Hc));
+          const int cx0 = static_cast<int>(tc_src(x0, args.scale_x, args.Wc));
+          int k[4] = {(tp.ya - cy0) * args.cbox_w + tp.xa - cx0, (tp.ya - cy0) * args.cbox_w + tp.xb - cx0,
+                      (tp.yb - cy0) * args.cbox_w + tp.xa - cx0, (tp.yb - cy0) * args.cbox_w + tp.xb - cx0};
+          float w[4] = {tp.w00, tp.w01, tp.w10, tp.w11};
+          // (corners that coincide at the map's border add their weights)
 #pragma unroll
-        for (int i = 1; i < 4; ++i)
+          for (int i = 1; i < 4; ++i)
 #pragma unroll
-          for (int j = 0; j < i; ++j)
-            if (k[i] == k[j] && w[j] != 0.f) {
-              w[j] += w[i];
-              w[i] = 0.f;
-            }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if (w[i] == 0.f || k[i] < 0 || k[i] >= args.cbox_w * args.cbox_h) continue;
-          const uint32_t byte = static_cast<uint32_t>(k[i]) * 2u;
-          st_shared_u16(t_addr + row * 128 + ((((byte >> 4) ^ (row & 7)) & 7) << 4) + (byte & 15),
-                        Pack<T>::bits(w[i]));
-        }
-        fence_proxy_async_smem();
-        mbar_arrive(wfull_bar);
-      }
-      uint4* hid = nullptr;  // this thread's pixel of `hidden`
-      if (ad.hidden != nullptr && slice == 0 && valid)
-        hid = reinterpret_cast<uint4*>(
-            static_cast<uint8_t*>(ad.hidden) +
-            ((static_cast<size_t>(n) * args.H + py) * args.W + px) * ad.rank_pad * (2 * ad_stored<T>(ad.store)));
-      if (has) {
-        if (ad.want_out && cq >= 2 && (adapter != v_adapter || slice != v_slice)) {
-          // up[a] (this slice's 256 rows): one row a thread of the upper two quarters
-          const int c = (cq - 2) * kTcBlockM + row;
-          const int ch = slice * kTcBlockN + c;
-          const uint16_t* src = static_cast<const uint16_t*>(ad.v) + adapter * ad.va + ch * ad.vc;
-#pragma unroll
-          for (int j = 0; j < RP / 8; ++j) {
-            uint4 q = make_uint4(0u, 0u, 0u, 0u);
-            if (ch < ad.v_rows && j * 8 < ad.rank) {
-              if (ad.v_vec) {
-                q = __ldg(reinterpret_cast<const uint4*>(src) + j);
-              } else {
-                uint32_t w[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                  const int r = j * 8 + 2 * i;
-                  const uint32_t lo = r < ad.rank ? __ldg(src + r * ad.vr) : 0;
-                  const uint32_t hi = r + 1 < ad.rank ? __ldg(src + (r + 1) * ad.vr) : 0;
-                  w[i] = lo | (hi << 16);
-                }
-                q = make_uint4(w[0], w[1], w[2], w[3]);
+            for (int j = 0; j < i; ++j)
+              if (k[i] == k[j] && w[j] != 0.f) {
+                w[j] += w[i];
+                w[i] = 0.f;
               }
-            }
-            st_shared_v4(v_addr + row_chunk<Cfg::kRow>(c, j), q);
-          }
-        }
-        v_adapter = adapter;
-        v_slice = slice;
-        const float s = ad.scale * (ad.scales != nullptr ? __ldg(ad.scales + adapter) : 1.f);
-        // (every warp waits for the tile's h, so that none runs ahead on the barriers below)
-        const bool ok = mbar_wait(hfull_bar, h_phase, abort_flag, args.status, kDevTimeoutAdapter);
-        if (!__all_sync(0xffffffffu, ok)) break;
-        tc_fence_after();
-        const uint32_t hacc = tmem_base + kHCol + lane_addr;
-        // 8 columns at a time, by the quarters in turn
-#pragma unroll 1
-        for (int j = cq; j < RP / 8; j += 4) {
-          uint32_t r[8];
-          float h[8];
-          __syncwarp();
-          tmem_ld8(hacc + j * 8, r);
-          tmem_wait_ld();
 #pragma unroll
-          for (int i = 0; i < 8; ++i) h[i] = __uint_as_float(r[i]);
-          for (int q = 1; q < ad.h_accs; ++q) {
-            tmem_ld8(hacc + q * RP + j * 8, r);
+          for (int i = 0; i < 4; ++i) {
+            if (w[i] == 0.f || k[i] < 0 || k[i] >= args.cbox_w * args.cbox_h) continue;
+            const uint32_t byte = static_cast<uint32_t>(k[i]) * 2u;
+            uint16_t bits = Pack<T>::bits(w[i]);
+            if (cq > 0) bits = Pack<T>::bits(w[i] - Pack<T>::unpack(static_cast<uint32_t>(bits)).x);
+            st_shared_u16(wrow + ((((byte >> 4) ^ (row & 7)) & 7) << 4) + (byte & 15), bits);
+          }
+          fence_proxy_async_smem();
+          mbar_arrive(wfull_bar);
+        }
+        uint4* hid = nullptr;  // this thread's pixel of `hidden`
+        if (ad.hidden != nullptr && slice == 0 && valid)
+          hid = reinterpret_cast<uint4*>(
+              static_cast<uint8_t*>(ad.hidden) +
+              ((static_cast<size_t>(n) * args.H + py) * args.W + px) * ad.rank_pad * (2 * ad_stored<T>(ad.store)));
+        if (has) {
+          if (ad.want_out && cq >= 2 && (adapter != v_adapter || slice != v_slice)) {
+            // up[a] (this slice's 256 rows): one row a thread of the upper two quarters
+            const int c = (cq - 2) * kTcBlockM + row;
+            const int ch = slice * kTcBlockN + c;
+            const uint16_t* src = static_cast<const uint16_t*>(ad.v) + adapter * ad.va + ch * ad.vc;
+#pragma unroll
+            for (int j = 0; j < RP / 8; ++j) {
+              uint4 q = make_uint4(0u, 0u, 0u, 0u);
+              if (ch < ad.v_rows && j * 8 < ad.rank) {
+                if (ad.v_vec) {
+                  q = __ldg(reinterpret_cast<const uint4*>(src) + j);
+                } else {
+                  uint32_t w[4];
+#pragma unroll
+                  for (int i = 0; i < 4; ++i) {
+                    const int r = j * 8 + 2 * i;
+                    const uint32_t lo = r < ad.rank ? __ldg(src + r * ad.vr) : 0;
+                    const uint32_t hi = r + 1 < ad.rank ? __ldg(src + (r + 1) * ad.vr) : 0;
+                    w[i] = lo | (hi << 16);
+                  }
+                  q = make_uint4(w[0], w[1], w[2], w[3]);
+                }
+              }
+              st_shared_v4(v_addr + row_chunk<Cfg::kRow>(c, j), q);
+            }
+          }
+          v_adapter = adapter;
+          v_slice = slice;
+          const float s = ad.scale * (ad.scales != nullptr ? __ldg(ad.scales + adapter) : 1.f);
+          // (every warp waits for the tile's h, so that none runs ahead on the barriers below)
+          const bool ok = mbar_wait(hfull_bar, h_phase, abort_flag, args.status, kDevTimeoutAdapter);
+          if (!__all_sync(0xffffffffu, ok)) break;
+          tc_fence_after();
+          const uint32_t hacc = tmem_base + kHCol + lane_addr;
+          // 8 columns at a time, by the quarters in turn
+#pragma unroll 1
+          for (int j = cq; j < RP / 8; j += 4) {
+            uint32_t r[8];
+            float h[8];
+            __syncwarp();
+            tmem_ld8(hacc + j * 8, r);
             tmem_wait_ld();
 #pragma unroll
-            for (int i = 0; i < 8; ++i) h[i] += __uint_as_float(r[i]);
-          }
+            for (int i = 0; i < 8; ++i) h[i] = __uint_as_float(r[i]);
+            for (int q = 1; q < ad.h_accs; ++q) {
+              tmem_ld8(hacc + q * RP + j * 8, r);
+              tmem_wait_ld();
 #pragma unroll
-          for (int i = 0; i < 8; ++i) h[i] = j * 8 + i < ad.rank ? s * h[i] : 0.f;
-          if (kParts == kAdStored || ad.want_out) {
-            uint32_t w[kParts][4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              uint16_t p0[kParts], p1[kParts];
-              ad_split<T>(h[2 * i], p0);
-              ad_split<T>(h[2 * i + 1], p1);
-#pragma unroll
-              for (int part = 0; part < kParts; ++part)
-                w[part][i] = p0[part] | (static_cast<uint32_t>(p1[part]) << 16);
+              for (int i = 0; i < 8; ++i) h[i] += __uint_as_float(r[i]);
             }
 #pragma unroll
-            for (int part = 0; part < kParts; ++part) {
-              const uint4 q = make_uint4(w[part][0], w[part][1], w[part][2], w[part][3]);
-              if (ad.want_out) st_shared_v4(t_addr + part * Cfg::kPart + row_chunk<Cfg::kRow>(row, j), q);
-              if (kParts == kAdStored && hid != nullptr && j * 8 < ad.rank_pad)
-                hid[(part * ad.rank_pad >> 3) + j] = q;
+            for (int i = 0; i < 8; ++i) h[i] = j * 8 + i < ad.rank ? s * h[i] : 0.f;
+            if (kParts == kAdStored || ad.want_out) {
+              uint32_t w[kParts][4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                uint16_t p0[kParts], p1[kParts];
+                ad_split<T>(h[2 * i], p0);
+                ad_split<T>(h[2 * i + 1], p1);
+#pragma unroll
+                for (int part = 0; part < kParts; ++part)
+                  w[part][i] = p0[part] | (static_cast<uint32_t>(p1[part]) << 16);
+              }
+#pragma unroll
+              for (int part = 0; part < kParts; ++part) {
+                const uint4 q = make_uint4(w[part][0], w[part][1], w[part][2], w[part][3]);
+                if (ad.want_out) st_shared_v4(t_addr + part * Cfg::kPart + row_chunk<Cfg::kRow>(row, j), q);
+                if (kParts == kAdStored && hid != nullptr && j * 8 < ad.rank_pad)
+                  hid[(part * ad.rank_pad >> 3) + j] = q;
+              }
             }
+            if (kParts != kAdStored && hid != nullptr && j * 8 < ad.rank_pad)
+              ad_take8<T>(hid + j, ad.rank_pad >> 3, ad.store, h[0], h[1], h[2], h[3], h[4], h[5], h[6], h[7]);
           }
-          if (kParts != kAdStored && hid != nullptr && j * 8 < ad.rank_pad)
-            ad_take8<T>(hid + j, ad.rank_pad >> 3, ad.store, h[0], h[1], h[2], h[3], h[4], h[5], h[6], h[7]);
+          fence_proxy_async_smem();
+          tc_fence_before();
+          mbar_arrive(tfull_bar);
+          h_phase ^= 1u;
+          if (!ad.want_out) mbar_arrive(acce_bar);
+        } else if (hid != nullptr && cq == 0) {
+          for (int j = 0; j < ad.rank_pad * ad_stored<T>(ad.store) / 8; ++j) hid[j] = make_uint4(0u, 0u, 0u, 0u);
         }
-        fence_proxy_async_smem();
-        tc_fence_before();
-        mbar_arrive(tfull_bar);
-        h_phase ^= 1u;
-        if (!ad.want_out) mbar_arrive(acce_bar);
-      } else if (hid != nullptr && cq == 0) {
-        for (int j = 0; j < ad.rank_pad * ad_stored<T>(ad.store) / 8; ++j) hid[j] = make_uint4(0u, 0u, 0u, 0u);
-      }
-      if (!ad.want_out) continue;
+        if (!ad.want_out) continue;
 
-      const bool ok = mbar_wait(accf_bar, tile_phase, abort_flag, args.status, kDevTimeoutAdapter);
-      if (!__all_sync(0xffffffffu, ok)) break;
-      tile_phase ^= 1u;
-      tc_fence_after();
-      // The warp's accumulators go to registers at once, so that the next tile's MMAs start while
-      // they are converted and stored.
-      uint32_t rr[kAdWarpCols];
-      __syncwarp();
+        const bool ok = mbar_wait(accf_bar, tile_phase, abort_flag, args.status, kDevTimeoutAdapter);
+        if (!__all_sync(0xffffffffu, ok)) break;
+        tile_phase ^= 1u;
+        tc_fence_after();
+        if (!kTaps && bil_mma && !bil) {  // once more, with the taps
+          const TcTaps tp = ad_taps(py, px, args.H, args.W, args.Hc, args.Wc, args.scale_y, args.scale_x);
+          const T* c = static_cast<const T*>(args.coarse) +
+                       static_cast<size_t>(n) * args.Hc * args.Wc * kTcBlockN + cq * kAdWarpCols;
+          T* const o = static_cast<T*>(ad.out) +
+                       ((static_cast<size_t>(n) * args.H + py) * args.W + px) * kTcBlockN + cq * kAdWarpCols;
+#pragma unroll 1
+          for (int j = 0; j < kAdWarpCols / 8; ++j) {
+            uint32_t r[8];
+            __syncwarp();
+            tmem_ld8(tmem_base + cq * kAdWarpCols + j * 8 + lane_addr, r);
+            tmem_wait_ld();
+            float v[8];
 #pragma unroll
-      for (int q = 0; q < kAdWarpCols / 32; ++q)
-        tmem_ld32(tmem_base + cq * kAdWarpCols + q * 32 + lane_addr,
-                  *reinterpret_cast<uint32_t(*)[32]>(&rr[q * 32]));
-      tmem_wait_ld();
-      tc_fence_before();
-      mbar_arrive(acce_bar);
-
-      TcTaps tp{};
-      const T* tap[4];
-      if constexpr (kTaps) {
-        tp = tc_taps(py, px, args.H, args.W, args.Hc, args.Wc, args.scale_y, args.scale_x);
-        const T* c = static_cast<const T*>(args.coarse) +
-                     static_cast<size_t>(n) * args.Hc * args.Wc * kTcBlockN + cq * kAdWarpCols;
-        tap[0] = c + (static_cast<size_t>(tp.ya) * args.Wc + tp.xa) * kTcBlockN;
-        tap[1] = c + (static_cast<size_t>(tp.ya) * args.Wc + tp.xb) * kTcBlockN;
-        tap[2] = c + (static_cast<size_t>(tp.yb) * args.Wc + tp.xa) * kTcBlockN;
-        tap[3] = c + (static_cast<size_t>(tp.yb) * args.Wc + tp.xb) * kTcBlockN;
-      }
-      uint4 pk[kAdWarpCols / 8];  // the pixel's channels, rounded
-#pragma unroll
-      for (int step = 0; step < kAdWarpCols / 16; ++step) {
-        float v[16];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float4 b = *reinterpret_cast<const float4*>(bias_s + step * 16 + 4 * i);
-          v[4 * i + 0] = __uint_as_float(rr[step * 16 + 4 * i + 0]) + b.x;
-          v[4 * i + 1] = __uint_as_float(rr[step * 16 + 4 * i + 1]) + b.y;
-          v[4 * i + 2] = __uint_as_float(rr[step * 16 + 4 * i + 2]) + b.z;
-          v[4 * i + 3] = __uint_as_float(rr[step * 16 + 4 * i + 3]) + b.w;
-        }
-        if constexpr (kTaps) {
-          const float w[4] = {tp.w00, tp.w01, tp.w10, tp.w11};
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const uint4 q = __ldg(reinterpret_cast<const uint4*>(tap[k] + step * 16) + h);
+            for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(r[i]) + bias_s[j * 8 + i];
+#pragma unroll 1
+            for (int k = 0; k < 4; ++k) {
+              const float wk = k == 0 ? tp.w00 : k == 1 ? tp.w01 : k == 2 ? tp.w10 : tp.w11;
+              const size_t at = static_cast<size_t>(k < 2 ? tp.ya : tp.yb) * args.Wc + ((k & 1) == 0 ? tp.xa : tp.xb);
+              const uint4 q = __ldg(reinterpret_cast<const uint4*>(c + at * kTcBlockN) + j);
               const uint32_t u[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
                 const float2 f = Pack<T>::unpack(u[e]);
-                v[8 * h + 2 * e] = fmaf(w[k], f.x, v[8 * h + 2 * e]);
-                v[8 * h + 2 * e + 1] = fmaf(w[k], f.y, v[8 * h + 2 * e + 1]);
+                v[2 * e] = fmaf(wk, f.x, v[2 * e]);
+                v[2 * e + 1] = fmaf(wk, f.y, v[2 * e + 1]);
               }
             }
+            if (valid)
+              reinterpret_cast<uint4*>(o)[j] = make_uint4(Pack<T>::pack(v[0], v[1]), Pack<T>::pack(v[2], v[3]),
+                                                          Pack<T>::pack(v[4], v[5]), Pack<T>::pack(v[6], v[7]));
+          }
+          tc_fence_before();
+          mbar_arrive(acce_bar);
+          continue;
         }
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-          pk[2 * step + h] =
-              make_uint4(Pack<T>::pack(v[8 * h + 0], v[8 * h + 1]), Pack<T>::pack(v[8 * h + 2], v[8 * h + 3]),
-                         Pack<T>::pack(v[8 * h + 4], v[8 * h + 5]), Pack<T>::pack(v[8 * h + 6], v[8 * h + 7]));
-      }
-      // 8 pixels at a time through the warp's 1 KB of shared memory, so that 8 lanes write the 128 bytes of a
-      // pixel: lane l stores chunk l % 8 of pixels l / 8 and l / 8 + 4.  (32 pixels of 16 channels at a time
-      // touched 16 lines an instruction instead of 4: 145 us for P2 of eight images.)
-      const int scol = slice * kTcBlockN + cq * kAdWarpCols + (lane & 7) * 8;
-      const bool in_cols = scol < ad.out_c;
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        if ((lane >> 3) == g) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) st_shared_v4(stage_addr + row_chunk<128>(lane & 7, j), pk[j]);
-        }
-        __syncwarp();
-        uint4 o[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) o[i] = ld_shared_v4(stage_addr + row_chunk<128>((lane >> 3) + 4 * i, lane & 7));
+        // The warp's accumulators go to registers at once, so that the next tile's MMAs start while
+        // they are converted and stored.
+        uint32_t rr[kAdWarpCols];
         __syncwarp();
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int r = quarter * 32 + g * 8 + (lane >> 3) + 4 * i;
-          const int sy = y0 + (r >> tw_shift), sx = x0 + (r & tw_mask);
-          if (in_cols && sy < args.H && sx < args.W)
-            *reinterpret_cast<uint4*>(static_cast<T*>(ad.out) +
-                                      ((static_cast<size_t>(n) * args.H + sy) * args.W + sx) * ad.out_c + scol) = o[i];
+        for (int q = 0; q < kAdWarpCols / 32; ++q)
+          tmem_ld32(tmem_base + cq * kAdWarpCols + q * 32 + lane_addr,
+                    *reinterpret_cast<uint32_t(*)[32]>(&rr[q * 32]));
+        tmem_wait_ld();
+        tc_fence_before();
+        mbar_arrive(acce_bar);
+
+        TcTaps tp{};
+        const T* tap[4];
+        if constexpr (kTaps) {
+          tp = ad_taps(py, px, args.H, args.W, args.Hc, args.Wc, args.scale_y, args.scale_x);
+          const T* c = static_cast<const T*>(args.coarse) +
+                       static_cast<size_t>(n) * args.Hc * args.Wc * kTcBlockN + cq * kAdWarpCols;
+          tap[0] = c + (static_cast<size_t>(tp.ya) * args.Wc + tp.xa) * kTcBlockN;
+          tap[1] = c + (static_cast<size_t>(tp.ya) * args.Wc + tp.xb) * kTcBlockN;
+          tap[2] = c + (static_cast<size_t>(tp.yb) * args.Wc + tp.xa) * kTcBlockN;
+          tap[3] = c + (static_cast<size_t>(tp.yb) * args.Wc + tp.xb) * kTcBlockN;
+        }
+        uint4 pk[kAdWarpCols / 8];  // the pixel's channels, rounded
+#pragma unroll
+        for (int step = 0; step < kAdWarpCols / 16; ++step) {
+          float v[16];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float4 b = *reinterpret_cast<const float4*>(bias_s + step * 16 + 4 * i);
+            v[4 * i + 0] = __uint_as_float(rr[step * 16 + 4 * i + 0]) + b.x;
+            v[4 * i + 1] = __uint_as_float(rr[step * 16 + 4 * i + 1]) + b.y;
+            v[4 * i + 2] = __uint_as_float(rr[step * 16 + 4 * i + 2]) + b.z;
+            v[4 * i + 3] = __uint_as_float(rr[step * 16 + 4 * i + 3]) + b.w;
+          }
+          if constexpr (kTaps) {
+            const float w[4] = {tp.w00, tp.w01, tp.w10, tp.w11};
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const uint4 q = __ldg(reinterpret_cast<const uint4*>(tap[k] + step * 16) + h);
+                const uint32_t u[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  const float2 f = Pack<T>::unpack(u[e]);
+                  v[8 * h + 2 * e] = fmaf(w[k], f.x, v[8 * h + 2 * e]);
+                  v[8 * h + 2 * e + 1] = fmaf(w[k], f.y, v[8 * h + 2 * e + 1]);
+                }
+              }
+          }
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            pk[2 * step + h] =
+                make_uint4(Pack<T>::pack(v[8 * h + 0], v[8 * h + 1]), Pack<T>::pack(v[8 * h + 2], v[8 * h + 3]),
+                           Pack<T>::pack(v[8 * h + 4], v[8 * h + 5]), Pack<T>::pack(v[8 * h + 6], v[8 * h + 7]));
+        }
+        // 8 pixels at a time through the warp's 1 KB of shared memory, so that 8 lanes write the 128 bytes of a
+        // pixel: lane l stores chunk l % 8 of pixels l / 8 and l / 8 + 4.  (32 pixels of 16 channels at a time
+        // touched 16 lines an instruction instead of 4: 145 us for P2 of eight images.)
+        const int scol = slice * kTcBlockN + cq * kAdWarpCols + (lane & 7) * 8;
+        const bool in_cols = scol < ad.out_c;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          if ((lane >> 3) == g) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) st_shared_v4(stage_addr + row_chunk<128>(lane & 7, j), pk[j]);
+          }
+          __syncwarp();
+          uint4 o[2];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) o[i] = ld_shared_v4(stage_addr + row_chunk<128>((lane >> 3) + 4 * i, lane & 7));
+          __syncwarp();
+          if (g == 0 && bil) {  // (all 64 channels, of four pixels)
+            constexpr uint32_t kInf = TcElem<T>::kFmt == 0 ? 0x7c007c00u : 0x7f807f80u, kAbs = 0x7fff7fffu;
+            const uint32_t most = __vmaxu2(__vmaxu2(o[0].x & kAbs, o[0].y & kAbs), __vmaxu2(o[0].z & kAbs, o[0].w & kAbs));
+            if (__vcmpgeu2(most, kInf) != 0u) *nonfinite = 1;
+          }
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int r = quarter * 32 + g * 8 + (lane >> 3) + 4 * i;
+            const int sy = y0 + (r >> tw_shift), sx = x0 + (r & tw_mask);
+            if (in_cols && sy < args.H && sx < args.W)
+              *reinterpret_cast<uint4*>(static_cast<T*>(ad.out) +
+                                        ((static_cast<size_t>(n) * args.H + sy) * args.W + sx) * ad.out_c + scol) = o[i];
+          }
         }
       }
+      if (!bil || !__all_sync(0xffffffffu, again())) break;
     }
   }
 
@@ -892,7 +973,7 @@ __global__ void __launch_bounds__(kAdThreads, 1)
         for (int i = 0; i < kBatch; ++i) {
           const int p = min(x0 + r0 + 8 * S * (i0 + i), pixels - 1);
           const int py = p / ad.map_w, px = p - py * ad.map_w;
-          const TcTaps tp = tc_taps(py, px, ad.map_h, ad.map_w, args.Hc, args.Wc, args.scale_y, args.scale_x);
+          const TcTaps tp = ad_taps(py, px, ad.map_h, ad.map_w, args.Hc, args.Wc, args.scale_y, args.scale_x);
           const T* top = coarse + static_cast<size_t>(tp.ya) * args.Wc * kTcBlockN;
           const T* bottom = coarse + static_cast<size_t>(tp.yb) * args.Wc * kTcBlockN;
           q[i][0] = __ldg(reinterpret_cast<const uint2*>(top + tp.xa * kTcBlockN));
@@ -1346,7 +1427,7 @@ __global__ void __launch_bounds__(256)
 template <typename T, int RP, bool kTaps>
 cudaError_t launch_adapter_rp(const TcPlan& p, const CUtensorMap& map_u, const AdArgs& ad, const LaunchOpts& opts,
                               cudaStream_t s) {
-  using Cfg = AdCfg<RP, kAdParts<T>>;
+  using Cfg = AdCfg<RP, kAdParts<T>, kTaps>;
   auto kern = fpn_adapter_kernel<T, RP, kTaps>;
   static std::atomic<bool> configured[64];
   cudaError_t e = once_per_device(configured, [&] {
@@ -1574,6 +1655,16 @@ cudaError_t adapter_grads_t(const AdapterProblem& p, const void* x, const void* 
   return cudaSuccess;
 }
 
+// 16-bit parts of the bilinear weights on the tensor cores: one where they are exact (ratios of 1 to 8 that are
+// powers of two: products of the axes' 0, 2, 3 or 4 bits), else two, 16 bits and more of a weight.  (One rounded
+// part left a constant coarse map up to 2.9e-3 off in bf16; two cost 6 % on two 200 x 304 maps over 67 x 102.)
+int bilinear_parts(int H, int W, int Hc, int Wc) {
+  auto bits = [](int out, int in) {
+    return out == in ? 0 : out == 2 * in ? 2 : out == 4 * in ? 3 : out == 8 * in ? 4 : 16;
+  };
+  return bits(H, Hc) + bits(W, Wc) <= 8 ? 1 : 2;
+}
+
 }  // namespace
 
 cudaError_t launch_lateral_adapters(const AdapterProblem& p, const void* x, const void* w,
@@ -1607,6 +1698,7 @@ cudaError_t launch_lateral_adapters(const AdapterProblem& p, const void* x, cons
   ad.out_c = 256;
   ad.map_h = p.H;
   ad.map_w = p.W;
+  ad.bil_parts = coarse ? bilinear_parts(p.H, p.W, Hc, Wc) : 1;
   TcPlan plan;
   // Few tiles: split over k (at most half the SMs, so that two CTAs a tile fit).
   if ((p.Cin + 63) / 64 >= 8 &&
@@ -1685,6 +1777,7 @@ cudaError_t launch_lateral_adapters_backward(const AdapterProblem& p, const void
   ad.rank_pad = pad8(p.rank);
   ad.want_out = dx != nullptr;
   ad.h_accs = ad_h_accs(4);
+  ad.bil_parts = 1;
   ad.out = dx;
   ad.out_c = p.Cin;
   e = p.dtype == DType::BF16 ? launch_adapter_t<__nv_bfloat16>(plan, map_u, ad, adapter_ahead(), s)

@@ -92,7 +92,9 @@ def fpn_lateral_adapters(input: torch.Tensor, weight: torch.Tensor, bias: torch.
     without an adapter; ``scale``: a number, or [L] on the device.  ``weight`` [256, Cin] or [256,
     Cin, 1, 1], ``bias`` [256], Cin a multiple of 8, at most 2048.  Sums are fp32 and rounded once;
     h is carried in 16-bit parts of 22 bits and more together, of which fp16 loses what is below 2^-25 (up
-    to 2^-25 * sum_r |up| in the output, whose own steps end at 2^-24).  With ``return_hidden`` also returns
+    to 2^-25 * sum_r |up| in the output, whose own steps end at 2^-24); the bilinear weights are fp32 or have 16
+    bits and more.  Values of ``coarse`` that are not finite reach the pixels that use them alone (a call
+    that meets any takes up to twice as long).  With ``return_hidden`` also returns
     h in parts (opaque, [N, H, W, 3, R rounded up to 8]; fp16: what is below 2^-36 is lost) for
     :func:`fpn_lateral_adapters_backward`."""
     down, up, index, scales, scale = _check(input, down, up, index, scale)

@@ -283,7 +283,8 @@ int ufpn_conv3x3_act(int dtype, const void* x, const void* w, const float* bias,
  * dtype F16/BF16 (x, w, down, up, coarse, out); Cin a multiple of 8, at most 2048; rank 1..64;
  * every tensor 16-byte aligned.  No reference counterpart.
  *   down [adapters][rank][Cin], up [adapters][256][rank], index int32 [N] on the device, scales fp32
- *   [adapters] on the device or NULL (1); coarse as ufpn_lateral_conv, or NULL.
+ *   [adapters] on the device or NULL (1); coarse as ufpn_lateral_conv, or NULL (its bilinear weights are
+ *   fp32 or have 16 bits and more; values that are not finite reach the pixels that use them alone).
  *   hidden: NULL, or [N * H * W][parts][rank rounded up to 8] elements that receive h for the
  *   backward, in 3 parts (BF16) or 2 (F16): the 16-bit value nearest to h, then the nearest to what
  *   is left; zeros without an adapter.
