@@ -10,11 +10,13 @@
 //   dx = rstd * (w dz - mean_g(w dz) - xhat * mean_g(w dz xhat))
 //
 // All statistics and sums are fp32.  The variance never comes from a difference of raw moments: a
-// thread sums its pixels relative to its first one, so that what it subtracts is of the size of the
-// spread, and such (count, mean, M2) triples merge as
+// thread sums its pixels relative to the channel's median of three of them (a fixed three of the image,
+// or of the block's share), so that what it subtracts is of the size of the spread, and such (count, mean,
+// M2) triples merge as
 //   M2_ab = M2_a + M2_b + (mean_b - mean_a)^2 n_a n_b / (n_a + n_b),
-// their means taken relative to the group's first value in the image (the pivot): a mean far above
-// the spread costs no digits in between.  Every sum has a fixed order (no atomics): the same inputs
+// their means taken relative to that of the group's first channel (the pivot): a mean far above the
+// spread costs no digits in between, and neither does one value far from all others (relative to the
+// first pixel, a value of 1e6 there left the mean 4e-5 of the spread off, and rstd 9e-6).  Every sum has a fixed order (no atomics): the same inputs
 // give the same bits.
 //
 // The kernel moves bytes.  The batch is cut into segments whose maps stay in the 126 MB L2 cache;
@@ -208,7 +210,7 @@ __device__ __forceinline__ float2 gn_act_grad(float2 dy, float2 z, float alpha) 
 struct GnSmem {
   uint8_t stats_ring[kGnWarps][kGnStatsStages * kGnStage];
   uint8_t apply_ring[kGnWarps][kGnApplyStages * kGnStage];
-  // statistics: the image's first pixel; a chunk's pixel lanes [lane][C] and their pixel counts
+  // statistics: the image's medians of three pixels; a chunk's pixel lanes [lane][C] and their pixel counts
   float first[kGnMaxChannels];
   float a[kGnMaxChannels], b[kGnMaxChannels], d[kGnMaxChannels];
   float cnt[kGnThreads];  // [warp][pixel lane of the warp]
@@ -381,12 +383,10 @@ struct GnRing {
   __device__ __forceinline__ void prefetch(const GnArgs& a, const GnLanes& ln) {
     for (; ahead < kStages && ahead < nb; ++ahead) issue(a, ln, ahead, (stage + ahead) % kStages);
   }
-  // The chunk's pixels in the ring: begin(a pixel of the thread) once, then f(its 8 channels of x (, of
-  // dy), where they go in `out`, the thread's first vector of the chunk's first pixel); K pixels are
-  // read before their arithmetic.
-  template <int K, typename B, typename F>
-  __device__ __forceinline__ void pixels(const GnArgs& a, const GnLanes& ln, GnSmem& s, T* out, B&& begin,
-                                         F&& f) {
+  // The chunk's pixels in the ring: f(their 8 channels of x (, of dy), where they go in `out`, the thread's
+  // first vector of the chunk's first pixel); K pixels are read before their arithmetic.
+  template <int K, typename F>
+  __device__ __forceinline__ void pixels(const GnArgs& a, const GnLanes& ln, GnSmem& s, T* out, F&& f) {
     prefetch(a, ln);
     const int row = ln.nv * 8 * kEsz, step = ln.wl * row;
     const uint32_t mine = smem_u32(buf) + static_cast<uint32_t>(ln.pl * row + (ln.v - ln.v0) * 8 * kEsz);
@@ -402,11 +402,6 @@ struct GnRing {
         uint32_t p = mine + stage * kGnStage;
         T* o = o0;
         int q = ln.pl;
-        if (i == 0 && q < n) {
-          Gn8<T> t;
-          t.load_shared(p);
-          begin(t);
-        }
         for (; q + (K - 1) * ln.wl < n; q += K * ln.wl) {
           Gn8<T> v[K], d[K];
 #pragma unroll
@@ -475,30 +470,41 @@ __device__ __forceinline__ void gn_lane_store(float* dst, const float2 (&f)[4]) 
   *(reinterpret_cast<float4*>(dst) + 1) = make_float4(f[2].x, f[2].y, f[3].x, f[3].y);
 }
 
-// Statistics of a chunk by group: part[row][g] = (mean - pivot, M2); the pivots are the group's
-// first channel of the image's first pixel.
+// The median of three values of each channel.
+template <typename T>
+__device__ __forceinline__ void gn_medians(const Gn8<T>& a, const Gn8<T>& b, const Gn8<T>& c, float2 (&m)[4]) {
+  float2 x[4], y[4], z[4];
+  a.get(x);
+  b.get(y);
+  c.get(z);
+  auto median = [](float u, float v, float w) { return fmaxf(fminf(u, v), fminf(fmaxf(u, v), w)); };
+#pragma unroll
+  for (int i = 0; i < 4; ++i) m[i] = make_float2(median(x[i].x, y[i].x, z[i].x), median(x[i].y, y[i].y, z[i].y));
+}
+
+// Statistics of a chunk by group: part[row][g] = (mean - pivot, M2); the pivots are the medians of the
+// group's first channel.
 template <typename T, typename Ring>
 __device__ __forceinline__ void gn_stats_sums(const GnArgs& a, const GnPlace& at, const GnLanes& ln,
                                               GnSmem& s, Ring& ring) {
-  if (ln.active && ln.lane_index() == 0) {
-    const GnRun& r = a.run[at.run];
-    Gn8<T> t;
-    float2 f[4];
-    t.load(static_cast<const T*>(r.x) + static_cast<size_t>(at.n) * r.pixels * a.C + ln.v * 8);
-    t.get(f);
-    gn_lane_store(&s.first[ln.v * 8], f);
-  }
-  float2 np[4], s1[4], s2[4];  // minus the thread's first pixel; sums relative to it
+  float2 np[4], s1[4], s2[4];  // minus the medians; sums relative to them
 #pragma unroll
   for (int i = 0; i < 4; ++i) np[i] = s1[i] = s2[i] = both(0.f);
-  ring.template pixels<kGnK * 2 / sizeof(T)>(
-      a, ln, s, static_cast<T*>(nullptr),
-      [&](const Gn8<T>& x) {
-        x.get(np);
+  ring.prefetch(a, ln);
+  if (ln.active) {
+    const GnRun& r = a.run[at.run];
+    const T* image = static_cast<const T*>(r.x) + static_cast<size_t>(at.n) * r.pixels * a.C + ln.v * 8;
+    Gn8<T> t[3];
+    t[0].load(image);
+    t[1].load(image + static_cast<size_t>(r.pixels / 2) * a.C);
+    t[2].load(image + static_cast<size_t>(r.pixels - 1) * a.C);
+    gn_medians(t[0], t[1], t[2], np);
+    if (ln.lane_index() == 0) gn_lane_store(&s.first[ln.v * 8], np);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) np[i] = make_float2(-np[i].x, -np[i].y);
-      },
-      [&](const Gn8<T>& x, const Gn8<T>&, T*) {
+    for (int i = 0; i < 4; ++i) np[i] = make_float2(-np[i].x, -np[i].y);
+  }
+  ring.template pixels<kGnK * 2 / sizeof(T)>(
+      a, ln, s, static_cast<T*>(nullptr), [&](const Gn8<T>& x, const Gn8<T>&, T*) {
         float2 f[4];
         x.get(f);
 #pragma unroll
@@ -777,7 +783,7 @@ __device__ __forceinline__ void gn_apply_chunk(const GnArgs& a, const GnPlace& a
                                                Ring& ring, const GnChannels<kWhole>& ch) {
   const float alpha = a.alpha;
   ring.template pixels<kGnK / sizeof(T)>(
-      a, ln, s, static_cast<T*>(a.run[at.run].y) + at.base + ln.v * 8, [](const Gn8<T>&) {},
+      a, ln, s, static_cast<T*>(a.run[at.run].y) + at.base + ln.v * 8,
       [&](const Gn8<T>& x, const Gn8<T>&, T* y) {
         float2 f[4];
         x.get(f);
@@ -805,7 +811,7 @@ __device__ __forceinline__ void gn_bwd_chunk_sums(const GnArgs& a, const GnPlace
                                                   float2 (&sz)[4], float2 (&sx)[4]) {
   const float alpha = a.alpha;
   ring.template pixels<kGnK / sizeof(T)>(
-      a, ln, s, static_cast<T*>(nullptr), [](const Gn8<T>&) {},
+      a, ln, s, static_cast<T*>(nullptr),
       [&](const Gn8<T>& x, const Gn8<T>& d, T*) {
         float2 f[4], h[4];
         x.get(f);
@@ -940,7 +946,7 @@ __device__ __forceinline__ void gn_bwd_apply_chunk(const GnArgs& a, const GnPlac
                                                    const GnGradient<kWhole>& gr) {
   const float alpha = a.alpha;
   ring.template pixels<kGnK / 2 / sizeof(T)>(
-      a, ln, s, static_cast<T*>(a.run[at.run].y) + at.base + ln.v * 8, [](const Gn8<T>&) {},
+      a, ln, s, static_cast<T*>(a.run[at.run].y) + at.base + ln.v * 8,
       [&](const Gn8<T>& x, const Gn8<T>& d, T* dx) {
         float2 f[4], h[4];
         x.get(f);
@@ -1211,7 +1217,9 @@ __global__ void __launch_bounds__(kGsThreads, 1) gn_small_kernel(const __grid_co
   __syncthreads();
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // (this block has started)
 
-  // The block's mean by group, relative to the group's first value in the block (the pivot).
+  // The block's mean by group, relative to the medians of three pixels of its first piece (that of the group's
+  // first channel: the pivot).
+  const int mid = max(piece - 1, 0) / 2, last = max(min(piece, cnt) - 1, 0);
   bool ok = true;
   float2 acc[4], p[4];
 #pragma unroll
@@ -1219,9 +1227,11 @@ __global__ void __launch_bounds__(kGsThreads, 1) gn_small_kernel(const __grid_co
   for (int i = 0; i * piece < cnt; ++i) {
     ok = mbar_wait(&s.full[i], 0, &s.abort_flag, a.status, kDevTimeoutNorm) && ok;
     if (i == 0) {
-      Gn8<T> f;
-      f.load_shared(mine);
-      f.get(p);
+      Gn8<T> f[3];
+      f[0].load_shared(mine);
+      f[1].load_shared(mine + static_cast<uint32_t>(mid) * row);
+      f[2].load_shared(mine + static_cast<uint32_t>(last) * row);
+      gn_medians(f[0], f[1], f[2], p);
     }
     if (active)
       gn_small_pixels<T>(mine, row, pl, lanes, i * piece, min(cnt, (i + 1) * piece), [&](const Gn8<T>& x, int) {
@@ -1266,16 +1276,21 @@ __global__ void __launch_bounds__(kGsThreads, 1) gn_small_kernel(const __grid_co
     }
     __syncthreads();
   };
+  auto median = [&](int c) {
+    const float u = to_float(first_pixel[c]), v = to_float(first_pixel[mid * a.C + c]),
+                w = to_float(first_pixel[last * a.C + c]);
+    return fmaxf(fminf(u, v), fminf(fmaxf(u, v), w));
+  };
   const float inv_cnt = cnt > 0 ? 1.f / static_cast<float>(cnt) : 0.f;
   const float inv_cg = 1.f / static_cast<float>(a.cg);
   sums(
       [&](int c, float z) {
         if (cnt == 0) return 0.f;
         const int c0 = pow2 ? c & ~(a.cg - 1) : c - c % a.cg;
-        return (to_float(first_pixel[c]) - to_float(first_pixel[c0])) + z * inv_cnt;
+        return (median(c) - median(c0)) + z * inv_cnt;
       },
       [&](int g, float z) {
-        s.pivot[g] = cnt > 0 ? to_float(first_pixel[g * a.cg]) : 0.f;
+        s.pivot[g] = cnt > 0 ? median(g * a.cg) : 0.f;
         s.mean[g] = z * inv_cg;
       });
   // Its squares about that mean.
