@@ -110,6 +110,8 @@ def fpn_lateral_adapters(input: torch.Tensor, weight: torch.Tensor, bias: torch.
         if coarse.dtype is not x.dtype or coarse.dim() != 4 or coarse.shape[0] != n or coarse.shape[1] != 256 \
                 or coarse.device != dev:
             raise ValueError("coarse must match the output's dtype, device, batch and channels")
+        if coarse.numel() == 0:
+            raise ValueError("coarse must not be empty")
         coarse = _cl(coarse)
         hc, wc = coarse.shape[2:]
     count, rank = down.shape[:2]
