@@ -364,7 +364,8 @@ class FPNNeck(torch.nn.Module):
         calls must match the samples' shapes, dtypes and strides, and no output of an eager
         call may still hold its autograd graph while this captures (its gradient-accumulation
         nodes would tie the capture to the default stream).  With ``adapter_index`` the callable is
-        ``f(feats, adapter_index)``, and later calls may pass other indices."""
+        ``f(feats, adapter_index)``, and later calls may pass other indices; without it no image has an
+        adapter, and the adapters get no gradients."""
         module = _Positional(self)
         if adapter_index is not None:
             graphed = torch.cuda.make_graphed_callables(module, (*sample_feats, adapter_index))
@@ -372,7 +373,8 @@ class FPNNeck(torch.nn.Module):
             def run_adapters(feats: Sequence[torch.Tensor], adapter_index: torch.Tensor):
                 return list(graphed(*feats, adapter_index))
             return run_adapters
-        graphed = torch.cuda.make_graphed_callables(module, tuple(sample_feats))
+        # (adapters have no part in a step without an index: no gradients)
+        graphed = torch.cuda.make_graphed_callables(module, tuple(sample_feats), allow_unused_input=self.adapters > 0)
 
         def run(feats: Sequence[torch.Tensor]):
             return list(graphed(*feats))
