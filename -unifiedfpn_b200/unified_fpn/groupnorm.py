@@ -158,8 +158,9 @@ def fpn_group_norm_backward(input, grad_output, mean, rstd, weight=None, bias=No
                             need_input_grad: bool = True):
     """Gradients of :func:`fpn_group_norm` with the ``mean`` and ``rstd`` that it returned:
     ``(grad_input, grad_weight, grad_bias)``; grad_input like the input(s) (None without
-    ``need_input_grad``), the other two fp32 [C] -- summed over the maps where ``weight`` is shared
-    (or None), else a list with one per map.  ``grad_output``: the shapes and dtype of the outputs.
+    ``need_input_grad``), the other two fp32 [C] -- summed over the maps where ``weight`` (for grad_weight)
+    or ``bias`` (for grad_bias) is shared or None, else a list with one per map.  ``grad_output``: the
+    shapes and dtype of the outputs.
     Deterministic (every sum in a fixed order)."""
     if activation not in _ACTIVATIONS:
         raise ValueError(f"unknown activation {activation!r}")
@@ -203,6 +204,5 @@ def fpn_group_norm_backward(input, grad_output, mean, rstd, weight=None, bias=No
         _ACTIVATIONS[activation], alpha, work.data_ptr(), need, _stream(dev)), "ufpn_group_norm_backward")
     if single or shared:
         return (gxs[0] if single and gxs else gxs), gw[0], gb[0]
-    # a parameter shared by the maps beside one that is not: its gradient is the sum over the maps
-    return (gxs, torch.stack(gw).sum(0) if shared_w and weight is not None else gw,
-            torch.stack(gb).sum(0) if shared_b and bias is not None else gb)
+    # a parameter shared by the maps (or None) beside one that is not: its gradient is the sum over the maps
+    return gxs, torch.stack(gw).sum(0) if shared_w else gw, torch.stack(gb).sum(0) if shared_b else gb
