@@ -1559,6 +1559,47 @@ cudaError_t gn_run(const GnSchedule& sc, const GnArgs& a, const GroupNormLevel* 
   return e == cudaSuccess ? gn_sum_rows(sc, a, lv, levels, s) : e;
 }
 
+template <typename K>
+cudaError_t gn_small_attributes(K kernel) {
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             kGsDataOffset + static_cast<int>(kGsMaxShare));
+  return e != cudaSuccess ? e : cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+}
+// Whether the current device can hold a cluster of 2^log_blocks of the small kernel's blocks with the largest
+// share (a part of a GPU may have no 16 SMs in one cluster's reach).  One answer for all its types: every
+// block takes an SM.  Without an answer: yes, and the launch tells.
+bool gn_small_fits(int log_blocks) {
+  static std::atomic<int> known[64][5];  // 0: not asked yet, 1: no, 2: yes
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) {
+    cudaGetLastError();
+    return true;
+  }
+  int answer = known[dev][log_blocks].load(std::memory_order_relaxed);
+  if (answer == 0) {
+    const auto kernel = gn_small_kernel<__nv_bfloat16, true>;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(1u << log_blocks);
+    cfg.blockDim = dim3(kGsThreads);
+    cfg.dynamicSmemBytes = kGsDataOffset + static_cast<size_t>(kGsMaxShare);
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 1u << log_blocks;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int clusters = 0;
+    if (gn_small_attributes(kernel) != cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg) != cudaSuccess) {
+      cudaGetLastError();
+      return true;
+    }
+    answer = clusters > 0 ? 2 : 1;
+    known[dev][log_blocks].store(answer, std::memory_order_relaxed);
+  }
+  return answer == 2;
+}
+
 // The small kernel's cluster size for these maps, 0 where it does not apply: shares of about 16 KB (8 and
 // 32 KB measure the same), in one wave of clusters.  (A cluster's SMs lie in one GPC, so that not all 148
 // can be used: 16 clusters of 8 took two waves, 18.5 us against 10.4 us for 8 of them.)  Against the
@@ -1575,18 +1616,16 @@ int gn_small_blocks(DType dt, int levels, int N, int C, const long long* pixels,
   int blocks = 1;
   while (blocks < kGsMaxCluster && (most + blocks - 1) / blocks * row > (16 << 10)) blocks *= 2;
   while (blocks > 1 && items * blocks > (blocks >= 8 ? 64 : 128)) blocks /= 2;
+  int log_blocks = 0;
+  while ((1 << log_blocks) < blocks) ++log_blocks;
+  while (log_blocks > 0 && !gn_small_fits(log_blocks)) blocks = 1 << --log_blocks;
   return (most + blocks - 1) / blocks * row <= kGsMaxShare ? blocks : 0;
 }
 template <typename T, bool kWhole>
 cudaError_t gn_small_launch(GnArgs& a, int levels, int blocks, cudaStream_t s) {
   const auto kernel = gn_small_kernel<T, kWhole>;
   static std::atomic<bool> configured[64];
-  const cudaError_t e = once_per_device(configured, [&] {
-    const cudaError_t f =
-        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             kGsDataOffset + static_cast<int>(kGsMaxShare));
-    return f != cudaSuccess ? f : cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-  });
+  const cudaError_t e = once_per_device(configured, [&] { return gn_small_attributes(kernel); });
   if (e != cudaSuccess) return e;
   int share = 0, log_blocks = 0;
   while ((1 << log_blocks) < blocks) ++log_blocks;
