@@ -1001,9 +1001,13 @@ int ufpn_lateral_adapters_parts(int dtype, const void* x, const void* w, const f
 
 size_t ufpn_lateral_adapters_workspace(int dtype, int N, int Cin, int H, int W, int rank,
                                        int adapters, int has_w_t, int need_grad_x) {
-  ufpn::AdapterProblem p;
-  if (adapter_problem(dtype, N, Cin, H, W, rank, adapters, nullptr, nullptr, 1.f, 3, &p) != UFPN_OK) return 0;
-  return ufpn::lateral_adapters_workspace_bytes(p, has_w_t != 0, need_grad_x != 0);
+  try {
+    ufpn::AdapterProblem p;
+    if (adapter_problem(dtype, N, Cin, H, W, rank, adapters, nullptr, nullptr, 1.f, 3, &p) != UFPN_OK) return 0;
+    return ufpn::lateral_adapters_workspace_bytes(p, has_w_t != 0, need_grad_x != 0);
+  } catch (...) {
+    return 0;
+  }
 }
 
 int ufpn_lateral_adapters_backward(int dtype, const void* x, const void* w, const void* w_t,
