@@ -42,10 +42,12 @@ namespace {
 constexpr int kAdMaxRank = 64;
 // TMA warp, MMA warp, 16 epilogue warps: what the epilogue does for a tile is one long chain of
 // instructions, so that twice the warps halve its time (8 warps: about 6000 cycles a tile).  On P2 of eight
-// images, 142 us, a tile takes 10000 cycles: h and its parts 2000, the last MMA and the accumulators' reading
+// images, 144 us, a tile takes 10000 cycles: h and its parts 2000, the last MMA and the accumulators' reading
 // 1500, stores 4700, the next top-down weights 1200.  Four more warps that make h and those weights while
 // the others store took 154 us (118 instead of 122 without a top-down add): the k-loop then waits for
-// loads, x from HBM and the 128 KB of weights that every tile reads again from L2.
+// loads, x from HBM and the 128 KB of weights that every tile reads again from L2.  (These times and the others
+// of P2 in this file are of the same maps pass after pass, of which L2 keeps a part: a call whose maps are
+// new takes 156 to 167 us, and choices that lie a few percent apart were not compared there.)
 constexpr int kAdEpiWarps = 16;
 constexpr int kAdThreads = 64 + 32 * kAdEpiWarps;
 constexpr int kAdWarpCols = kTcBlockN / (kAdEpiWarps / 4);  // output channels of a warp
@@ -74,7 +76,8 @@ __device__ __forceinline__ uint32_t row_chunk(int row, int chunk) {
 }
 
 // Shared memory of fpn_adapter_kernel for ranks up to RP.  (Keeping 256 x 256 weights resident instead
-// of streaming them with every tile changed nothing: 148 against 146 us on P2 of eight images.)
+// of streaming them with every tile changed nothing: 148 against 146 us on P2 of eight images, the same
+// maps pass after pass.)
 template <int RP, int kParts, bool kTaps>
 struct AdCfg {
   static constexpr int kRow = RP * 2;   // bytes of a row of h or up

@@ -298,7 +298,8 @@ class FPNNeck(torch.nn.Module):
     level; P6 comes from the normed P5.  ``adapters``: that many low-rank adapters of ``adapter_rank`` on
     every lateral (``adapter_down`` [L, R, Cin], ``adapter_up`` [L, 256, R], zero at first), scaled by
     ``adapter_scale``; ``forward`` then takes an adapter index per image.  To train adapters and norms
-    alone, switch the other parameters' requires_grad off: their gradients are then not computed."""
+    alone, switch the other parameters' requires_grad off: with an adapter index their gradients are then
+    not computed (without one the whole plain backward runs as soon as any of it is needed)."""
 
     def __init__(self, in_channels: Sequence[int] = (256, 512, 1024, 2048), out_channels: int = 256,
                  return_p6: bool = True, seed: int = 0, norm_groups: int | None = None,
