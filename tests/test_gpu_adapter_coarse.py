@@ -112,3 +112,32 @@ def test_many_tiles_with_and_without(cuda_device):
     assert _beside(out, clean, args, coarse, ~used)
     torch.cuda.synchronize()
     assert U.device_status() == 0
+
+
+def test_graph_replay_and_streams(cuda_device):
+    """A captured call on coarse maps that come and go with such values, and two calls at once."""
+    import unified_fpn as U
+    args, coarse = _inputs(cuda_device, torch.bfloat16, (101, 67, 51, 34, 64), 16)
+    dirty = coarse.clone(memory_format=torch.preserve_format)
+    dirty[:, 3, 20, 20] = float("nan")
+    want = [U.fpn_lateral_adapters(*args, coarse=c) for c in (coarse, dirty)]
+    assert not want[1].isfinite().all() and want[0].isfinite().all()
+    same = lambda a, b: torch.equal(a.view(torch.int16), b.view(torch.int16))  # noqa: E731
+    static = coarse.clone(memory_format=torch.preserve_format)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = U.fpn_lateral_adapters(*args, coarse=static)
+    for k in (1, 0, 1, 1, 0):
+        static.copy_((coarse, dirty)[k])
+        graph.replay()
+        torch.cuda.synchronize()
+        assert same(out, want[k]), k
+    streams = [torch.cuda.Stream(cuda_device) for _ in range(2)]
+    got = []
+    for _ in range(8):
+        for k, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got.append((k, U.fpn_lateral_adapters(*args, coarse=(coarse, dirty)[k])))
+    torch.cuda.synchronize()
+    assert all(same(o, want[k]) for k, o in got)
+    assert U.device_status() == 0
