@@ -24,6 +24,7 @@ import ctypes
 from typing import Sequence
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._lib import check, lib
@@ -224,6 +225,7 @@ class _NormFunction(torch.autograd.Function):
         return (*outs, fpn_p6(outs[3])) if return_p6 else tuple(outs)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, *grads):
         t = ctx.saved_tensors
         maps, mean, rstd, w, b = (list(t[i:i + 4]) for i in range(0, 20, 4))
@@ -255,6 +257,7 @@ class _AdapterNeckFunction(torch.autograd.Function):
         return (*outs, fpn_p6(outs[3])) if return_p6 else tuple(outs)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, *grads):
         t = ctx.saved_tensors
         index = t[0]
